@@ -24,6 +24,7 @@ enum : int {
   kStatusPeerFlagTimeout = 4,
   kStatusBadArgument = 5,
   kStatusBoundsViolation = 6,  // debug builds (-DOSLO_DEBUG_BOUNDS): an index left its buffer; the access was skipped
+  kStatusPageRange = 7,  // paged cache: a page, position or length outside its pool or table; the access was skipped
 };
 
 // Debug bounds checks.  With -DOSLO_DEBUG_BOUNDS (python -m oslo_b200.csrc.build --debug-bounds; OSLO_B200_DEBUG_BOUNDS=1

@@ -12,8 +12,10 @@ from oslo_b200.ops.activation import (  # noqa: F401
     swiglu,
 )
 from oslo_b200.ops.attention import attention, qkv_attention  # noqa: F401
+from oslo_b200.ops.logits import pack_token_mask, process_logits  # noqa: F401
 from oslo_b200.ops.norm import layer_norm as fused_layer_norm  # noqa: F401
 from oslo_b200.ops.norm import rms_norm as fused_rms_norm  # noqa: F401
+from oslo_b200.ops.paged import paged_attention, paged_kv_append  # noqa: F401
 from oslo_b200.ops.softmax import apply_rope, rope_tables, scale_mask_softmax  # noqa: F401
 
 

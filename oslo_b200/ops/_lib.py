@@ -123,5 +123,6 @@ def check_status(device=None) -> None:
     if code != 0:
         status_word(device).zero_()
         names = {1: "TMA producer wait", 2: "MMA wait", 3: "epilogue wait", 4: "peer flag wait", 5: "bad argument",
-                 6: "index out of bounds (debug build; the access was skipped)"}
+                 6: "index out of bounds (debug build; the access was skipped)",
+                 7: "paged cache: page, position or length out of range (the access was skipped)"}
         raise RuntimeError(f"oslo_b200 kernel reported status {code} ({names.get(code, 'unknown')})")

@@ -1,0 +1,156 @@
+"""Penalties for repeated tokens, biases and grammar masks on next-token logits (``csrc/logits_sm100a.cu``).
+
+``process_logits(logits, tokens, ...)`` changes the logits of one decoding step before a token is picked from them;
+``pack_token_mask(mask)`` packs a boolean mask of allowed tokens into the 32-bit words that it takes.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Union
+
+import torch
+
+from . import _lib
+
+_DT = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def pack_token_mask(mask: torch.Tensor) -> torch.Tensor:
+    """Boolean ``[rows, vocab]`` (true = allowed) -> int32 ``[rows, ceil(vocab / 32)]``; token ``j`` is bit ``j % 32`` of word
+    ``j // 32``."""
+    if mask.dim() != 2 or mask.dtype != torch.bool:
+        raise ValueError(f"mask is boolean [rows, vocab]: got {mask.dtype} {tuple(mask.shape)}")
+    rows, v = mask.shape
+    bits = torch.nn.functional.pad(mask, (0, -v % 32)).view(rows, -1, 32).long()
+    words = (bits << torch.arange(32, device=mask.device)).sum(-1)
+    return torch.where(words >= 1 << 31, words - (1 << 32), words).to(torch.int32)
+
+
+def _per_row(name, p, rows: int, device):
+    """(tensor or None, scalar) of a penalty given as a number or as one number a row."""
+    if isinstance(p, torch.Tensor):
+        if p.shape != (rows,) or p.device != device or not p.is_floating_point():
+            raise ValueError(f"{name} is a number or a floating tensor [{rows}] on {device}: got {p.dtype} {tuple(p.shape)} on {p.device}")
+        return p.float().contiguous(), 0.0
+    return None, float(p)
+
+
+def process_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, token_lengths: Optional[torch.Tensor] = None,
+                   prompt_lengths: Optional[torch.Tensor] = None, repetition_penalty: Union[float, torch.Tensor] = 1.0,
+                   presence_penalty: Union[float, torch.Tensor] = 0.0, frequency_penalty: Union[float, torch.Tensor] = 0.0,
+                   bias: Optional[torch.Tensor] = None, allowed: Optional[torch.Tensor] = None,
+                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Next-token ``logits [rows, vocab]`` after penalties, biases and a grammar mask, in this order:
+
+    1. a token that occurs in the row's history has its logit ``x`` divided by ``repetition_penalty`` (multiplied where ``x`` is
+       not positive);
+    2. a token that was generated ``c > 0`` times loses ``presence_penalty + frequency_penalty * c``;
+    3. ``bias`` is added;
+    4. tokens that are not ``allowed`` become ``-inf``.
+
+    ``tokens``: int64 or int32 ``[rows, length]``, the history; ids outside the vocabulary are ignored.  ``token_lengths``: int32
+    ``[rows]``, how many of them count (``None``: all).  ``prompt_lengths``: int32 ``[rows]``, how many of those are the prompt, not
+    generated (``None``: none).  The penalties are numbers or floating tensors ``[rows]``.  ``bias``: ``[vocab]`` or ``[rows, vocab]``.
+    ``allowed``: int32 ``[rows or 1, ceil(vocab / 32)]`` from :func:`pack_token_mask`; a row that allows nothing is all ``-inf``.
+    The result is a new tensor, or ``out`` (which may be ``logits``).  For inference: no gradient.
+    """
+    if logits.dim() != 2 or logits.dtype not in _DT:
+        raise ValueError(f"logits are float32, float16 or bfloat16 [rows, vocab]: got {logits.dtype} {tuple(logits.shape)}")
+    if torch.is_grad_enabled() and (logits.requires_grad or (bias is not None and bias.requires_grad)):
+        raise RuntimeError("process_logits is for inference: call it under torch.no_grad() or detach its inputs")
+    rows, v = logits.shape
+    dev = logits.device
+    rep, rep_s = _per_row("repetition_penalty", repetition_penalty, rows, dev)
+    pres, pres_s = _per_row("presence_penalty", presence_penalty, rows, dev)
+    freq, freq_s = _per_row("frequency_penalty", frequency_penalty, rows, dev)
+    if rep is None and not rep_s > 0:
+        raise ValueError(f"repetition_penalty is positive: got {rep_s}")
+    if tokens is None:
+        if token_lengths is not None or prompt_lengths is not None:
+            raise ValueError("token_lengths and prompt_lengths describe tokens, which are missing")
+        if rep is not None or pres is not None or freq is not None or rep_s != 1.0 or pres_s or freq_s:
+            raise ValueError("the penalties need the tokens of each row's history")
+    else:
+        if tokens.dim() != 2 or tokens.shape[0] != rows or tokens.dtype not in (torch.int64, torch.int32) or tokens.device != dev:
+            raise ValueError(f"tokens are int64 or int32 [{rows}, length] on {dev}: got {tokens.dtype} {tuple(tokens.shape)} on "
+                             f"{tokens.device}")
+        for name, t in (("token_lengths", token_lengths), ("prompt_lengths", prompt_lengths)):
+            if t is not None and (t.dtype != torch.int32 or t.shape != (rows,) or t.device != dev or not t.is_contiguous()):
+                raise ValueError(f"{name} is a contiguous int32 tensor [{rows}] on {dev}: got {t.dtype} {tuple(t.shape)} on {t.device}")
+    if bias is not None:
+        if bias.shape not in ((v,), (rows, v)) or not bias.is_floating_point() or bias.device != dev:
+            raise ValueError(f"bias is a floating tensor [{v}] or [{rows}, {v}] on {dev}: got {bias.dtype} {tuple(bias.shape)} on "
+                             f"{bias.device}")
+        bias = bias.float()
+    if allowed is not None and (allowed.dtype != torch.int32 or allowed.dim() != 2 or allowed.shape[0] not in (1, rows)
+                                or allowed.shape[1] != (v + 31) // 32 or allowed.device != dev):
+        raise ValueError(f"allowed is int32 [{rows} or 1, {(v + 31) // 32}] on {dev}: got {allowed.dtype} {tuple(allowed.shape)} on "
+                         f"{allowed.device}")
+    if out is not None and (out.shape != logits.shape or out.dtype != logits.dtype or out.device != dev or out.stride(1) != 1):
+        raise ValueError(f"out is like the logits, with contiguous rows: got {out.dtype} {tuple(out.shape)} on {out.device}")
+    if not logits.is_cuda:
+        y = _reference(logits, tokens, token_lengths, prompt_lengths, *(t if t is not None else s for t, s in
+                       ((rep, rep_s), (pres, pres_s), (freq, freq_s))), bias, allowed)
+        return y if out is None else out.copy_(y)
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return process_logits(logits, tokens, token_lengths, prompt_lengths, repetition_penalty, presence_penalty,
+                                  frequency_penalty, bias, allowed, out)
+    if logits.stride(1) != 1:
+        logits = logits.contiguous()
+    y = torch.empty(rows, v, dtype=logits.dtype, device=dev) if out is None else out
+    length = 0
+    if tokens is not None:
+        tokens = tokens if tokens.stride(1) == 1 else tokens.contiguous()
+        length = tokens.shape[1]
+    if bias is not None and bias.stride(-1) != 1:
+        bias = bias.contiguous()
+    if allowed is not None and allowed.stride(1) != 1:
+        allowed = allowed.contiguous()
+    p = lambda t: t.data_ptr() if t is not None else None
+    rc = _fn()(
+        logits.data_ptr(), y.data_ptr(), p(tokens) if length else None, p(token_lengths), p(prompt_lengths), p(rep), p(pres), p(freq),
+        p(bias), p(allowed), logits.stride(0), y.stride(0), tokens.stride(0) if length else 0,
+        bias.stride(0) if bias is not None and bias.dim() == 2 else 0,
+        allowed.stride(0) if allowed is not None and allowed.shape[0] == rows else 0, rep_s, pres_s, freq_s, rows, v, length,
+        1 if length and tokens.dtype == torch.int64 else 0, _DT[logits.dtype], _raw_stream(dev.index))
+    if rc:
+        raise RuntimeError(f"oslo_process_logits failed ({rc})")
+    return y
+
+
+_native = None
+
+
+def _fn():
+    global _native
+    if _native is None:
+        lib = _lib.cuda_lib()
+        P, L, F, I = ctypes.c_void_p, ctypes.c_longlong, ctypes.c_float, ctypes.c_int
+        _lib._load_cuda_lib().oslo_process_logits.argtypes = [P] * 10 + [L] * 5 + [F] * 3 + [I] * 5 + [P]
+        _native = lib.oslo_process_logits
+    return _native
+
+
+def _reference(logits, tokens, token_lengths, prompt_lengths, rep, pres, freq, bias, allowed):
+    x = logits.float()
+    rows, v = x.shape
+    col = lambda p: p[:, None] if isinstance(p, torch.Tensor) else p
+    if tokens is not None and tokens.shape[1]:
+        t = torch.arange(tokens.shape[1], device=x.device)
+        known = (tokens >= 0) & (tokens < v)
+        if token_lengths is not None:
+            known &= t < token_lengths[:, None]
+        made = known if prompt_lengths is None else known & (t >= prompt_lengths[:, None])
+        ids = tokens.long().clamp(0, v - 1)
+        seen = torch.zeros_like(x).scatter_add_(1, ids, known.float()) > 0
+        c = torch.zeros_like(x).scatter_add_(1, ids, made.float())
+        x = torch.where(seen, torch.where(x > 0, x / col(rep), x * col(rep)), x)
+        x = torch.where(c > 0, x - col(pres) - col(freq) * c, x)
+    if bias is not None:
+        x = x + bias
+    if allowed is not None:
+        j = torch.arange(v, device=x.device)
+        x = x.masked_fill(((allowed[:, j // 32] >> (j % 32).to(torch.int32)) & 1) == 0, float("-inf"))
+    return x.to(logits.dtype)

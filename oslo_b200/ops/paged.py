@@ -1,0 +1,268 @@
+"""Paged key / value cache for serving (``csrc/paged_cache_sm100a.cu``, ``csrc/paged_attention_sm100a.cu``).
+
+Keys and values live in pools ``[pages, kv_heads, page_size, head_dim]``; ``block_table[b, j]`` is the page that holds tokens
+``j * page_size ..`` of sequence ``b``, so sequences of any lengths share one pool and grow without being copied.
+
+``paged_kv_append``   rotates new queries and keys by their positions and stores keys and values in their pages, one pass
+``paged_attention``   softmax attention of the newest tokens over the pages
+``PagedDecodeCache``  the paged counterpart of :class:`oslo_b200.ops.attention.DecodeCache`: pages are taken from a free list as
+                      sequences grow, and the sequences of a batch may have different lengths
+
+The functions are for inference: inputs that require a gradient are refused.  On the GPU a page, position or length outside
+its pool or table is skipped by the kernel and reported by ``oslo_b200.ops._lib.check_status()``; on the CPU it raises.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import List, Optional, Sequence
+
+import torch
+
+from . import _lib
+
+_DT = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+MAX_HEAD_DIM = 256
+
+
+def _check_pages(k_pages, v_pages, block_table, b: int, hd: int, dtype, device):
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
+        raise ValueError(f"k_pages and v_pages are [pages, kv_heads, page_size, head_dim], both alike: got {tuple(k_pages.shape)} "
+                         f"and {tuple(v_pages.shape)}")
+    pages, hkv, page, d = k_pages.shape
+    if dtype not in _DT or k_pages.dtype != dtype or v_pages.dtype != dtype:
+        raise ValueError(f"queries, keys, values and pages share one of float32, float16, bfloat16: got {dtype}, {k_pages.dtype}, "
+                         f"{v_pages.dtype}")
+    if d != hd:
+        raise ValueError(f"head_dim of the pages is {d}, of the tokens {hd}")
+    if page == 0 or page % 16 or d == 0 or d % 8 or d > MAX_HEAD_DIM or hkv == 0:
+        raise ValueError(f"page_size is a multiple of 16 and head_dim a multiple of 8 up to {MAX_HEAD_DIM}: got {page}, {d} "
+                         f"({hkv} key heads)")
+    for t in (k_pages, v_pages):
+        st = t.stride()
+        if st[3] != 1 or st[2] != d or st[0] % 8 or st[1] % 8 or t.data_ptr() % 16:
+            raise ValueError("the tokens of a head inside a page are contiguous, and pages and heads start on 16-byte boundaries")
+        if t.device != device:
+            raise ValueError(f"tensors are on {device} and {t.device}")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != b or block_table.stride(1) != 1:
+        raise ValueError(f"block_table is int32 [{b}, pages per sequence] with contiguous rows: got {block_table.dtype} "
+                         f"{tuple(block_table.shape)}")
+    if block_table.device != device:
+        raise ValueError(f"tensors are on {device} and {block_table.device}")
+    if block_table.shape[1] * page > 0x3FFFFFFF:
+        raise ValueError("block_table spans more than 2**30 tokens")
+
+
+def _check_ints(name, t, b: int, device):
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != b or not t.is_contiguous() or t.device != device:
+        raise ValueError(f"{name} is a contiguous int32 tensor [{b}] on {device}: got {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def _no_grad(*tensors):
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError("the paged cache is for inference: call it under torch.no_grad() or detach its inputs")
+
+
+def _aligned(t):
+    """``t`` with unit inner stride and 16-byte aligned heads (a copy where it has not)."""
+    st = t.stride()
+    n = 16 // t.element_size()
+    if st[3] == 1 and not (st[0] % n or st[1] % n or st[2] % n or t.data_ptr() % 16):
+        return t
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def paged_kv_append(k, v, k_pages, v_pages, block_table, start, count=None, q=None, rope=None):
+    """Store new tokens in the paged cache, rotated by their positions.
+
+    ``k``, ``v``: ``[b, s, kv_heads, head_dim]`` (any strides), token ``i`` of sequence ``b`` has position ``start[b] + i``.
+    ``start``: int32 ``[b]``, the tokens that each sequence holds already.  ``count``: int32 ``[b]``, how many of the ``s`` tokens
+    are real (the rest is padding and is not stored; ``None``: all).  ``rope = (cos, sin, rot_dim, neox)`` as for
+    :func:`oslo_b200.ops.attention.qkv_attention` rotates keys and queries; the tables need a row for every position.
+    Pages are written in place, everything else in them stays; two tokens with the same page and row are a mistake of the
+    caller (either may be stored).
+
+    Returns the rotated ``q`` ``[b, s, heads, head_dim]`` as a new tensor (rows of padding are zeros), or ``None`` without ``q``.
+    """
+    if k.dim() != 4 or k.shape != v.shape or v.dtype != k.dtype or v.device != k.device:
+        raise ValueError(f"k and v are [b, s, kv_heads, head_dim], both alike: got {tuple(k.shape)} {k.dtype} and {tuple(v.shape)} "
+                         f"{v.dtype}")
+    b, s, hkv, hd = k.shape
+    dev = k.device
+    _no_grad(k, v, q, k_pages, v_pages)
+    _check_pages(k_pages, v_pages, block_table, b, hd, k.dtype, dev)
+    if k_pages.shape[1] != hkv:
+        raise ValueError(f"the pages hold {k_pages.shape[1]} key heads, the tokens {hkv}")
+    _check_ints("start", start, b, dev)
+    if count is not None:
+        _check_ints("count", count, b, dev)
+    if q is not None and (q.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != hd or q.dtype != k.dtype or q.device != dev):
+        raise ValueError(f"q is [{b}, {s}, heads, {hd}] {k.dtype} on {dev}: got {tuple(q.shape)} {q.dtype} on {q.device}")
+    cos = sin = None
+    rot, neox = 0, True
+    if rope is not None:
+        cos, sin, rot, neox = rope
+        if rot < 0 or rot % 2 or rot > hd:
+            raise ValueError(f"rot_dim is even and at most {hd}: got {rot}")
+        for t in (cos, sin):
+            if t.dtype != torch.float32 or t.dim() != 2 or t.shape != cos.shape or t.shape[1] != rot // 2 or not t.is_contiguous() \
+                    or t.device != dev:
+                raise ValueError(f"the rotation's tables are contiguous float32 [positions, {rot // 2}] on {dev}: got {t.dtype} "
+                                 f"{tuple(t.shape)} on {t.device}")
+    if not k.is_cuda:
+        return _append_reference(k, v, k_pages, v_pages, block_table, start, count, q, rope if rot else None)
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return paged_kv_append(k, v, k_pages, v_pages, block_table, start, count, q, rope)
+    k, v = _aligned(k), _aligned(v)
+    hq, out, qs = 0, None, (0, 0, 0)
+    if q is not None:
+        q = _aligned(q)
+        hq, qs = q.shape[2], q.stride()[:3]
+        out = torch.empty(b, s, hq, hd, dtype=q.dtype, device=dev)
+    strides = (ctypes.c_longlong * 14)(*qs, *k.stride()[:3], *v.stride()[:3], *k_pages.stride()[:2], *v_pages.stride()[:2],
+                                       block_table.stride(0))
+    rc = _fn("oslo_paged_kv_append", _APPEND_ARGS)(
+        q.data_ptr() if hq else None, k.data_ptr(), v.data_ptr(), out.data_ptr() if hq else None, k_pages.data_ptr(), v_pages.data_ptr(),
+        block_table.data_ptr(), start.data_ptr(), count.data_ptr() if count is not None else None, cos.data_ptr() if rot else None,
+        sin.data_ptr() if rot else None, strides, b, s, hq, hkv, hd, rot, 1 if neox else 0, cos.shape[0] if rot else 0,
+        k_pages.shape[2], block_table.shape[1], k_pages.shape[0], _DT[k.dtype], _lib.status_word(dev).data_ptr(),
+        _raw_stream(dev.index))
+    if rc:
+        raise RuntimeError(f"oslo_paged_kv_append failed ({rc})")
+    return out
+
+
+def paged_attention(q, k_pages, v_pages, block_table, lengths, scale: Optional[float] = None, mask=None):
+    """Attention of the newest tokens over a paged cache.
+
+    ``q``: ``[b, s, heads, head_dim]`` (any strides), the newest ``s`` tokens of each sequence; their keys and values are in the
+    pages already.  ``lengths``: int32 ``[b]``, the tokens in each sequence, the new ones included: query ``i`` sees the first
+    ``lengths[b] - s + 1 + i``.  ``heads`` is a multiple of the pages' ``kv_heads``; consecutive heads share one.
+    ``mask``: additive, ``[b or 1, 1, s or 1, tokens]``, any floating type; tokens at ``-inf`` take no part, whatever they hold,
+    nor does what lies behind a sequence's last token.  It covers the longest sequence.  A query that sees nothing gives zeros.
+
+    Returns ``[b, s, heads * head_dim]``, like :func:`oslo_b200.ops.attention.attention`.
+    """
+    if q.dim() != 4:
+        raise ValueError(f"q is [b, s, heads, head_dim]: got {tuple(q.shape)}")
+    b, s, hq, hd = q.shape
+    dev = q.device
+    _no_grad(q, k_pages, v_pages, mask)
+    _check_pages(k_pages, v_pages, block_table, b, hd, q.dtype, dev)
+    _check_ints("lengths", lengths, b, dev)
+    hkv = k_pages.shape[1]
+    if hq == 0 or hq % hkv:
+        raise ValueError(f"{hq} query heads do not share {hkv} key heads evenly")
+    scale = float(scale) if scale is not None else 1.0 / math.sqrt(hd)
+    if not math.isfinite(scale):
+        raise ValueError(f"scale is a finite number: got {scale}")
+    if mask is not None:
+        if mask.dim() != 4 or mask.shape[0] not in (1, b) or mask.shape[1] != 1 or mask.shape[2] not in (1, s) or mask.device != dev \
+                or not mask.is_floating_point():
+            raise ValueError(f"mask is an additive floating tensor [{b} or 1, 1, {s} or 1, tokens] on {dev}: got {mask.dtype} "
+                             f"{tuple(mask.shape)} on {mask.device}")
+        mask = mask.float()
+    if not q.is_cuda:
+        return _attention_reference(q, k_pages, v_pages, block_table, lengths, scale, mask)
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return paged_attention(q, k_pages, v_pages, block_table, lengths, scale, mask)
+    q = _aligned(q)
+    out = torch.empty(b, s, hq * hd, dtype=q.dtype, device=dev)
+    ms, mlen = (0, 0), 0
+    if mask is not None:
+        mask = mask.expand(b, 1, s, mask.shape[3])
+        if mask.stride(3) != 1:
+            mask = mask.contiguous()
+        ms, mlen = (mask.stride(0), mask.stride(2)), mask.shape[3]
+    strides = (ctypes.c_longlong * 10)(*q.stride()[:3], *k_pages.stride()[:2], *v_pages.stride()[:2], block_table.stride(0), *ms)
+    rc = _fn("oslo_paged_attention", _ATTEND_ARGS)(
+        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), lengths.data_ptr(),
+        mask.data_ptr() if mask is not None else None, out.data_ptr(), strides, b, s, hkv, hq // hkv, hd, k_pages.shape[2],
+        block_table.shape[1], k_pages.shape[0], mlen, scale, _DT[q.dtype], _lib.status_word(dev).data_ptr(), _raw_stream(dev.index))
+    if rc:
+        raise RuntimeError(f"oslo_paged_attention failed ({rc})")
+    return out
+
+
+_P, _I, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
+_APPEND_ARGS = [_P] * 12 + [_I] * 12 + [_P, _P]
+_ATTEND_ARGS = [_P] * 8 + [_I] * 9 + [_F, _I, _P, _P]
+_fns = {}
+
+
+def _fn(name, argtypes):
+    """The library's entry point with its argument types set, so that ctypes converts plain numbers."""
+    fn = _fns.get(name)
+    if fn is None:
+        lib = _lib.cuda_lib()
+        getattr(_lib._load_cuda_lib(), name).argtypes = argtypes
+        fn = _fns[name] = getattr(lib, name)
+    return fn
+
+
+# ------------------------------------------------------------------------------------------------ plain forms
+def _rows_of(block_table, page: int, pages: int, row: int, n: int):
+    """Page and row in it of tokens ``0 .. n`` of one sequence."""
+    if n > block_table.shape[1] * page:
+        raise ValueError(f"sequence {row} has {n} tokens, its row of the block table holds {block_table.shape[1] * page}")
+    t = torch.arange(n, device=block_table.device)
+    where = block_table[row].long()[t // page]
+    if n and (int(where.min()) < 0 or int(where.max()) >= pages):
+        raise ValueError(f"block_table names a page outside the pool of {pages}")
+    return where, t % page
+
+
+def _append_reference(k, v, k_pages, v_pages, block_table, start, count, q, rope):
+    from .softmax import rope_reference
+
+    b, s = k.shape[:2]
+    pages, _, page, _ = k_pages.shape
+    out = torch.zeros(q.shape, dtype=q.dtype, device=q.device) if q is not None else None
+    for r in range(b):
+        first, n = int(start[r]), s if count is None else max(0, min(s, int(count[r])))
+        if first < 0 or (n and rope is not None and first + n > rope[0].shape[0]):
+            raise ValueError(f"sequence {r} has positions {first} to {first + n}, the rotation's tables do not")
+        where, at = (t[first:] for t in _rows_of(block_table, page, pages, r, first + n)) if n else (None, None)
+        if not n:
+            continue
+        turn = lambda x: x
+        if rope is not None:
+            cos, sin, rot, neox = rope
+            pos = torch.arange(first, first + n, device=k.device)
+            turn = lambda x: rope_reference(x, cos, sin, rot, neox, positions=pos)
+        k_pages[where, :, at] = turn(k[r, :n])
+        v_pages[where, :, at] = v[r, :n]
+        if out is not None:
+            out[r, :n] = turn(q[r, :n])
+    return out
+
+
+def _attention_reference(q, k_pages, v_pages, block_table, lengths, scale, mask):
+    b, s, hq, hd = q.shape
+    pages, hkv, page, _ = k_pages.shape
+    out = torch.zeros(b, s, hq, hd, dtype=torch.float32, device=q.device)
+    for r in range(b):
+        n = max(0, int(lengths[r]))
+        if mask is not None and n > mask.shape[3]:
+            raise ValueError(f"the mask covers {mask.shape[3]} tokens, sequence {r} has {n}")
+        where, at = _rows_of(block_table, page, pages, r, n)
+        k, v = (t[where, :, at].float().repeat_interleave(hq // hkv, dim=1) for t in (k_pages, v_pages))  # [n, hq, hd]
+        for i in range(s):
+            end = n - s + 1 + i
+            if end <= 0:
+                continue
+            x = torch.einsum("hd,nhd->hn", q[r, i].float(), k[:end]) * scale
+            vv = v[:end]
+            if mask is not None:
+                add = mask[r % mask.shape[0], 0, i % mask.shape[2], :end]
+                keep = add != float("-inf")
+                x, vv = (x + add)[:, keep], vv[keep]
+            if x.shape[1]:
+                out[r, i] = torch.einsum("hn,nhd->hd", torch.softmax(x, dim=-1), vv)
+    return out.to(q.dtype).view(b, s, hq * hd)
