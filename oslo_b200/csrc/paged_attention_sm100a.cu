@@ -4,8 +4,15 @@
 //   gives zeros.
 //
 // Every key and value is used by `group` query heads only, so HBM bounds it: 4 * head_dim bytes a token and key head against
-// 4 * group * head_dim operations.  A block of four warps takes one (query token, key head); each warp walks 16-token tiles
-// (8 for fp32) with its own running maximum, sum and output, and the four are joined at the end.
+// 4 * group * head_dim operations.
+//
+// Work is cut into units of 64 tokens (32 for fp32) of one (query token, key head, block of query heads), a "segment" being all
+// units of one such triple.  As many blocks as the GPU holds at once take equal, contiguous ranges of units, found on the
+// device from the lengths: one long sequence occupies every SM, a ragged batch leaves none idle, and the host needs to know
+// no length.  Inside a block each of four warps walks every fourth 16-token tile (8 for fp32) with its own running maximum,
+// sum and output; the four are joined when the segment or the range ends.  Segments that several blocks share are joined by a
+// second kernel, launched programmatically so that its start overlaps the first one's end; the parts are added in block order,
+// so results do not depend on timing.
 //
 // The tiles go from HBM straight into the registers in the layout that mma.sync wants as its B operand, 16 bytes per load and
 // without shared memory, because the order of the summed index is free as long as both operands share it:
@@ -28,9 +35,15 @@ struct PagedAttnParams {
   const int* lens;
   int* status;
   long long q_sb, q_ss, q_sh, k_page, k_head, v_page, v_head, table_stride, m_sb, m_ss;
+  float* part_o;   // [grid, 2, RT, DP] unnormalised outputs of shared segments: 0 = begun by an earlier block, 1 = begun here
+  float2* part_ml;  // [grid, 2, RT] their maxima and sums
+  int4* shared_seg;  // [grid] of the segment begun earlier that ends here: (first block, query, key head, first row); x < 0: none
   int b, s, hkv, group, d, page_size, max_pages, num_pages, mask_len, row_tiles;
   float scale;
 };
+
+//: units a block takes at least
+constexpr int kMinUnits = 2;
 
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -93,9 +106,18 @@ OSLO_DEVINL void mma_3xtf32(float (&c)[4], const float (&a)[4], float b0, float 
   mma_tf32(c, h0, h1, h2, h3, g0, g1);
 }
 
-OSLO_DEVINL float pa_out(float x, float) { return x; }
-OSLO_DEVINL __half pa_out(float x, __half) { return __float2half_rn(x); }
-OSLO_DEVINL __nv_bfloat16 pa_out(float x, __nv_bfloat16) { return __float2bfloat16_rn(x); }
+// s / l, zeros where nothing was seen
+OSLO_DEVINL void pa_store(float* dst, float4 s, float l) {
+  const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
+  *reinterpret_cast<float4*>(dst) = make_float4(s.x * inv, s.y * inv, s.z * inv, s.w * inv);
+}
+template <typename T>
+OSLO_DEVINL void pa_store(T* dst, float4 s, float l) {
+  const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
+  uint2 r;
+  r.x = Mma16<T>::pack(s.x * inv, s.y * inv), r.y = Mma16<T>::pack(s.z * inv, s.w * inv);
+  *reinterpret_cast<uint2*>(dst) = r;
+}
 
 // T: element type; DP: head_dim rounded up to 64, 128 or 256; WIDE: 9 to 16 query heads per block instead of up to 8
 template <typename T, int DP, bool WIDE, bool MASK>
@@ -109,6 +131,8 @@ struct PagedAttn {
   static constexpr int RT = WIDE ? 16 : 8;  // query rows
   static constexpr int ROW = DP + 4;        // padded row of the joining buffer
   static constexpr int WARPS = 4;
+  // Blocks an SM should hold: enough loads in flight to cover HBM's latency (8 KB a warp and tile) without spilling.
+  static constexpr int BLOCKS = DP == 64 ? (sizeof(T) == 2 ? 4 : 2) : DP == 128 && sizeof(T) == 2 && !WIDE ? 3 : 2;
   static constexpr size_t kSmem = sizeof(float) * (WARPS * RT * ROW + 2 * WARPS * RT);
 
   uint4 q0[KC], q1[WIDE ? KC : 1];
@@ -322,103 +346,294 @@ struct PagedAttn {
   }
 };
 
+// The tokens a query sees, as far as the table (and the mask) reach.
+template <bool MASK>
+OSLO_DEVINL int query_limit(const PagedAttnParams& p, int query, bool report) {
+  const int b = query / p.s, i = query - b * p.s;
+  const long long limit = static_cast<long long>(p.lens[b]) - p.s + 1 + i;
+  const int cap = MASK ? min(p.mask_len, p.max_pages * p.page_size) : p.max_pages * p.page_size;
+  if (limit > cap && report) atomicCAS(p.status, kStatusOk, kStatusPageRange);
+  return static_cast<int>(min(max(limit, 0ll), static_cast<long long>(cap)));
+}
+
 template <typename T, int DP, bool WIDE, bool MASK>
-__global__ void __launch_bounds__(128) paged_attention_kernel(const PagedAttnParams p) {
+__global__ void __launch_bounds__(128, PagedAttn<T, DP, WIDE, MASK>::BLOCKS) paged_attention_kernel(const PagedAttnParams p) {
   using A = PagedAttn<T, DP, WIDE, MASK>;
+  constexpr int UNIT = A::WARPS * A::TT;
   extern __shared__ float4 smem4[];
+  __shared__ long long scan[A::WARPS + 2];
   float* buf = reinterpret_cast<float*>(smem4);
   float* ml = buf + A::WARPS * A::RT * A::ROW;
-  int seg = blockIdx.x;
-  const int row0 = (seg % p.row_tiles) * A::RT;
-  seg /= p.row_tiles;
-  const int h = seg % p.hkv;
-  const int query = seg / p.hkv, b = query / p.s, i = query % p.s;
-  int limit = p.lens[b] - p.s + 1 + i;
-  const int cap = MASK ? min(p.mask_len, p.max_pages * p.page_size) : p.max_pages * p.page_size;
-  if (limit > cap) {
-    limit = cap;
-    if (threadIdx.x == 0) atomicCAS(p.status, kStatusOk, kStatusPageRange);
-  }
-  A a;
-  a.load_q(p, static_cast<const T*>(p.q) + b * p.q_sb + i * p.q_ss + static_cast<long long>(h) * p.group * p.q_sh, row0);
-  a.clear();
-  const float* mask = MASK ? p.mask + b * p.m_sb + i * p.m_ss : nullptr;
-  for (int t = (threadIdx.x >> 5) * A::TT; t < limit; t += A::WARPS * A::TT) {
-    const int page = p.table[b * p.table_stride + t / p.page_size];
-    const bool ok = page >= 0 && page < p.num_pages;
-    if (!ok && (threadIdx.x & 31) == 0) atomicCAS(p.status, kStatusOk, kStatusPageRange);
-    if (!ok) continue;
-    const long long in_page = static_cast<long long>(t % p.page_size) * p.d;
-    a.tile(p, static_cast<const T*>(p.k) + page * p.k_page + h * p.k_head + in_page,
-           static_cast<const T*>(p.v) + page * p.v_page + h * p.v_head + in_page, t, limit, mask);
-  }
-  a.join(buf, ml);
-  T* out = static_cast<T*>(p.out) + (static_cast<long long>(query) * p.hkv + h) * p.group * p.d;
-  for (int x = threadIdx.x; x < A::RT * (DP / 4); x += blockDim.x) {
-    const int row = x / (DP / 4), dim = x % (DP / 4) * 4;
-    if (row0 + row >= p.group || dim >= p.d) continue;
-    float l = 0.f;
-    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  // This block's range of units: an exclusive prefix sum of the queries' units over the block's threads, each of which owns a
+  // contiguous run of queries.  A query without tokens is one unit, so that its zeros are written.
+  const int queries = p.b * p.s, run = (queries + 127) / 128;
+  const int first = min(queries, static_cast<int>(threadIdx.x) * run), last = min(queries, first + run);
+  long long mine = 0;
+  for (int i = first; i < last; ++i) mine += max(1, (query_limit<MASK>(p, i, false) + UNIT - 1) / UNIT);
+  long long incl = mine;
 #pragma unroll
-    for (int w = 0; w < A::WARPS; ++w) {
-      l += ml[(A::WARPS + w) * A::RT + row];
-      const float4 y = *reinterpret_cast<const float4*>(buf + (w * A::RT + row) * A::ROW + dim);
-      s.x += y.x, s.y += y.y, s.z += y.z, s.w += y.w;
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long n = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += n;
+  }
+  if (lane == 31) scan[warp] = incl;
+  __syncthreads();
+  long long before = incl - mine, total = 0;
+#pragma unroll
+  for (int w = 0; w < A::WARPS; ++w) {
+    if (w < warp) before += scan[w];
+    total += scan[w];
+  }
+  const int heads = p.hkv * p.row_tiles;  // segments of a query
+  const long long units = total * heads;
+  const long long blocks = min(static_cast<long long>(gridDim.x), max(1ll, units / kMinUnits));
+  if (threadIdx.x == 0) p.shared_seg[blockIdx.x] = make_int4(-1, 0, 0, 0);
+  if (blockIdx.x >= blocks) return;
+  long long u = units * blockIdx.x / blocks;
+  const long long u_end = units * (blockIdx.x + 1) / blocks;
+  const long long at = u / heads;
+  __syncthreads();
+  if (mine > 0 && at >= before && at < before + mine) {
+    int i = first;
+    long long n;
+    while (at >= before + (n = max(1, (query_limit<MASK>(p, i, false) + UNIT - 1) / UNIT))) before += n, ++i;
+    scan[0] = i;
+    scan[1] = before;
+  }
+  __syncthreads();
+  int query = static_cast<int>(scan[0]);
+  long long base = scan[1] * heads;  // first unit of the query
+  int limit = query_limit<MASK>(p, query, threadIdx.x == 0);
+  int n_units = max(1, (limit + UNIT - 1) / UNIT);
+
+  while (u < u_end) {
+    if (u >= base + static_cast<long long>(n_units) * heads) {
+      base += static_cast<long long>(n_units) * heads;
+      ++query;
+      limit = query_limit<MASK>(p, query, threadIdx.x == 0);
+      n_units = max(1, (limit + UNIT - 1) / UNIT);
     }
-    const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
-    T* dst = out + (row0 + row) * p.d + dim;
-    dst[0] = pa_out(s.x * inv, T()), dst[1] = pa_out(s.y * inv, T()), dst[2] = pa_out(s.z * inv, T()), dst[3] = pa_out(s.w * inv, T());
+    const int seg = static_cast<int>((u - base) / n_units);
+    const int a = static_cast<int>((u - base) - static_cast<long long>(seg) * n_units);
+    const int e = static_cast<int>(min(static_cast<long long>(n_units), a + (u_end - u)));
+    const int h = seg / p.row_tiles, row0 = (seg - h * p.row_tiles) * A::RT;
+    const int b = query / p.s, i = query - b * p.s;
+
+    A acc;
+    acc.load_q(p, static_cast<const T*>(p.q) + b * p.q_sb + i * p.q_ss + static_cast<long long>(h) * p.group * p.q_sh, row0);
+    acc.clear();
+    const float* mask = MASK ? p.mask + b * p.m_sb + i * p.m_ss : nullptr;
+    const int* table = p.table + b * p.table_stride;
+    const int end = min(limit, e * UNIT);
+    int t = a * UNIT + warp * A::TT;
+    int page = t < end ? table[t / p.page_size] : 0;
+    while (t < end) {
+      const int next = t + UNIT, next_page = next < end ? table[next / p.page_size] : 0;
+      if (page >= 0 && page < p.num_pages) {
+        const long long in_page = static_cast<long long>(t % p.page_size) * p.d;
+        acc.tile(p, static_cast<const T*>(p.k) + page * p.k_page + h * p.k_head + in_page,
+                 static_cast<const T*>(p.v) + page * p.v_page + h * p.v_head + in_page, t, limit, mask);
+      } else if (lane == 0) {
+        atomicCAS(p.status, kStatusOk, kStatusPageRange);
+      }
+      t = next, page = next_page;
+    }
+    acc.join(buf, ml);
+
+    const bool whole = a == 0 && e == n_units;
+    const long long slot = static_cast<long long>(blockIdx.x) * 2 + (a == 0 ? 1 : 0);
+    T* out = static_cast<T*>(p.out) + (static_cast<long long>(query) * p.hkv + h) * p.group * p.d;
+    for (int x = threadIdx.x; x < A::RT * (DP / 4); x += blockDim.x) {
+      const int row = x / (DP / 4), dim = x % (DP / 4) * 4;
+      if (row0 + row >= p.group || dim >= p.d) continue;
+      float l = 0.f, m = -INFINITY;
+      float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < A::WARPS; ++w) {
+        l += ml[(A::WARPS + w) * A::RT + row];
+        m = fmaxf(m, ml[w * A::RT + row]);
+        const float4 y = *reinterpret_cast<const float4*>(buf + (w * A::RT + row) * A::ROW + dim);
+        s.x += y.x, s.y += y.y, s.z += y.z, s.w += y.w;
+      }
+      if (whole) {
+        pa_store(out + (row0 + row) * p.d + dim, s, l);
+      } else {
+        *reinterpret_cast<float4*>(p.part_o + (slot * A::RT + row) * DP + dim) = s;
+        if (dim == 0) p.part_ml[slot * A::RT + row] = make_float2(m, l);
+      }
+    }
+    if (threadIdx.x == 0 && a > 0 && e == n_units) {
+      const long long start = base + static_cast<long long>(seg) * n_units;
+      p.shared_seg[blockIdx.x] = make_int4(static_cast<int>(((start + 1) * blocks - 1) / units), query, h, row0);
+    }
+    u += e - a;
+    __syncthreads();  // buf is free for the next segment
   }
 }
+
+// Joins a segment that several blocks of the first kernel share.  Block (row, last block of the segment); warp w adds every
+// eighth part, then the warps' sums are added.
+template <typename T, int DP, bool WIDE, bool MASK>
+__global__ void __launch_bounds__(256) paged_attention_join_kernel(const PagedAttnParams p) {
+  using A = PagedAttn<T, DP, WIDE, MASK>;
+  constexpr int V = DP / 128 > 0 ? DP / 128 : 1;  // float4s of a lane
+  constexpr int LANES = DP / 4 < 32 ? DP / 4 : 32;
+  __shared__ float4 sums[8][DP / 4];
+  __shared__ float red[8];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int4 seg = p.shared_seg[blockIdx.y];
+  const int row = blockIdx.x;
+  if (seg.x < 0 || seg.w + row >= p.group) return;
+  const int parts = blockIdx.y - seg.x + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const auto slot = [&](int i) { return (static_cast<long long>(seg.x + i) * 2 + (i == 0 ? 1 : 0)) * A::RT + row; };
+  float m = -INFINITY;
+  for (int i = threadIdx.x; i < parts; i += 256) m = fmaxf(m, p.part_ml[slot(i)].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (lane == 0) red[warp] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) m = fmaxf(m, red[w]);
+  __syncthreads();
+  float l = 0.f;
+  float4 o[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) o[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int i = warp; i < parts; i += 8) {
+    const float2 x = p.part_ml[slot(i)];
+    const float w = A::weight(x.x, m);
+    l += x.y * w;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int dim = (j * 32 + lane) * 4;
+      if (lane < LANES && dim < p.d) {
+        const float4 y = *reinterpret_cast<const float4*>(p.part_o + slot(i) * DP + dim);
+        o[j].x += y.x * w, o[j].y += y.y * w, o[j].z += y.z * w, o[j].w += y.w * w;
+      }
+    }
+  }
+  if (lane == 0) red[warp] = l;
+#pragma unroll
+  for (int j = 0; j < V; ++j)
+    if (lane < LANES) sums[warp][j * 32 + lane] = o[j];
+  __syncthreads();
+  const int dim = threadIdx.x * 4;
+  if (dim >= p.d) return;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  l = 0.f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    const float4 y = sums[w][threadIdx.x];
+    s.x += y.x, s.y += y.y, s.z += y.z, s.w += y.w;
+    l += red[w];
+  }
+  T* out = static_cast<T*>(p.out) + ((static_cast<long long>(seg.y) * p.hkv + seg.z) * p.group + seg.w + row) * p.d;
+  pa_store(out + dim, s, l);
+}
+
+// What the caller's workspace has to hold for one block of the grid, in bytes.
+constexpr long long part_bytes(int rt, int dp) { return 2ll * rt * (dp * 4 + 8) + 16; }
 
 template <typename T, int DP, bool WIDE, bool MASK>
-int paged_attention_launch(PagedAttnParams& p, cudaStream_t st) {
+struct PagedAttnLaunch {
   using A = PagedAttn<T, DP, WIDE, MASK>;
-  p.row_tiles = (p.group + A::RT - 1) / A::RT;
-  const long long grid = static_cast<long long>(p.b) * p.s * p.hkv * p.row_tiles;
-  if (grid > 0x7fffffffll) return -1;
-  auto kernel = paged_attention_kernel<T, DP, WIDE, MASK>;
-  if (A::kSmem > 48 * 1024 &&
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(A::kSmem)) != cudaSuccess)
-    return -2;
-  kernel<<<static_cast<unsigned>(grid), 128, A::kSmem, st>>>(p);
-  return cudaGetLastError() == cudaSuccess ? 0 : -2;
-}
+  // Blocks that one SM holds at once; negative: an error.
+  static int resident() {
+    auto kernel = paged_attention_kernel<T, DP, WIDE, MASK>;
+    if (A::kSmem > 48 * 1024 &&
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(A::kSmem)) != cudaSuccess)
+      return -2;
+    int n = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, 128, A::kSmem) != cudaSuccess || n < 1) return -2;
+    return n;
+  }
+  static int launch(PagedAttnParams& p, int grid, void* ws, long long ws_bytes, cudaStream_t st) {
+    if (grid <= 0 || ws_bytes < grid * part_bytes(A::RT, DP)) return -1;
+    char* w = static_cast<char*>(ws);
+    p.part_o = reinterpret_cast<float*>(w);
+    p.part_ml = reinterpret_cast<float2*>(w + static_cast<long long>(grid) * 2 * A::RT * DP * 4);
+    p.shared_seg = reinterpret_cast<int4*>(w + static_cast<long long>(grid) * 2 * A::RT * (DP * 4 + 8));
+    p.row_tiles = (p.group + A::RT - 1) / A::RT;
+    paged_attention_kernel<T, DP, WIDE, MASK><<<grid, 128, A::kSmem, st>>>(p);
+    if (cudaGetLastError() != cudaSuccess) return -2;
+    if (grid == 1) return 0;  // nothing is shared
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(p.group < A::RT ? p.group : A::RT, grid);
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, paged_attention_join_kernel<T, DP, WIDE, MASK>, p) == cudaSuccess ? 0 : -2;
+  }
+};
 
-template <typename T, int DP>
-int paged_attention_dp(PagedAttnParams& p, cudaStream_t st) {
-  const bool wide = p.group > 8;
-  if (p.mask) return wide ? paged_attention_launch<T, DP, true, true>(p, st) : paged_attention_launch<T, DP, false, true>(p, st);
-  return wide ? paged_attention_launch<T, DP, true, false>(p, st) : paged_attention_launch<T, DP, false, false>(p, st);
+// Calls f with the PagedAttnLaunch of these types and sizes.
+template <typename T, int DP, typename F>
+int paged_attention_dp(bool wide, bool mask, F f) {
+  if (mask) return wide ? f(PagedAttnLaunch<T, DP, true, true>()) : f(PagedAttnLaunch<T, DP, false, true>());
+  return wide ? f(PagedAttnLaunch<T, DP, true, false>()) : f(PagedAttnLaunch<T, DP, false, false>());
 }
-
-template <typename T>
-int paged_attention_type(PagedAttnParams& p, cudaStream_t st) {
-  if (p.d <= 64) return paged_attention_dp<T, 64>(p, st);
-  if (p.d <= 128) return paged_attention_dp<T, 128>(p, st);
-  return paged_attention_dp<T, 256>(p, st);
+template <typename T, typename F>
+int paged_attention_type(int d, bool wide, bool mask, F f) {
+  if (d <= 64) return paged_attention_dp<T, 64>(wide, mask, f);
+  if (d <= 128) return paged_attention_dp<T, 128>(wide, mask, f);
+  return paged_attention_dp<T, 256>(wide, mask, f);
+}
+template <typename F>
+int paged_attention_dispatch(int dtype, int d, int group, bool mask, F f) {
+  const bool wide = group > 8;
+  if (dtype == 0) return paged_attention_type<float>(d, wide, mask, f);
+  if (dtype == 1) return paged_attention_type<__half>(d, wide, mask, f);
+  if (dtype == 2) return paged_attention_type<__nv_bfloat16>(d, wide, mask, f);
+  return -1;
 }
 
 }  // namespace oslo
 
-// strides (elements): batch, token, head of q; page, head of the two pools; rows of the table; batch, token of the mask.
-extern "C" int oslo_paged_attention(const void* q, const void* k_pages, const void* v_pages, const int* table, const int* lens,
-                                    const float* mask, void* out, const long long* strides, int b, int s, int hkv, int group, int d,
-                                    int page_size, int max_pages, int num_pages, int mask_len, float scale, int dtype, int* status,
-                                    void* stream) {
+extern "C" {
+
+// Everything a call needs, eight bytes each.  Strides in elements.
+struct OsloPagedAttentionArgs {
+  long long q, k_pages, v_pages, table, lens, mask, out, workspace, status, stream;  // addresses; mask may be 0
+  long long q_b, q_s, q_h, k_page, k_head, v_page, v_head, table_row, mask_b, mask_s;
+  long long b, s, hkv, group, d, page_size, max_pages, num_pages, mask_len, dtype, grid, workspace_bytes;
+  double scale;
+};
+
+// Blocks of the first kernel that one SM of the current device holds (negative: an error).
+int oslo_paged_attention_resident_parts(int dtype, int d, int group, int mask) {
   using namespace oslo;
-  if (b <= 0 || s <= 0) return 0;
-  if (hkv <= 0 || group <= 0 || d <= 0 || d > 256 || d % 8 || page_size <= 0 || page_size % 16) return -1;
+  return paged_attention_dispatch(dtype, d, group, mask != 0, [](auto l) { return decltype(l)::resident(); });
+}
+// Workspace of one block of the grid.
+long long oslo_paged_attention_block_bytes(int d, int group) {
+  return oslo::part_bytes(group > 8 ? 16 : 8, d <= 64 ? 64 : d <= 128 ? 128 : 256);
+}
+
+int oslo_paged_attention(const OsloPagedAttentionArgs* a) {
+  using namespace oslo;
+  if (a->b <= 0 || a->s <= 0) return 0;
+  if (a->hkv <= 0 || a->group <= 0 || a->d <= 0 || a->d > 256 || a->d % 8 || a->page_size <= 0 || a->page_size % 16) return -1;
+  if (a->b * a->s > 0x3fffffff || a->max_pages * a->page_size > 0x3fffffff) return -1;
   PagedAttnParams p{};
-  p.q = q, p.k = k_pages, p.v = v_pages, p.mask = mask, p.out = out, p.table = table, p.lens = lens, p.status = status;
-  p.q_sb = strides[0], p.q_ss = strides[1], p.q_sh = strides[2];
-  p.k_page = strides[3], p.k_head = strides[4], p.v_page = strides[5], p.v_head = strides[6], p.table_stride = strides[7];
-  p.m_sb = strides[8], p.m_ss = strides[9];
-  p.b = b, p.s = s, p.hkv = hkv, p.group = group, p.d = d, p.page_size = page_size, p.max_pages = max_pages, p.num_pages = num_pages;
-  p.mask_len = mask_len, p.scale = scale;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == 0) return paged_attention_type<float>(p, st);
-  if (dtype == 1) return paged_attention_type<__half>(p, st);
-  if (dtype == 2) return paged_attention_type<__nv_bfloat16>(p, st);
-  return -1;
+  p.q = reinterpret_cast<const void*>(a->q), p.k = reinterpret_cast<const void*>(a->k_pages), p.v = reinterpret_cast<const void*>(a->v_pages);
+  p.mask = reinterpret_cast<const float*>(a->mask), p.out = reinterpret_cast<void*>(a->out);
+  p.table = reinterpret_cast<const int*>(a->table), p.lens = reinterpret_cast<const int*>(a->lens);
+  p.status = reinterpret_cast<int*>(a->status);
+  p.q_sb = a->q_b, p.q_ss = a->q_s, p.q_sh = a->q_h, p.k_page = a->k_page, p.k_head = a->k_head, p.v_page = a->v_page;
+  p.v_head = a->v_head, p.table_stride = a->table_row, p.m_sb = a->mask_b, p.m_ss = a->mask_s;
+  p.b = a->b, p.s = a->s, p.hkv = a->hkv, p.group = a->group, p.d = a->d, p.page_size = a->page_size, p.max_pages = a->max_pages;
+  p.num_pages = a->num_pages, p.mask_len = a->mask_len, p.scale = static_cast<float>(a->scale);
+  return paged_attention_dispatch(a->dtype, a->d, a->group, a->mask != 0, [&](auto l) {
+    return decltype(l)::launch(p, static_cast<int>(a->grid), reinterpret_cast<void*>(a->workspace), a->workspace_bytes,
+                               reinterpret_cast<cudaStream_t>(a->stream));
+  });
+}
 }

@@ -15,6 +15,8 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
+from functools import lru_cache
 from typing import List, Optional, Sequence
 
 import torch
@@ -180,19 +182,31 @@ def paged_attention(q, k_pages, v_pages, block_table, lengths, scale: Optional[f
         if mask.stride(3) != 1:
             mask = mask.contiguous()
         ms, mlen = (mask.stride(0), mask.stride(2)), mask.shape[3]
-    strides = (ctypes.c_longlong * 10)(*q.stride()[:3], *k_pages.stride()[:2], *v_pages.stride()[:2], block_table.stride(0), *ms)
-    rc = _fn("oslo_paged_attention", _ATTEND_ARGS)(
+    d_index = dev.index
+    masked = mask is not None
+    blocks, block_bytes = _attention_plan(_DT[q.dtype], hd, hq // hkv, masked, d_index)
+    qs, ks, vs = q.stride(), k_pages.stride(), v_pages.stride()
+    pages, _, page, _ = k_pages.shape
+    width = block_table.shape[1]
+    # no more blocks than the longest possible sequences have work for (in units of 32 tokens, the smallest of the kernel's)
+    most = min(width * page, mlen) if masked else width * page
+    grid = max(1, min(blocks, b * s * hq * -(-most // 32)))
+    ws = torch.empty(grid * block_bytes, dtype=torch.uint8, device=dev)
+    args = _ATTEND_ARGS.pack(
         q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), lengths.data_ptr(),
-        mask.data_ptr() if mask is not None else None, out.data_ptr(), strides, b, s, hkv, hq // hkv, hd, k_pages.shape[2],
-        block_table.shape[1], k_pages.shape[0], mlen, scale, _DT[q.dtype], _lib.status_word(dev).data_ptr(), _raw_stream(dev.index))
+        mask.data_ptr() if masked else 0, out.data_ptr(), ws.data_ptr(), _lib.status_word(dev).data_ptr(), _raw_stream(d_index),
+        qs[0], qs[1], qs[2], ks[0], ks[1], vs[0], vs[1], block_table.stride(0), *ms,
+        b, s, hkv, hq // hkv, hd, page, width, pages, mlen, _DT[q.dtype], grid, grid * block_bytes, scale)
+    rc = _fn("oslo_paged_attention", _PACKED)(args)
     if rc:
         raise RuntimeError(f"oslo_paged_attention failed ({rc})")
     return out
 
 
-_P, _I, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
+_P, _I = ctypes.c_void_p, ctypes.c_int
 _APPEND_ARGS = [_P] * 12 + [_I] * 12 + [_P, _P]
-_ATTEND_ARGS = [_P] * 8 + [_I] * 9 + [_F, _I, _P, _P]
+_PACKED = [ctypes.c_char_p]  # a struct of eight-byte fields
+_ATTEND_ARGS = struct.Struct("=32qd")
 _fns = {}
 
 
@@ -204,6 +218,17 @@ def _fn(name, argtypes):
         getattr(_lib._load_cuda_lib(), name).argtypes = argtypes
         fn = _fns[name] = getattr(lib, name)
     return fn
+
+
+@lru_cache(maxsize=None)
+def _attention_plan(dtype: int, hd: int, group: int, masked: bool, device: int):
+    """(blocks that the device holds at once, workspace bytes of a block) of the attention kernel for these types and sizes."""
+    lib = _lib._load_cuda_lib()
+    lib.oslo_paged_attention_block_bytes.restype = ctypes.c_longlong
+    n = lib.oslo_paged_attention_resident_parts(dtype, hd, group, 1 if masked else 0)
+    if n <= 0:
+        raise RuntimeError(f"oslo_paged_attention_resident_parts failed ({n})")
+    return n * _lib.num_sms(device), lib.oslo_paged_attention_block_bytes(hd, group)
 
 
 # ------------------------------------------------------------------------------------------------ plain forms
