@@ -154,33 +154,38 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const PagedAppendPara
 
 }  // namespace oslo
 
-// strides: batch, token, head of q, k, v; page, head of the two pools; rows of the table (elements).
-extern "C" int oslo_paged_kv_append(const void* q, const void* k, const void* v, void* q_out, void* k_pages, void* v_pages,
-                                    const int* table, const int* start, const int* count, const float* cosb, const float* sinb,
-                                    const long long* strides, int b, int s, int hq, int hkv, int d, int rot, int neox, int positions,
-                                    int page_size, int max_pages, int num_pages, int dtype, int* status, void* stream) {
+// Everything a call needs, eight bytes each.  Strides in elements.
+struct OsloPagedAppendArgs {
+  long long q, k, v, q_out, k_pages, v_pages, table, start, count, cosb, sinb, status, stream;  // addresses; q, count, cosb may be 0
+  long long q_b, q_s, q_h, k_b, k_s, k_h, v_b, v_s, v_h, k_page, k_head, v_page, v_head, table_row;
+  long long b, s, hq, hkv, d, rot, neox, positions, page_size, max_pages, num_pages, dtype;
+};
+
+extern "C" int oslo_paged_kv_append(const OsloPagedAppendArgs* a) {
   using namespace oslo;
-  if (b <= 0 || s <= 0) return 0;
-  if (hkv <= 0 || d <= 0 || d % 8 || page_size <= 0 || rot < 0 || rot > d || rot % 2) return -1;
+  if (a->b <= 0 || a->s <= 0) return 0;
+  if (a->hkv <= 0 || a->d <= 0 || a->d % 8 || a->page_size <= 0 || a->rot < 0 || a->rot > a->d || a->rot % 2) return -1;
   PagedAppendParams p;
-  p.q = q, p.k = k, p.v = v, p.q_out = q_out, p.k_pages = k_pages, p.v_pages = v_pages;
-  p.table = table, p.start = start, p.count = count, p.cosb = rot ? cosb : nullptr, p.sinb = rot ? sinb : nullptr, p.status = status;
-  p.q_sb = strides[0], p.q_ss = strides[1], p.q_sh = strides[2];
-  p.k_sb = strides[3], p.k_ss = strides[4], p.k_sh = strides[5];
-  p.v_sb = strides[6], p.v_ss = strides[7], p.v_sh = strides[8];
-  p.kp_page = strides[9], p.kp_head = strides[10], p.vp_page = strides[11], p.vp_head = strides[12], p.table_stride = strides[13];
-  p.b = b, p.s = s, p.hq = q ? hq : 0, p.hkv = hkv, p.d = d, p.rot = rot, p.neox = neox, p.positions = positions;
-  p.page_size = page_size, p.max_pages = max_pages, p.num_pages = num_pages;
-  const int e = dtype == 0 ? 4 : 8;
-  const long long chunks = static_cast<long long>(p.hq + 2 * hkv) * (d / e);
-  const long long tokens = static_cast<long long>(b) * s;
+  p.q = reinterpret_cast<const void*>(a->q), p.k = reinterpret_cast<const void*>(a->k), p.v = reinterpret_cast<const void*>(a->v);
+  p.q_out = reinterpret_cast<void*>(a->q_out), p.k_pages = reinterpret_cast<void*>(a->k_pages);
+  p.v_pages = reinterpret_cast<void*>(a->v_pages), p.table = reinterpret_cast<const int*>(a->table);
+  p.start = reinterpret_cast<const int*>(a->start), p.count = reinterpret_cast<const int*>(a->count);
+  p.cosb = reinterpret_cast<const float*>(a->rot ? a->cosb : 0), p.sinb = reinterpret_cast<const float*>(a->rot ? a->sinb : 0);
+  p.status = reinterpret_cast<int*>(a->status);
+  p.q_sb = a->q_b, p.q_ss = a->q_s, p.q_sh = a->q_h, p.k_sb = a->k_b, p.k_ss = a->k_s, p.k_sh = a->k_h;
+  p.v_sb = a->v_b, p.v_ss = a->v_s, p.v_sh = a->v_h;
+  p.kp_page = a->k_page, p.kp_head = a->k_head, p.vp_page = a->v_page, p.vp_head = a->v_head, p.table_stride = a->table_row;
+  p.b = a->b, p.s = a->s, p.hq = a->q ? a->hq : 0, p.hkv = a->hkv, p.d = a->d, p.rot = a->rot, p.neox = a->neox;
+  p.positions = a->positions, p.page_size = a->page_size, p.max_pages = a->max_pages, p.num_pages = a->num_pages;
+  const int e = a->dtype == 0 ? 4 : 8;
+  const long long chunks = static_cast<long long>(p.hq + 2 * p.hkv) * (p.d / e);
   const long long parts = (chunks + 255) / 256;
-  if (tokens * parts > 0x7fffffffll) return -1;
-  const unsigned grid = static_cast<unsigned>(tokens * parts);
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == 0) paged_append_kernel<float><<<grid, 256, 0, st>>>(p, static_cast<int>(parts));
-  else if (dtype == 1) paged_append_kernel<__half><<<grid, 256, 0, st>>>(p, static_cast<int>(parts));
-  else if (dtype == 2) paged_append_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(p, static_cast<int>(parts));
+  if (a->b * a->s * parts > 0x7fffffffll) return -1;
+  const unsigned grid = static_cast<unsigned>(a->b * a->s * parts);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(a->stream);
+  if (a->dtype == 0) paged_append_kernel<float><<<grid, 256, 0, st>>>(p, static_cast<int>(parts));
+  else if (a->dtype == 1) paged_append_kernel<__half><<<grid, 256, 0, st>>>(p, static_cast<int>(parts));
+  else if (a->dtype == 2) paged_append_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(p, static_cast<int>(parts));
   else return -1;
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }

@@ -6,6 +6,7 @@
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Optional, Union
 
 import torch
@@ -13,7 +14,8 @@ import torch
 from . import _lib
 
 _DT = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # of a device's current stream
+_device = getattr(torch._C, "_cuda_getDevice", None)
 
 
 def pack_token_mask(mask: torch.Tensor) -> torch.Tensor:
@@ -32,7 +34,7 @@ def _per_row(name, p, rows: int, device):
     if isinstance(p, torch.Tensor):
         if p.shape != (rows,) or p.device != device or not p.is_floating_point():
             raise ValueError(f"{name} is a number or a floating tensor [{rows}] on {device}: got {p.dtype} {tuple(p.shape)} on {p.device}")
-        return p.float().contiguous(), 0.0
+        return (p if p.dtype == torch.float32 and p.is_contiguous() else p.float().contiguous()), 0.0
     return None, float(p)
 
 
@@ -55,12 +57,12 @@ def process_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     ``allowed``: int32 ``[rows or 1, ceil(vocab / 32)]`` from :func:`pack_token_mask`; a row that allows nothing is all ``-inf``.
     The result is a new tensor, or ``out`` (which may be ``logits``).  For inference: no gradient.
     """
-    if logits.dim() != 2 or logits.dtype not in _DT:
-        raise ValueError(f"logits are float32, float16 or bfloat16 [rows, vocab]: got {logits.dtype} {tuple(logits.shape)}")
+    dtype, dev = logits.dtype, logits.device
+    if logits.dim() != 2 or dtype not in _DT:
+        raise ValueError(f"logits are float32, float16 or bfloat16 [rows, vocab]: got {dtype} {tuple(logits.shape)}")
     if torch.is_grad_enabled() and (logits.requires_grad or (bias is not None and bias.requires_grad)):
         raise RuntimeError("process_logits is for inference: call it under torch.no_grad() or detach its inputs")
     rows, v = logits.shape
-    dev = logits.device
     rep, rep_s = _per_row("repetition_penalty", repetition_penalty, rows, dev)
     pres, pres_s = _per_row("presence_penalty", presence_penalty, rows, dev)
     freq, freq_s = _per_row("frequency_penalty", frequency_penalty, rows, dev)
@@ -82,7 +84,7 @@ def process_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
         if bias.shape not in ((v,), (rows, v)) or not bias.is_floating_point() or bias.device != dev:
             raise ValueError(f"bias is a floating tensor [{v}] or [{rows}, {v}] on {dev}: got {bias.dtype} {tuple(bias.shape)} on "
                              f"{bias.device}")
-        bias = bias.float()
+        bias = bias if bias.dtype == torch.float32 else bias.float()
     if allowed is not None and (allowed.dtype != torch.int32 or allowed.dim() != 2 or allowed.shape[0] not in (1, rows)
                                 or allowed.shape[1] != (v + 31) // 32 or allowed.device != dev):
         raise ValueError(f"allowed is int32 [{rows} or 1, {(v + 31) // 32}] on {dev}: got {allowed.dtype} {tuple(allowed.shape)} on "
@@ -93,43 +95,50 @@ def process_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
         y = _reference(logits, tokens, token_lengths, prompt_lengths, *(t if t is not None else s for t, s in
                        ((rep, rep_s), (pres, pres_s), (freq, freq_s))), bias, allowed)
         return y if out is None else out.copy_(y)
-    if dev.index != torch.cuda.current_device():
+    if dev.index != _device():
         with torch.cuda.device(dev):
             return process_logits(logits, tokens, token_lengths, prompt_lengths, repetition_penalty, presence_penalty,
                                   frequency_penalty, bias, allowed, out)
-    if logits.stride(1) != 1:
+    xs = logits.stride()
+    if xs[1] != 1:
         logits = logits.contiguous()
-    y = torch.empty(rows, v, dtype=logits.dtype, device=dev) if out is None else out
-    length = 0
-    if tokens is not None:
-        tokens = tokens if tokens.stride(1) == 1 else tokens.contiguous()
-        length = tokens.shape[1]
-    if bias is not None and bias.stride(-1) != 1:
-        bias = bias.contiguous()
-    if allowed is not None and allowed.stride(1) != 1:
-        allowed = allowed.contiguous()
-    p = lambda t: t.data_ptr() if t is not None else None
-    rc = _fn()(
-        logits.data_ptr(), y.data_ptr(), p(tokens) if length else None, p(token_lengths), p(prompt_lengths), p(rep), p(pres), p(freq),
-        p(bias), p(allowed), logits.stride(0), y.stride(0), tokens.stride(0) if length else 0,
-        bias.stride(0) if bias is not None and bias.dim() == 2 else 0,
-        allowed.stride(0) if allowed is not None and allowed.shape[0] == rows else 0, rep_s, pres_s, freq_s, rows, v, length,
-        1 if length and tokens.dtype == torch.int64 else 0, _DT[logits.dtype], _raw_stream(dev.index))
+        xs = logits.stride()
+    y = torch.empty((rows, v), dtype=dtype, device=dev) if out is None else out
+    length = tok_stride = 0
+    if tokens is not None and tokens.shape[1]:
+        length, ts = tokens.shape[1], tokens.stride()
+        if ts[1] != 1:
+            tokens = tokens.contiguous()
+            ts = tokens.stride()
+        tok_stride = ts[0]
+    bias_stride = allowed_stride = 0
+    if bias is not None:
+        bias = bias if bias.stride(-1) == 1 else bias.contiguous()
+        bias_stride = bias.stride(0) if bias.dim() == 2 else 0
+    if allowed is not None:
+        allowed = allowed if allowed.stride(1) == 1 else allowed.contiguous()
+        allowed_stride = allowed.stride(0) if allowed.shape[0] > 1 else 0
+    rc = _fn()(_ARGS.pack(
+        logits.data_ptr(), y.data_ptr(), tokens.data_ptr() if length else 0, 0 if token_lengths is None else token_lengths.data_ptr(),
+        0 if prompt_lengths is None else prompt_lengths.data_ptr(), 0 if rep is None else rep.data_ptr(),
+        0 if pres is None else pres.data_ptr(), 0 if freq is None else freq.data_ptr(), 0 if bias is None else bias.data_ptr(),
+        0 if allowed is None else allowed.data_ptr(), _raw_stream(dev.index), xs[0], v if out is None else out.stride(0), tok_stride,
+        bias_stride, allowed_stride, rows, v, length, 1 if length and tokens.dtype == torch.int64 else 0, _DT[dtype], rep_s, pres_s,
+        freq_s))
     if rc:
         raise RuntimeError(f"oslo_process_logits failed ({rc})")
     return y
 
 
+_ARGS = struct.Struct("=21q3d")  # arguments travel as one struct of eight-byte fields
 _native = None
 
 
 def _fn():
     global _native
     if _native is None:
-        lib = _lib.cuda_lib()
-        P, L, F, I = ctypes.c_void_p, ctypes.c_longlong, ctypes.c_float, ctypes.c_int
-        _lib._load_cuda_lib().oslo_process_logits.argtypes = [P] * 10 + [L] * 5 + [F] * 3 + [I] * 5 + [P]
-        _native = lib.oslo_process_logits
+        _lib._load_cuda_lib().oslo_process_logits.argtypes = [ctypes.c_char_p]
+        _native = _lib.cuda_lib().oslo_process_logits
     return _native
 
 

@@ -24,15 +24,18 @@ import torch
 from . import _lib
 
 _DT = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # of a device's current stream
+_device = getattr(torch._C, "_cuda_getDevice", None)
 MAX_HEAD_DIM = 256
 
 
 def _check_pages(k_pages, v_pages, block_table, b: int, hd: int, dtype, device):
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
-        raise ValueError(f"k_pages and v_pages are [pages, kv_heads, page_size, head_dim], both alike: got {tuple(k_pages.shape)} "
+    """Raises unless pools and table fit ``b`` sequences of this type; returns what the kernels need of their layout."""
+    shape, ks, vs = k_pages.shape, k_pages.stride(), v_pages.stride()
+    if len(shape) != 4 or v_pages.shape != shape:
+        raise ValueError(f"k_pages and v_pages are [pages, kv_heads, page_size, head_dim], both alike: got {tuple(shape)} "
                          f"and {tuple(v_pages.shape)}")
-    pages, hkv, page, d = k_pages.shape
+    pages, hkv, page, d = shape
     if dtype not in _DT or k_pages.dtype != dtype or v_pages.dtype != dtype:
         raise ValueError(f"queries, keys, values and pages share one of float32, float16, bfloat16: got {dtype}, {k_pages.dtype}, "
                          f"{v_pages.dtype}")
@@ -41,23 +44,22 @@ def _check_pages(k_pages, v_pages, block_table, b: int, hd: int, dtype, device):
     if page == 0 or page % 16 or d == 0 or d % 8 or d > MAX_HEAD_DIM or hkv == 0:
         raise ValueError(f"page_size is a multiple of 16 and head_dim a multiple of 8 up to {MAX_HEAD_DIM}: got {page}, {d} "
                          f"({hkv} key heads)")
-    for t in (k_pages, v_pages):
-        st = t.stride()
-        if st[3] != 1 or st[2] != d or st[0] % 8 or st[1] % 8 or t.data_ptr() % 16:
+    for t, st in ((k_pages, ks), (v_pages, vs)):
+        if st[3] != 1 or st[2] != d or (st[0] | st[1]) % 8 or t.data_ptr() % 16:
             raise ValueError("the tokens of a head inside a page are contiguous, and pages and heads start on 16-byte boundaries")
-        if t.device != device:
-            raise ValueError(f"tensors are on {device} and {t.device}")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != b or block_table.stride(1) != 1:
-        raise ValueError(f"block_table is int32 [{b}, pages per sequence] with contiguous rows: got {block_table.dtype} "
-                         f"{tuple(block_table.shape)}")
-    if block_table.device != device:
-        raise ValueError(f"tensors are on {device} and {block_table.device}")
-    if block_table.shape[1] * page > 0x3FFFFFFF:
+    table = block_table.shape
+    row, col = block_table.stride() if len(table) == 2 else (0, 0)
+    if block_table.dtype != torch.int32 or len(table) != 2 or table[0] != b or (col != 1 and table[1] > 1):
+        raise ValueError(f"block_table is int32 [{b}, pages per sequence] with contiguous rows: got {block_table.dtype} {tuple(table)}")
+    if k_pages.device != device or v_pages.device != device or block_table.device != device:
+        raise ValueError(f"tensors are on {device}, {k_pages.device}, {v_pages.device} and {block_table.device}")
+    if table[1] * page > 0x3FFFFFFF:
         raise ValueError("block_table spans more than 2**30 tokens")
+    return pages, hkv, page, table[1], row, ks, vs
 
 
 def _check_ints(name, t, b: int, device):
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != b or not t.is_contiguous() or t.device != device:
+    if t.dtype != torch.int32 or t.shape != (b,) or not t.is_contiguous() or t.device != device:
         raise ValueError(f"{name} is a contiguous int32 tensor [{b}] on {device}: got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
@@ -69,13 +71,12 @@ def _no_grad(*tensors):
 
 
 def _aligned(t):
-    """``t`` with unit inner stride and 16-byte aligned heads (a copy where it has not)."""
+    """``t`` with unit inner stride and 16-byte aligned heads (a copy where it has not), and its strides."""
     st = t.stride()
-    n = 16 // t.element_size()
-    if st[3] == 1 and not (st[0] % n or st[1] % n or st[2] % n or t.data_ptr() % 16):
-        return t
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    if st[3] == 1 and not ((st[0] | st[1] | st[2]) % (16 // t.element_size()) or t.data_ptr() % 16):
+        return t, st
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.stride()
 
 
 def paged_kv_append(k, v, k_pages, v_pages, block_table, start, count=None, q=None, rope=None):
@@ -90,22 +91,26 @@ def paged_kv_append(k, v, k_pages, v_pages, block_table, start, count=None, q=No
 
     Returns the rotated ``q`` ``[b, s, heads, head_dim]`` as a new tensor (rows of padding are zeros), or ``None`` without ``q``.
     """
-    if k.dim() != 4 or k.shape != v.shape or v.dtype != k.dtype or v.device != k.device:
-        raise ValueError(f"k and v are [b, s, kv_heads, head_dim], both alike: got {tuple(k.shape)} {k.dtype} and {tuple(v.shape)} "
+    shape, dtype, dev = k.shape, k.dtype, k.device
+    if len(shape) != 4 or v.shape != shape or v.dtype != dtype or v.device != dev:
+        raise ValueError(f"k and v are [b, s, kv_heads, head_dim], both alike: got {tuple(shape)} {dtype} and {tuple(v.shape)} "
                          f"{v.dtype}")
-    b, s, hkv, hd = k.shape
-    dev = k.device
+    b, s, hkv, hd = shape
     _no_grad(k, v, q, k_pages, v_pages)
-    _check_pages(k_pages, v_pages, block_table, b, hd, k.dtype, dev)
-    if k_pages.shape[1] != hkv:
-        raise ValueError(f"the pages hold {k_pages.shape[1]} key heads, the tokens {hkv}")
+    pages, heads, page, width, row, kps, vps = _check_pages(k_pages, v_pages, block_table, b, hd, dtype, dev)
+    if heads != hkv:
+        raise ValueError(f"the pages hold {heads} key heads, the tokens {hkv}")
     _check_ints("start", start, b, dev)
     if count is not None:
         _check_ints("count", count, b, dev)
-    if q is not None and (q.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != hd or q.dtype != k.dtype or q.device != dev):
-        raise ValueError(f"q is [{b}, {s}, heads, {hd}] {k.dtype} on {dev}: got {tuple(q.shape)} {q.dtype} on {q.device}")
+    hq = 0
+    if q is not None:
+        qshape = q.shape
+        if len(qshape) != 4 or qshape[0] != b or qshape[1] != s or qshape[3] != hd or q.dtype != dtype or q.device != dev:
+            raise ValueError(f"q is [{b}, {s}, heads, {hd}] {dtype} on {dev}: got {tuple(qshape)} {q.dtype} on {q.device}")
+        hq = qshape[2]
     cos = sin = None
-    rot, neox = 0, True
+    rot, neox, positions = 0, True, 0
     if rope is not None:
         cos, sin, rot, neox = rope
         if rot < 0 or rot % 2 or rot > hd:
@@ -115,25 +120,25 @@ def paged_kv_append(k, v, k_pages, v_pages, block_table, start, count=None, q=No
                     or t.device != dev:
                 raise ValueError(f"the rotation's tables are contiguous float32 [positions, {rot // 2}] on {dev}: got {t.dtype} "
                                  f"{tuple(t.shape)} on {t.device}")
+        positions = cos.shape[0]
     if not k.is_cuda:
         return _append_reference(k, v, k_pages, v_pages, block_table, start, count, q, rope if rot else None)
-    if dev.index != torch.cuda.current_device():
+    index = dev.index
+    if index != _device():
         with torch.cuda.device(dev):
             return paged_kv_append(k, v, k_pages, v_pages, block_table, start, count, q, rope)
-    k, v = _aligned(k), _aligned(v)
-    hq, out, qs = 0, None, (0, 0, 0)
+    k, ks = _aligned(k)
+    v, vs = _aligned(v)
+    out, qs = None, ks
     if q is not None:
-        q = _aligned(q)
-        hq, qs = q.shape[2], q.stride()[:3]
-        out = torch.empty(b, s, hq, hd, dtype=q.dtype, device=dev)
-    strides = (ctypes.c_longlong * 14)(*qs, *k.stride()[:3], *v.stride()[:3], *k_pages.stride()[:2], *v_pages.stride()[:2],
-                                       block_table.stride(0))
-    rc = _fn("oslo_paged_kv_append", _APPEND_ARGS)(
-        q.data_ptr() if hq else None, k.data_ptr(), v.data_ptr(), out.data_ptr() if hq else None, k_pages.data_ptr(), v_pages.data_ptr(),
-        block_table.data_ptr(), start.data_ptr(), count.data_ptr() if count is not None else None, cos.data_ptr() if rot else None,
-        sin.data_ptr() if rot else None, strides, b, s, hq, hkv, hd, rot, 1 if neox else 0, cos.shape[0] if rot else 0,
-        k_pages.shape[2], block_table.shape[1], k_pages.shape[0], _DT[k.dtype], _lib.status_word(dev).data_ptr(),
-        _raw_stream(dev.index))
+        out = torch.empty(qshape, dtype=dtype, device=dev)
+        q, qs = _aligned(q)
+    rc = _fn("oslo_paged_kv_append")(_APPEND_ARGS.pack(
+        q.data_ptr() if hq else 0, k.data_ptr(), v.data_ptr(), out.data_ptr() if hq else 0, k_pages.data_ptr(), v_pages.data_ptr(),
+        block_table.data_ptr(), start.data_ptr(), count.data_ptr() if count is not None else 0, cos.data_ptr() if rot else 0,
+        sin.data_ptr() if rot else 0, _status_ptr(index), _raw_stream(index),
+        qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], kps[0], kps[1], vps[0], vps[1], row,
+        b, s, hq, hkv, hd, rot, 1 if neox else 0, positions, page, width, pages, _DT[dtype]))
     if rc:
         raise RuntimeError(f"oslo_paged_kv_append failed ({rc})")
     return out
@@ -150,14 +155,13 @@ def paged_attention(q, k_pages, v_pages, block_table, lengths, scale: Optional[f
 
     Returns ``[b, s, heads * head_dim]``, like :func:`oslo_b200.ops.attention.attention`.
     """
-    if q.dim() != 4:
-        raise ValueError(f"q is [b, s, heads, head_dim]: got {tuple(q.shape)}")
-    b, s, hq, hd = q.shape
-    dev = q.device
+    shape, dtype, dev = q.shape, q.dtype, q.device
+    if len(shape) != 4:
+        raise ValueError(f"q is [b, s, heads, head_dim]: got {tuple(shape)}")
+    b, s, hq, hd = shape
     _no_grad(q, k_pages, v_pages, mask)
-    _check_pages(k_pages, v_pages, block_table, b, hd, q.dtype, dev)
+    pages, hkv, page, width, row, ks, vs = _check_pages(k_pages, v_pages, block_table, b, hd, dtype, dev)
     _check_ints("lengths", lengths, b, dev)
-    hkv = k_pages.shape[1]
     if hq == 0 or hq % hkv:
         raise ValueError(f"{hq} query heads do not share {hkv} key heads evenly")
     scale = float(scale) if scale is not None else 1.0 / math.sqrt(hd)
@@ -171,53 +175,53 @@ def paged_attention(q, k_pages, v_pages, block_table, lengths, scale: Optional[f
         mask = mask.float()
     if not q.is_cuda:
         return _attention_reference(q, k_pages, v_pages, block_table, lengths, scale, mask)
-    if dev.index != torch.cuda.current_device():
+    index = dev.index
+    if index != _device():
         with torch.cuda.device(dev):
             return paged_attention(q, k_pages, v_pages, block_table, lengths, scale, mask)
-    q = _aligned(q)
-    out = torch.empty(b, s, hq * hd, dtype=q.dtype, device=dev)
-    ms, mlen = (0, 0), 0
+    q, qs = _aligned(q)
+    out = torch.empty((b, s, hq * hd), dtype=dtype, device=dev)
+    most = width * page
+    mptr = mb = mt = mlen = 0
     if mask is not None:
-        mask = mask.expand(b, 1, s, mask.shape[3])
+        mlen = mask.shape[3]
+        mask = mask.expand(b, 1, s, mlen)
         if mask.stride(3) != 1:
             mask = mask.contiguous()
-        ms, mlen = (mask.stride(0), mask.stride(2)), mask.shape[3]
-    d_index = dev.index
-    masked = mask is not None
-    blocks, block_bytes = _attention_plan(_DT[q.dtype], hd, hq // hkv, masked, d_index)
-    qs, ks, vs = q.stride(), k_pages.stride(), v_pages.stride()
-    pages, _, page, _ = k_pages.shape
-    width = block_table.shape[1]
+        mptr, mb, mt = mask.data_ptr(), mask.stride(0), mask.stride(2)
+        most = min(most, mlen)
+    group, kind = hq // hkv, _DT[dtype]
+    blocks, block_bytes = _attention_plan(kind, hd, group, mptr != 0, index)
     # no more blocks than the longest possible sequences have work for (in units of 32 tokens, the smallest of the kernel's)
-    most = min(width * page, mlen) if masked else width * page
     grid = max(1, min(blocks, b * s * hq * -(-most // 32)))
-    ws = torch.empty(grid * block_bytes, dtype=torch.uint8, device=dev)
-    args = _ATTEND_ARGS.pack(
-        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), lengths.data_ptr(),
-        mask.data_ptr() if masked else 0, out.data_ptr(), ws.data_ptr(), _lib.status_word(dev).data_ptr(), _raw_stream(d_index),
-        qs[0], qs[1], qs[2], ks[0], ks[1], vs[0], vs[1], block_table.stride(0), *ms,
-        b, s, hkv, hq // hkv, hd, page, width, pages, mlen, _DT[q.dtype], grid, grid * block_bytes, scale)
-    rc = _fn("oslo_paged_attention", _PACKED)(args)
+    room = grid * block_bytes
+    ws = torch.empty(room, dtype=torch.uint8, device=dev)
+    rc = _fn("oslo_paged_attention")(_ATTEND_ARGS.pack(
+        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), lengths.data_ptr(), mptr, out.data_ptr(),
+        ws.data_ptr(), _status_ptr(index), _raw_stream(index), qs[0], qs[1], qs[2], ks[0], ks[1], vs[0], vs[1], row, mb, mt,
+        b, s, hkv, group, hd, page, width, pages, mlen, kind, grid, room, scale))
     if rc:
         raise RuntimeError(f"oslo_paged_attention failed ({rc})")
     return out
 
 
-_P, _I = ctypes.c_void_p, ctypes.c_int
-_APPEND_ARGS = [_P] * 12 + [_I] * 12 + [_P, _P]
-_PACKED = [ctypes.c_char_p]  # a struct of eight-byte fields
+# arguments travel as one struct of eight-byte fields: ctypes converts one value instead of forty
+_APPEND_ARGS = struct.Struct("=39q")
 _ATTEND_ARGS = struct.Struct("=32qd")
 _fns = {}
 
 
-def _fn(name, argtypes):
-    """The library's entry point with its argument types set, so that ctypes converts plain numbers."""
+def _fn(name):
     fn = _fns.get(name)
     if fn is None:
-        lib = _lib.cuda_lib()
-        getattr(_lib._load_cuda_lib(), name).argtypes = argtypes
-        fn = _fns[name] = getattr(lib, name)
+        getattr(_lib._load_cuda_lib(), name).argtypes = [ctypes.c_char_p]
+        fn = _fns[name] = getattr(_lib.cuda_lib(), name)
     return fn
+
+
+@lru_cache(maxsize=None)
+def _status_ptr(device: int) -> int:
+    return _lib.status_word(torch.device("cuda", device)).data_ptr()
 
 
 @lru_cache(maxsize=None)
