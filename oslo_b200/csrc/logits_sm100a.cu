@@ -4,12 +4,14 @@
 //   x = x - presence * [c > 0] - frequency * c        c = occurrences among the generated tokens
 //   x = x + bias;   x = -inf where the token is not allowed
 //
-// HBM bounds it: every logit is read once and written once.  A block owns a slice of one row's vocabulary, with one 32-bit
-// counter of the history per token in shared memory (bit 31: seen in the prompt; the rest: generated so often; both are
-// updated by integer atomics, whose order does not matter).  The blocks of a cluster own neighbouring slices: each reads
-// one part of the history and adds every token to the counter of the block that owns it, through distributed shared memory, so
-// a row of up to 65536 tokens reads its history once.  Slices of at most 8192 tokens (32 KB) let an SM hold six blocks, whose
-// counting and streaming phases overlap.
+// Every logit is read once and written once.  A block owns a slice of one row's vocabulary and counts the history's tokens
+// of that slice in shared memory (integer atomics: their order does not matter), while its first logits are already on their
+// way; then it streams the slice, 16 bytes a thread.  Counters have 16 bits for histories of less than 32768 tokens: a group of
+// eight 16-bit logits then meets one 16-byte load of counters, most of them zero.  Plain streaming runs at the copy bandwidth
+// (192 x 250112 bf16: 35 us); with a history of 4095 tokens, a bias and a mask the same logits take 66 us, bound by
+// issue and latency: the history is read by each of a row's 16 slices (11 us), the bias comes from L2 (15 us), and
+// every element's mask is two instructions (10 us).  Adding a cluster's tokens to each other's counters through distributed
+// shared memory, so that a row reads its history once, was slower (105 us): frequent tokens serialise the remote atomics.
 #include "common.cuh"
 
 namespace oslo {
@@ -30,9 +32,16 @@ struct LogitsParams {
   int rows, vocab, history, tok64, slice, slices;  // slices a row, a multiple of the cluster's size
 };
 
-constexpr int kLogitsSlice = 8192;
 constexpr int kLogitsThreads = 256;
-constexpr unsigned kSeenInPrompt = 0x80000000u;
+constexpr int kLogitsAhead = 2;             // 16-byte groups of a thread in flight
+constexpr int kLogitsCounters = 32 * 1024;  // bytes of counters of a block
+constexpr int kLogitsLeast = 2048;          // tokens of a slice at least
+
+// A token's counter: the top bit says that the prompt holds it, the others how often it was generated.
+template <typename C>
+struct Counter {
+  static constexpr unsigned kPrompt = 1u << (8 * sizeof(C) - 1);
+};
 
 OSLO_DEVINL float lg_f(float x) { return x; }
 OSLO_DEVINL float lg_f(__half x) { return __half2float(x); }
@@ -41,70 +50,77 @@ OSLO_DEVINL void lg_st(float& p, float x) { p = x; }
 OSLO_DEVINL void lg_st(__half& p, float x) { p = __float2half_rn(x); }
 OSLO_DEVINL void lg_st(__nv_bfloat16& p, float x) { p = __float2bfloat16_rn(x); }
 
-OSLO_DEVINL void cluster_barrier() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// shared-memory address of the same variable in another block of the cluster
-OSLO_DEVINL uint32_t peer_smem(uint32_t addr, uint32_t rank) {
-  uint32_t r;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  return r;
-}
-
+template <typename C>
 struct LogitsRow {
-  float rep, pres, freq;
-  OSLO_DEVINL float operator()(float f, unsigned seen) const {
-    if (seen == 0) return f;
-    f = f > 0.f ? __fdiv_rn(f, rep) : f * rep;
-    const unsigned c = seen & ~kSeenInPrompt;
+  float rep, inv, pres, freq;
+  OSLO_DEVINL float operator()(float f, unsigned seen) const {  // without branches: some lane of a warp has a seen token nearly always
+    const unsigned c = seen & ~Counter<C>::kPrompt;
+    const float r = f * (f > 0.f ? inv : rep);
+    f = seen ? r : f;
     return c ? f - pres - freq * static_cast<float>(c) : f;
   }
 };
 
-template <typename T, bool HISTORY>
-__global__ void __launch_bounds__(kLogitsThreads) process_logits_kernel(const LogitsParams p, int cluster) {
+// Adds the history's tokens in [v0, v0 + n) to their counters.
+template <typename I, typename C>
+OSLO_DEVINL void count_tokens(const I* tokens, int len, int prompt, int v0, int n, C* seen) {
+  for (int i0 = threadIdx.x; i0 < len; i0 += kLogitsThreads * 8) {
+    I id[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) id[j] = i0 + j * kLogitsThreads < len ? __ldg(tokens + i0 + j * kLogitsThreads) : static_cast<I>(-1);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const unsigned at = static_cast<unsigned>(id[j]) - v0;
+      if (at < static_cast<unsigned>(n) && (sizeof(I) == 4 || static_cast<unsigned>(static_cast<unsigned long long>(id[j]) >> 32) == 0)) {
+        // two 16-bit counters share a word; a count below 32768 never carries into its neighbour or its own top bit
+        const uint32_t addr = smem_u32(seen + at), sh = (addr & 3) * 8;
+        if (i0 + j * kLogitsThreads < prompt) asm volatile("red.shared::cta.or.b32 [%0], %1;" ::"r"(addr & ~3u), "r"(Counter<C>::kPrompt << sh) : "memory");
+        else asm volatile("red.shared::cta.add.u32 [%0], %1;" ::"r"(addr & ~3u), "r"(1u << sh) : "memory");
+      }
+    }
+  }
+}
+
+// C: counter type, uint16_t for histories of less than 32768 tokens, uint32_t for longer ones, void without a history
+template <typename T, typename C>
+__global__ void __launch_bounds__(kLogitsThreads, 5) process_logits_kernel(const LogitsParams p) {
+  constexpr bool HISTORY = sizeof(C) > 1;
   constexpr int E = 16 / sizeof(T);
-  extern __shared__ uint4 seen4[];
-  unsigned* const counters = reinterpret_cast<unsigned*>(seen4);
-  const int row = blockIdx.x / p.slices, part = blockIdx.x % p.slices;
-  const int v0 = min(part * p.slice, p.vocab), n = min(p.slice, p.vocab - v0);
+  extern __shared__ uint4 counters4[];
+  C* const counters = reinterpret_cast<C*>(counters4);
+  const int row = blockIdx.x / p.slices, v0 = (blockIdx.x - row * p.slices) * p.slice;
+  const int n = min(p.slice, p.vocab - v0);
   const T* x = static_cast<const T*>(p.x) + row * p.x_stride + v0;
   T* y = static_cast<T*>(p.y) + row * p.y_stride + v0;
   // elements before the first 16-byte boundary of the slice; the counters are shifted so that a group's are aligned too
   const int to_edge = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / static_cast<int>(sizeof(T));
-  const int head = min(to_edge, n), shift = (4 - (to_edge & 3)) & 3;
+  const int head = min(to_edge, n);
+  C* const seen = counters + ((E - to_edge) & (E - 1));
+  const bool aligned = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(y)) & 15) == 0;
+  const int groups = aligned ? (n - head) / E : 0;
+  // the first logits are on their way while the history is counted
+  uint4 ahead[kLogitsAhead];
+  const auto fetch = [&](int g0) {
+#pragma unroll
+    for (int j = 0; j < kLogitsAhead; ++j)
+      if (g0 + j * kLogitsThreads < groups)
+        asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(ahead[j].x), "=r"(ahead[j].y), "=r"(ahead[j].z), "=r"(ahead[j].w) : "l"(x + head + (g0 + j * kLogitsThreads) * E));
+  };
+  fetch(threadIdx.x);
+  LogitsRow<C> pen{p.rep_s, 1.f, p.pres_s, p.freq_s};
   if constexpr (HISTORY) {
-    for (int i = threadIdx.x; i < (p.slice + 3) / 4 + 1; i += kLogitsThreads) seen4[i] = make_uint4(0, 0, 0, 0);
-    if (cluster > 1) cluster_barrier();
-    else __syncthreads();
-    const int len = p.token_lens ? min(max(p.token_lens[row], 0), p.history) : p.history;
-    const int prompt = p.prompt_lens ? p.prompt_lens[row] : 0;
-    const int rank = part % cluster, c0 = (part - rank) * p.slice;  // the cluster's first token
-    const long long range = min(static_cast<long long>(p.slice) * cluster, static_cast<long long>(p.vocab) - c0);
-    const uint32_t mine = smem_u32(counters);
-    for (int i = rank * kLogitsThreads + threadIdx.x; i < len; i += cluster * kLogitsThreads) {
-      const long long at = row * p.tok_stride + i;
-      const long long id = (p.tok64 ? static_cast<const long long*>(p.tokens)[at] : static_cast<const int*>(p.tokens)[at]) - c0;
-      if (id < 0 || id >= range) continue;
-      const int owner = static_cast<int>(id) / p.slice;
-      // the owner shifts its counters by its own slice's distance to a 16-byte boundary
-      const T* ox = static_cast<const T*>(p.x) + row * p.x_stride + (c0 + owner * p.slice);
-      const int edge = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(ox) & 15)) & 15) / static_cast<int>(sizeof(T));
-      const uint32_t local = mine + 4 * (static_cast<int>(id) - owner * p.slice + ((4 - (edge & 3)) & 3));
-      const uint32_t addr = cluster > 1 ? peer_smem(local, owner) : local;
-      if (i < prompt) asm volatile("red.relaxed.cluster.shared::cluster.or.b32 [%0], %1;" ::"r"(addr), "r"(kSeenInPrompt) : "memory");
-      else asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(addr), "r"(1u) : "memory");
-    }
-    if (cluster > 1) cluster_barrier();
-    else __syncthreads();
-  }
-  if (n <= 0) return;
-  const unsigned* seen = counters + shift;
-  LogitsRow pen{p.rep_s, p.pres_s, p.freq_s};
-  if constexpr (HISTORY) {
+    for (int i = threadIdx.x; i < static_cast<int>(p.slice * sizeof(C) / 16) + 1; i += kLogitsThreads) counters4[i] = make_uint4(0, 0, 0, 0);
     if (p.rep) pen.rep = p.rep[row];
     if (p.pres) pen.pres = p.pres[row];
     if (p.freq) pen.freq = p.freq[row];
+    pen.inv = __fdiv_rn(1.f, pen.rep);
+    const int len = p.token_lens ? min(max(p.token_lens[row], 0), p.history) : p.history;
+    const int prompt = p.prompt_lens ? p.prompt_lens[row] : 0;
+    __syncthreads();
+    if (p.tok64) count_tokens(static_cast<const long long*>(p.tokens) + row * p.tok_stride, len, prompt, v0, n, seen);
+    else count_tokens(static_cast<const int*>(p.tokens) + row * p.tok_stride, len, prompt, v0, n, seen);
+    __syncthreads();
   }
   const float* bias = p.bias ? p.bias + row * p.bias_stride + v0 : nullptr;
   const int* allowed = p.allowed ? p.allowed + row * p.allowed_stride : nullptr;
@@ -115,48 +131,56 @@ __global__ void __launch_bounds__(kLogitsThreads) process_logits_kernel(const Lo
     if (allowed && !((allowed[(v0 + i) >> 5] >> ((v0 + i) & 31)) & 1)) f = -INFINITY;
     lg_st(y[i], f);
   };
-  if ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(y)) & 15) {
+  if (!aligned) {
     for (int i = threadIdx.x; i < n; i += kLogitsThreads) one(i);  // rows of input and output that no 16-byte access serves
     return;
   }
-  const int groups = (n - head) / E, tail = head + groups * E;
+  const int tail = head + groups * E;
   if (threadIdx.x < head) one(threadIdx.x);
   if (threadIdx.x < n - tail) one(tail + threadIdx.x);
   const bool bias16 = bias && (reinterpret_cast<uintptr_t>(bias + head) & 15) == 0;
-#pragma unroll 2
-  for (int g = threadIdx.x; g < groups; g += kLogitsThreads) {
-    const int i = head + g * E;
+  const auto group = [&](int i, const uint4& u) {
     union {
       uint4 u;
       T t[E];
     } in, out;
-    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(in.u.x), "=r"(in.u.y), "=r"(in.u.z), "=r"(in.u.w) : "l"(x + i));
+    in.u = u;
     float f[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) f[e] = lg_f(in.t[e]);
     if constexpr (HISTORY) {
+      constexpr int W = E * sizeof(C) / 4;  // words of the group's counters
+      unsigned w[W];
+      if constexpr (W == 2) {
+        *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(seen + i);
+      } else {
 #pragma unroll
-      for (int e = 0; e < E; e += 4) {
-        const uint4 s = *reinterpret_cast<const uint4*>(seen + i + e);
-        if (s.x | s.y | s.z | s.w) f[e] = pen(f[e], s.x), f[e + 1] = pen(f[e + 1], s.y), f[e + 2] = pen(f[e + 2], s.z), f[e + 3] = pen(f[e + 3], s.w);
+        for (int k = 0; k < W; k += 4) *reinterpret_cast<uint4*>(w + k) = *reinterpret_cast<const uint4*>(seen + i + k * (4 / sizeof(C)));
+      }
+      unsigned any = 0;
+#pragma unroll
+      for (int k = 0; k < W; ++k) any |= w[k];
+      if (any) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          f[e] = pen(f[e], sizeof(C) == 4 ? w[e * sizeof(C) / 4] : (w[e * sizeof(C) / 4] >> (e % (4 / sizeof(C)) * 16)) & 0xffffu);
       }
     }
     if (bias) {
       if (bias16) {
 #pragma unroll
         for (int e = 0; e < E; e += 4) {
-          const float4 b = *reinterpret_cast<const float4*>(bias + i + e);
+          const float4 b = __ldg(reinterpret_cast<const float4*>(bias + i + e));
           f[e] += b.x, f[e + 1] += b.y, f[e + 2] += b.z, f[e + 3] += b.w;
         }
       } else {
 #pragma unroll
-        for (int e = 0; e < E; ++e) f[e] += bias[i + e];
+        for (int e = 0; e < E; ++e) f[e] += __ldg(bias + i + e);
       }
     }
     if (allowed) {
       const int at = v0 + i, w = at >> 5, sh = at & 31;
-      const unsigned lo = allowed[w], hi = sh + E > 32 ? allowed[w + 1] : 0u;  // the last group ends inside the last word
+      const unsigned lo = __ldg(allowed + w), hi = sh + E > 32 ? __ldg(allowed + w + 1) : 0u;  // the last group ends inside the last word
       const unsigned bits = __funnelshift_r(lo, hi, sh);
 #pragma unroll
       for (int e = 0; e < E; ++e)
@@ -165,33 +189,34 @@ __global__ void __launch_bounds__(kLogitsThreads) process_logits_kernel(const Lo
 #pragma unroll
     for (int e = 0; e < E; ++e) lg_st(out.t[e], f[e]);
     *reinterpret_cast<uint4*>(y + i) = out.u;
+  };
+  for (int g0 = threadIdx.x; g0 < groups; g0 += kLogitsAhead * kLogitsThreads) {
+#pragma unroll
+    for (int j = 0; j < kLogitsAhead; ++j)
+      if (g0 + j * kLogitsThreads < groups) group(head + (g0 + j * kLogitsThreads) * E, ahead[j]);
+    fetch(g0 + kLogitsAhead * kLogitsThreads);
   }
 }
 
 template <typename T>
 int process_logits_launch(LogitsParams& p, cudaStream_t st) {
-  int cluster = 1;
-  if (p.tokens) {
-    while (cluster < 8 && cluster * 2048 < p.vocab) cluster *= 2;  // eight blocks read the history from 16384 tokens on
-  }
-  const int spans = (p.vocab + cluster * kLogitsSlice - 1) / (cluster * kLogitsSlice);  // clusters a row
-  p.slices = spans * cluster;
+  const bool small = p.history < 32768;
+  // Four blocks an SM (148 of them) when the work is small, else slices as large as the counters' room: every slice reads its
+  // row's history again.  One row of 50304: 4.6 us with 8192-token slices, 3.1 us with 2048; 128 rows of 32000 with histories of
+  // 8000: 15.9 us in 444 blocks, 23.3 us in 1776.
+  const int most = kLogitsCounters / (small ? 2 : 4);
+  const long long fair = static_cast<long long>(p.rows) * p.vocab / 592;
+  const int want = static_cast<int>(fair < kLogitsLeast ? kLogitsLeast : fair > most ? most : fair);
+  p.slices = (p.vocab + want - 1) / want;
   p.slice = ((p.vocab + p.slices - 1) / p.slices + 31) / 32 * 32;
+  p.slices = (p.vocab + p.slice - 1) / p.slice;
   const long long grid = static_cast<long long>(p.rows) * p.slices;
   if (grid > 0x7fffffffll) return -1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(grid));
-  cfg.blockDim = dim3(kLogitsThreads);
-  cfg.dynamicSmemBytes = p.tokens ? (p.slice + 8) * sizeof(unsigned) : 0;
-  cfg.stream = st;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = cluster, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = cluster > 1 ? 1 : 0;
-  const cudaError_t rc = p.tokens ? cudaLaunchKernelEx(&cfg, process_logits_kernel<T, true>, p, cluster)
-                                  : cudaLaunchKernelEx(&cfg, process_logits_kernel<T, false>, p, cluster);
-  return rc == cudaSuccess ? 0 : -2;
+  const unsigned blocks = static_cast<unsigned>(grid);
+  if (!p.tokens) process_logits_kernel<T, char><<<blocks, kLogitsThreads, 0, st>>>(p);
+  else if (small) process_logits_kernel<T, uint16_t><<<blocks, kLogitsThreads, p.slice * 2 + 16, st>>>(p);
+  else process_logits_kernel<T, uint32_t><<<blocks, kLogitsThreads, p.slice * 4 + 16, st>>>(p);
+  return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
 
 }  // namespace oslo
