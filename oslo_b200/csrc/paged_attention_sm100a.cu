@@ -14,11 +14,15 @@
 // second kernel, launched programmatically so that its start overlaps the first one's end; the parts are added in block order,
 // so results do not depend on timing.
 //
-// The tiles go from HBM straight into the registers in the layout that mma.sync wants as its B operand, 16 bytes per load and
-// without shared memory, because the order of the summed index is free as long as both operands share it:
+// Each warp has a ring of tiles in shared memory, filled by 16-byte asynchronous copies that run ahead of the products; rows
+// that the query does not see are filled with zeros and never read, so they may hold anything.  The products are mma.sync with
+// the operands read 16 bytes at a time, without a transpose, because the order of the summed index is free as long as both
+// operands share it:
 //   scores   lane (r, q) = (lane / 4, lane % 4) holds 16 contiguous bytes of key r; Q is loaded with the same pattern.
 //   output   the accumulator columns of the scores (tokens 2q, 2q + 1) are the A operand's summed index, so lane (r, q) loads
 //            the values of exactly those tokens, 16 bytes at head dim r * E of each 8 E wide block.
+// (Rows of the ring are 16 bytes longer than a head, which keeps the value loads free of bank conflicts.)  tcgen05 would
+// multiply 128 rows where there are 1 to 16: the tensor cores are not what bounds this.
 // The probabilities enter the second product as the sum of two 16-bit numbers (high part and remainder), which keeps 16 bits
 // and more of each; fp32 inputs are split in the same way into tf32 parts (three products), which keeps 21 bits.
 #include "common.cuh"
@@ -42,8 +46,12 @@ struct PagedAttnParams {
   float scale;
 };
 
-//: units a block takes at least
-constexpr int kMinUnits = 2;
+#ifndef OV
+#define OV 2
+#define MU 4
+#endif
+constexpr int kSegmentUnits = OV;
+constexpr int kMinUnits = MU;
 
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -51,6 +59,15 @@ OSLO_DEVINL uint4 ldg16(const void* p) {
   uint4 r;
   asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
   return r;
+}
+// 16 bytes into shared memory, asynchronously; zeros where `valid` is false (nothing is read then)
+OSLO_DEVINL void copy16(void* dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+OSLO_DEVINL void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+OSLO_DEVINL void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 OSLO_DEVINL float ex2(float x) {
   float y;
@@ -131,9 +148,15 @@ struct PagedAttn {
   static constexpr int RT = WIDE ? 16 : 8;  // query rows
   static constexpr int ROW = DP + 4;        // padded row of the joining buffer
   static constexpr int WARPS = 4;
-  // Blocks an SM should hold: enough loads in flight to cover HBM's latency (8 KB a warp and tile) without spilling.
-  static constexpr int BLOCKS = DP == 64 ? (sizeof(T) == 2 ? 4 : 2) : DP == 128 && sizeof(T) == 2 && !WIDE ? 3 : 2;
-  static constexpr size_t kSmem = sizeof(float) * (WARPS * RT * ROW + 2 * WARPS * RT);
+  static constexpr int PITCH = DP + E;  // elements between two rows of a tile in the ring
+  static constexpr int TILE = TT * PITCH * 2;  // keys, then values
+  static constexpr int STAGES = DP == 64 ? 3 : 2;
+  // Blocks an SM should hold; the ring's size is chosen for it.
+  static constexpr int BLOCKS = (DP == 64 ? 4 : DP == 128 ? 3 : 2) - (sizeof(T) == 4 || DP == 256 ? 1 : 0);
+  static constexpr size_t kRing = sizeof(T) * TILE * STAGES;  // of one warp; the joining buffer takes its place at the end
+  static constexpr size_t kSmem = kRing * WARPS + sizeof(float) * 2 * WARPS * RT;
+  static_assert(kRing >= sizeof(float) * RT * ROW, "a warp's part of the joining buffer fits its ring");
+  static_assert((kSmem + 1024) * BLOCKS <= 227 * 1024 + 1024, "shared memory of the blocks of an SM");
 
   uint4 q0[KC], q1[WIDE ? KC : 1];
   float o[VC][E][WIDE ? 4 : 2];
@@ -160,10 +183,38 @@ struct PagedAttn {
         for (int x = 0; x < (WIDE ? 4 : 2); ++x) o[j][e][x] = 0.f;
   }
 
-  // One tile: its TT tokens start at `token`; the tile's keys and values at k, v; tokens at or past `limit` are not seen.
-  OSLO_DEVINL void tile(const PagedAttnParams& p, const T* k, const T* v, int token, int limit, const float* mask) {
+  // Starts the copy of one tile, `rows` of whose tokens are seen, into the ring.
+  static OSLO_DEVINL void fill(const PagedAttnParams& p, T* ring, const T* k, const T* v, int rows) {
+    constexpr int CHUNKS = DP / E;
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const T* src = half ? v : k;
+      T* dst = ring + half * TT * PITCH;
+#pragma unroll
+      for (int i = 0; i < TT * CHUNKS / 32; ++i) {
+        const int row = (i * 32 + lane) / CHUNKS, c = (i * 32 + lane) % CHUNKS;
+        const bool valid = row < rows && c * E < p.d;
+        copy16(dst + row * PITCH + c * E, valid ? src + row * p.d + c * E : src, valid);
+      }
+    }
+  }
+
+  // Block j of the values of this lane's tokens.
+  static OSLO_DEVINL void load_v(uint4 (&vr)[VT], const T* ring, int j, const bool (&seen)[NT][2]) {
     const int lane = threadIdx.x & 31, r = lane >> 2, quad = lane & 3;
-    uint4 kr[NT][KC], vr[VT][VC];
+#pragma unroll
+    for (int t = 0; t < VT; ++t) {
+      vr[t] = *reinterpret_cast<const uint4*>(ring + TT * PITCH + ((t >> 1) * 8 + quad * 2 + (t & 1)) * PITCH + j * 8 * E + r * E);
+      if constexpr (MASK) {  // a masked token may hold anything: its values do not enter the product
+        if (!seen[t >> 1][t & 1]) vr[t] = make_uint4(0, 0, 0, 0);
+      }
+    }
+  }
+
+  // One tile of the ring: its TT tokens start at `token`; tokens at or past `limit` are not seen.
+  OSLO_DEVINL void tile(const PagedAttnParams& p, const T* ring, int token, int limit, const float* mask) {
+    const int lane = threadIdx.x & 31, r = lane >> 2, quad = lane & 3;
     float add[NT][2];
     bool seen[NT][2];
 #pragma unroll
@@ -178,21 +229,6 @@ struct PagedAttn {
           seen[n][x] = seen[n][x] && add[n][x] != -INFINITY;
         }
       }
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int c = 0; c < KC; ++c) {
-        const int dim = c * 4 * E + quad * E;
-        kr[n][c] = dim < p.d ? ldg16(k + (n * 8 + r) * p.d + dim) : make_uint4(0, 0, 0, 0);
-      }
-#pragma unroll
-    for (int t = 0; t < VT; ++t)
-#pragma unroll
-      for (int c = 0; c < VC; ++c) {
-        const int dim = c * 8 * E + r * E;
-        // a token that is not seen may hold anything: its values never enter the product
-        vr[t][c] = dim < p.d && seen[t >> 1][t & 1] ? ldg16(v + ((t >> 1) * 8 + quad * 2 + (t & 1)) * p.d + dim) : make_uint4(0, 0, 0, 0);
-      }
     float sc[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -200,14 +236,15 @@ struct PagedAttn {
 #pragma unroll
       for (int c = 0; c < KC; ++c) {
         const uint4 qa = q0[c], qb = WIDE ? q1[WIDE ? c : 0] : make_uint4(0, 0, 0, 0);
+        const uint4 kr = *reinterpret_cast<const uint4*>(ring + (n * 8 + r) * PITCH + c * 4 * E + quad * E);
         if constexpr (sizeof(T) == 2) {
-          Mma16<T>::run(sc[n], qa.x, qb.x, qa.y, qb.y, kr[n][c].x, kr[n][c].y);
-          Mma16<T>::run(sc[n], qa.z, qb.z, qa.w, qb.w, kr[n][c].z, kr[n][c].w);
+          Mma16<T>::run(sc[n], qa.x, qb.x, qa.y, qb.y, kr.x, kr.y);
+          Mma16<T>::run(sc[n], qa.z, qb.z, qa.w, qb.w, kr.z, kr.w);
         } else {
           const float a[4] = {__uint_as_float(qa.x), __uint_as_float(qb.x), __uint_as_float(qa.y), __uint_as_float(qb.y)};
           const float b[4] = {__uint_as_float(qa.z), __uint_as_float(qb.z), __uint_as_float(qa.w), __uint_as_float(qb.w)};
-          mma_3xtf32(sc[n], a, __uint_as_float(kr[n][c].x), __uint_as_float(kr[n][c].y));
-          mma_3xtf32(sc[n], b, __uint_as_float(kr[n][c].z), __uint_as_float(kr[n][c].w));
+          mma_3xtf32(sc[n], a, __uint_as_float(kr.x), __uint_as_float(kr.y));
+          mma_3xtf32(sc[n], b, __uint_as_float(kr.z), __uint_as_float(kr.w));
         }
       }
     }
@@ -267,10 +304,12 @@ struct PagedAttn {
       if constexpr (!WIDE) hi[1] = hi[3] = lo[1] = lo[3] = 0;
 #pragma unroll
       for (int j = 0; j < VC; ++j) {
-        const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&vr[0][j]);
-        const uint32_t* w1 = reinterpret_cast<const uint32_t*>(&vr[1][j]);
-        const uint32_t* w2 = reinterpret_cast<const uint32_t*>(&vr[2][j]);
-        const uint32_t* w3 = reinterpret_cast<const uint32_t*>(&vr[3][j]);
+        uint4 vr[VT];
+        load_v(vr, ring, j, seen);
+        const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&vr[0]);
+        const uint32_t* w1 = reinterpret_cast<const uint32_t*>(&vr[1]);
+        const uint32_t* w2 = reinterpret_cast<const uint32_t*>(&vr[2]);
+        const uint32_t* w3 = reinterpret_cast<const uint32_t*>(&vr[3]);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
           const uint32_t sel = e & 1 ? 0x7632 : 0x5410;
@@ -286,8 +325,10 @@ struct PagedAttn {
       const float a[4] = {sc[0][0], WIDE ? sc[0][2] : 0.f, sc[0][1], WIDE ? sc[0][3] : 0.f};
 #pragma unroll
       for (int j = 0; j < VC; ++j) {
-        const float* w0 = reinterpret_cast<const float*>(&vr[0][j]);
-        const float* w1 = reinterpret_cast<const float*>(&vr[1][j]);
+        uint4 vr[VT];
+        load_v(vr, ring, j, seen);
+        const float* w0 = reinterpret_cast<const float*>(&vr[0]);
+        const float* w1 = reinterpret_cast<const float*>(&vr[1]);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
           float c[4] = {o[j][e][0], o[j][e][1], WIDE ? o[j][e][WIDE ? 2 : 0] : 0.f, WIDE ? o[j][e][WIDE ? 3 : 0] : 0.f};
@@ -309,8 +350,56 @@ struct PagedAttn {
     return ex2(MASK ? (x - mm) * kLog2e : x - mm);
   }
 
-  // Joins the warps' sums.  Afterwards every thread may read row sums / maxima (ml) and the output (buf, unnormalised).
-  OSLO_DEVINL void join(float* buf, float* ml) {
+  // Row maxima of the four warps, then their row sums.
+  static OSLO_DEVINL float* ml_of(char* smem) { return reinterpret_cast<float*>(smem + kRing * WARPS); }
+
+  // Attends over tokens [begin, end) of a segment with all warps of the block and joins them.
+  OSLO_DEVINL void walk(const PagedAttnParams& p, char* smem, int query, int h, int row0, int limit, int begin, int end) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int b = query / p.s, i = query - b * p.s;
+    const float* mask = MASK ? p.mask + b * p.m_sb + i * p.m_ss : nullptr;
+    const int* table = p.table + b * p.table_stride;
+    T* ring = reinterpret_cast<T*>(smem + kRing * warp);
+    const T* k = static_cast<const T*>(p.k) + h * p.k_head;
+    const T* v = static_cast<const T*>(p.v) + h * p.v_head;
+    constexpr int STEP = WARPS * TT;
+    int ahead = begin + warp * TT;  // the next tile to copy, and its page
+    int page = ahead < end ? table[ahead / p.page_size] : 0;
+    unsigned missing = 0;  // bit i: the tile in slot i of the ring has no page
+    const auto advance = [&](int slot) {
+      if (ahead < end) {
+        const bool ok = page >= 0 && page < p.num_pages;
+        const long long in_page = static_cast<long long>(ahead % p.page_size) * p.d;
+        fill(p, ring + slot * TILE, ok ? k + page * p.k_page + in_page : k, ok ? v + page * p.v_page + in_page : v, ok ? limit - ahead : 0);
+        missing = (missing & ~(1u << slot)) | (ok ? 0u : 1u << slot);
+        if (!ok && lane == 0) atomicCAS(p.status, kStatusOk, kStatusPageRange);
+        ahead += STEP;
+        if (ahead < end) page = table[ahead / p.page_size];
+      }
+      copy_commit();
+    };
+    int t = ahead;
+#pragma unroll
+    for (int x = 0; x < STAGES; ++x) advance(x);
+    load_q(p, static_cast<const T*>(p.q) + b * p.q_sb + i * p.q_ss + static_cast<long long>(h) * p.group * p.q_sh, row0);
+    clear();
+    for (int slot = 0; t < end; t += STEP) {
+      copy_wait<STAGES - 1>();
+      __syncwarp();
+      tile(p, ring + slot * TILE, t, (missing >> slot) & 1 ? 0 : limit, mask);
+      __syncwarp();
+      advance(slot);
+      slot = slot + 1 == STAGES ? 0 : slot + 1;
+    }
+    copy_wait<0>();
+    __syncwarp();
+    join(ring, ml_of(smem));
+  }
+
+  // Joins the warps' sums.  Afterwards every thread may read row sums / maxima (ml) and the warps' outputs, scaled to the same
+  // maximum, at the start of their rings.
+  OSLO_DEVINL void join(T* ring, float* ml) {
+    float* buf = reinterpret_cast<float*>(ring);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, quad = lane & 3;
     l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
     l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
@@ -336,7 +425,7 @@ struct PagedAttn {
     for (int j = 0; j < VC; ++j)
 #pragma unroll
       for (int x = 0; x < (WIDE ? 4 : 2); ++x) {
-        float* dst = buf + (warp * RT + r + (x >> 1) * 8) * ROW + j * 8 * E + (quad * 2 + (x & 1)) * E;
+        float* dst = buf + (r + (x >> 1) * 8) * ROW + j * 8 * E + (quad * 2 + (x & 1)) * E;
         const float f = x >> 1 ? f1 : f0;
 #pragma unroll
         for (int e = 0; e < E; e += 4)
@@ -356,14 +445,31 @@ OSLO_DEVINL int query_limit(const PagedAttnParams& p, int query, bool report) {
   return static_cast<int>(min(max(limit, 0ll), static_cast<long long>(cap)));
 }
 
+// Sum of the four warps' outputs at (row, dim) after join(), and the row's total.
+template <typename A>
+OSLO_DEVINL float4 block_sum(const char* smem, int row, int dim, float& l, float& m) {
+  const float* ml = A::ml_of(const_cast<char*>(smem));
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  l = 0.f, m = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < A::WARPS; ++w) {
+    l += ml[(A::WARPS + w) * A::RT + row];
+    m = fmaxf(m, ml[w * A::RT + row]);
+    const float4 y = *reinterpret_cast<const float4*>(smem + A::kRing * w + sizeof(float) * (row * A::ROW + dim));
+    s.x += y.x, s.y += y.y, s.z += y.z, s.w += y.w;
+  }
+  return s;
+}
+
+template <int UNIT>
+OSLO_DEVINL int segment_units(int limit) { return kSegmentUnits + max(1, (limit + UNIT - 1) / UNIT); }
+
 template <typename T, int DP, bool WIDE, bool MASK>
 __global__ void __launch_bounds__(128, PagedAttn<T, DP, WIDE, MASK>::BLOCKS) paged_attention_kernel(const PagedAttnParams p) {
   using A = PagedAttn<T, DP, WIDE, MASK>;
   constexpr int UNIT = A::WARPS * A::TT;
   extern __shared__ float4 smem4[];
   __shared__ long long scan[A::WARPS + 2];
-  float* buf = reinterpret_cast<float*>(smem4);
-  float* ml = buf + A::WARPS * A::RT * A::ROW;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
@@ -372,7 +478,7 @@ __global__ void __launch_bounds__(128, PagedAttn<T, DP, WIDE, MASK>::BLOCKS) pag
   const int queries = p.b * p.s, run = (queries + 127) / 128;
   const int first = min(queries, static_cast<int>(threadIdx.x) * run), last = min(queries, first + run);
   long long mine = 0;
-  for (int i = first; i < last; ++i) mine += max(1, (query_limit<MASK>(p, i, false) + UNIT - 1) / UNIT);
+  for (int i = first; i < last; ++i) mine += segment_units<UNIT>(query_limit<MASK>(p, i, false));
   long long incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -399,7 +505,7 @@ __global__ void __launch_bounds__(128, PagedAttn<T, DP, WIDE, MASK>::BLOCKS) pag
   if (mine > 0 && at >= before && at < before + mine) {
     int i = first;
     long long n;
-    while (at >= before + (n = max(1, (query_limit<MASK>(p, i, false) + UNIT - 1) / UNIT))) before += n, ++i;
+    while (at >= before + (n = segment_units<UNIT>(query_limit<MASK>(p, i, false)))) before += n, ++i;
     scan[0] = i;
     scan[1] = before;
   }
@@ -407,41 +513,25 @@ __global__ void __launch_bounds__(128, PagedAttn<T, DP, WIDE, MASK>::BLOCKS) pag
   int query = static_cast<int>(scan[0]);
   long long base = scan[1] * heads;  // first unit of the query
   int limit = query_limit<MASK>(p, query, threadIdx.x == 0);
-  int n_units = max(1, (limit + UNIT - 1) / UNIT);
+  int n_units = segment_units<UNIT>(limit);
 
   while (u < u_end) {
     if (u >= base + static_cast<long long>(n_units) * heads) {
       base += static_cast<long long>(n_units) * heads;
       ++query;
       limit = query_limit<MASK>(p, query, threadIdx.x == 0);
-      n_units = max(1, (limit + UNIT - 1) / UNIT);
+      n_units = segment_units<UNIT>(limit);
     }
     const int seg = static_cast<int>((u - base) / n_units);
-    const int a = static_cast<int>((u - base) - static_cast<long long>(seg) * n_units);
-    const int e = static_cast<int>(min(static_cast<long long>(n_units), a + (u_end - u)));
+    // [a, e) of the segment's units; a range that begins in the units without tokens begins with the segment, and one that ends
+    // there leaves the segment to the next block
+    const int a0 = static_cast<int>((u - base) - static_cast<long long>(seg) * n_units), a = a0 <= kSegmentUnits ? 0 : a0;
+    const int e = static_cast<int>(min(static_cast<long long>(n_units), a0 + (u_end - u)));
+    if (e <= kSegmentUnits) break;
     const int h = seg / p.row_tiles, row0 = (seg - h * p.row_tiles) * A::RT;
-    const int b = query / p.s, i = query - b * p.s;
 
     A acc;
-    acc.load_q(p, static_cast<const T*>(p.q) + b * p.q_sb + i * p.q_ss + static_cast<long long>(h) * p.group * p.q_sh, row0);
-    acc.clear();
-    const float* mask = MASK ? p.mask + b * p.m_sb + i * p.m_ss : nullptr;
-    const int* table = p.table + b * p.table_stride;
-    const int end = min(limit, e * UNIT);
-    int t = a * UNIT + warp * A::TT;
-    int page = t < end ? table[t / p.page_size] : 0;
-    while (t < end) {
-      const int next = t + UNIT, next_page = next < end ? table[next / p.page_size] : 0;
-      if (page >= 0 && page < p.num_pages) {
-        const long long in_page = static_cast<long long>(t % p.page_size) * p.d;
-        acc.tile(p, static_cast<const T*>(p.k) + page * p.k_page + h * p.k_head + in_page,
-                 static_cast<const T*>(p.v) + page * p.v_page + h * p.v_head + in_page, t, limit, mask);
-      } else if (lane == 0) {
-        atomicCAS(p.status, kStatusOk, kStatusPageRange);
-      }
-      t = next, page = next_page;
-    }
-    acc.join(buf, ml);
+    acc.walk(p, reinterpret_cast<char*>(smem4), query, h, row0, limit, max(0, a - kSegmentUnits) * UNIT, min(limit, (e - kSegmentUnits) * UNIT));
 
     const bool whole = a == 0 && e == n_units;
     const long long slot = static_cast<long long>(blockIdx.x) * 2 + (a == 0 ? 1 : 0);
@@ -449,15 +539,8 @@ __global__ void __launch_bounds__(128, PagedAttn<T, DP, WIDE, MASK>::BLOCKS) pag
     for (int x = threadIdx.x; x < A::RT * (DP / 4); x += blockDim.x) {
       const int row = x / (DP / 4), dim = x % (DP / 4) * 4;
       if (row0 + row >= p.group || dim >= p.d) continue;
-      float l = 0.f, m = -INFINITY;
-      float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < A::WARPS; ++w) {
-        l += ml[(A::WARPS + w) * A::RT + row];
-        m = fmaxf(m, ml[w * A::RT + row]);
-        const float4 y = *reinterpret_cast<const float4*>(buf + (w * A::RT + row) * A::ROW + dim);
-        s.x += y.x, s.y += y.y, s.z += y.z, s.w += y.w;
-      }
+      float l, m;
+      const float4 s = block_sum<A>(reinterpret_cast<const char*>(smem4), row, dim, l, m);
       if (whole) {
         pa_store(out + (row0 + row) * p.d + dim, s, l);
       } else {
@@ -467,72 +550,153 @@ __global__ void __launch_bounds__(128, PagedAttn<T, DP, WIDE, MASK>::BLOCKS) pag
     }
     if (threadIdx.x == 0 && a > 0 && e == n_units) {
       const long long start = base + static_cast<long long>(seg) * n_units;
-      p.shared_seg[blockIdx.x] = make_int4(static_cast<int>(((start + 1) * blocks - 1) / units), query, h, row0);
+      p.shared_seg[blockIdx.x] = make_int4(static_cast<int>(((start + kSegmentUnits + 1) * blocks - 1) / units), query, h, row0);
     }
-    u += e - a;
-    __syncthreads();  // buf is free for the next segment
+    u += e - a0;
+    __syncthreads();  // the rings are free for the next segment
   }
 }
 
-// Joins a segment that several blocks of the first kernel share.  Block (row, last block of the segment); warp w adds every
-// eighth part, then the warps' sums are added.
+OSLO_DEVINL void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+OSLO_DEVINL uint32_t peer_smem(uint32_t addr, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+OSLO_DEVINL float4 peer_load4(uint32_t addr) {
+  float4 r;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(r.x), "=f"(r.y), "=f"(r.z), "=f"(r.w) : "r"(addr) : "memory");
+  return r;
+}
+OSLO_DEVINL float2 peer_load2(uint32_t addr) {
+  float2 r;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(r.x), "=f"(r.y) : "r"(addr) : "memory");
+  return r;
+}
+
+// The same attention in one launch, for sequences that cannot be long: a cluster of up to eight blocks takes one segment, each an
+// equal part of its tokens, and joins the parts through distributed shared memory.
 template <typename T, int DP, bool WIDE, bool MASK>
-__global__ void __launch_bounds__(256) paged_attention_join_kernel(const PagedAttnParams p) {
+__global__ void __launch_bounds__(128, PagedAttn<T, DP, WIDE, MASK>::BLOCKS) paged_attention_cluster_kernel(const PagedAttnParams p, int cluster) {
+  using A = PagedAttn<T, DP, WIDE, MASK>;
+  constexpr int UNIT = A::WARPS * A::TT;
+  extern __shared__ float4 smem4[];
+  __shared__ float2 total[A::RT];
+  char* smem = reinterpret_cast<char*>(smem4);
+  const int rank = blockIdx.x % cluster, seg = blockIdx.x / cluster;
+  const int heads = p.hkv * p.row_tiles, query = seg / heads, rest = seg - query * heads;
+  const int h = rest / p.row_tiles, row0 = (rest - h * p.row_tiles) * A::RT;
+  const int limit = query_limit<MASK>(p, query, threadIdx.x == 0);
+  const int units = (limit + UNIT - 1) / UNIT;
+  A acc;
+  acc.walk(p, smem, query, h, row0, limit, units * rank / cluster * UNIT, min(limit, units * (rank + 1) / cluster * UNIT));
+  T* out = static_cast<T*>(p.out) + ((static_cast<long long>(query) * p.hkv + h) * p.group + row0) * p.d;
+  const int rows = min(A::RT, p.group - row0), quads = p.d / 4;
+  if (cluster == 1) {
+    for (int x = threadIdx.x; x < rows * quads; x += 128) {
+      const int row = x / quads, dim = (x - row * quads) * 4;
+      float l, m;
+      const float4 s = block_sum<A>(smem, row, dim, l, m);
+      pa_store(out + row * p.d + dim, s, l);
+    }
+    return;
+  }
+  // the block's sum replaces its first warp's output
+  for (int x = threadIdx.x; x < rows * quads; x += 128) {
+    const int row = x / quads, dim = (x - row * quads) * 4;
+    float l, m;
+    const float4 s = block_sum<A>(smem, row, dim, l, m);
+    *reinterpret_cast<float4*>(smem + sizeof(float) * (row * A::ROW + dim)) = s;
+    if (dim == 0) total[row] = make_float2(m, l);
+  }
+  cluster_barrier();
+  for (int x = rank * 128 + threadIdx.x; x < rows * quads; x += cluster * 128) {
+    const int row = x / quads, dim = (x - row * quads) * 4;
+    const uint32_t at = smem_u32(smem) + sizeof(float) * (row * A::ROW + dim), at_total = smem_u32(total + row);
+    float2 t[8];
+    float4 y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < cluster) t[i] = peer_load2(peer_smem(at_total, i)), y[i] = peer_load4(peer_smem(at, i));
+    float m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < cluster) m = fmaxf(m, t[i].x);
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < cluster) {
+        const float w = A::weight(t[i].x, m);
+        l += t[i].y * w;
+        s.x += y[i].x * w, s.y += y[i].y * w, s.z += y[i].z * w, s.w += y[i].w * w;
+      }
+    pa_store(out + row * p.d + dim, s, l);
+  }
+  cluster_barrier();  // a block's shared memory stays until all have read it
+}
+
+// Joins a segment that several blocks of the first kernel share.  Block (four rows, last block of the segment); of a row's four
+// warps each adds every fourth part with a running maximum, then the warps' sums are added.
+constexpr int kJoinRows = 4, kJoinWarps = 4;
+
+template <typename T, int DP, bool WIDE, bool MASK>
+__global__ void __launch_bounds__(32 * kJoinRows * kJoinWarps) paged_attention_join_kernel(const PagedAttnParams p) {
   using A = PagedAttn<T, DP, WIDE, MASK>;
   constexpr int V = DP / 128 > 0 ? DP / 128 : 1;  // float4s of a lane
   constexpr int LANES = DP / 4 < 32 ? DP / 4 : 32;
-  __shared__ float4 sums[8][DP / 4];
-  __shared__ float red[8];
+  __shared__ float4 sums[kJoinRows][kJoinWarps][DP / 4];
+  __shared__ float tops[kJoinRows][kJoinWarps], totals[kJoinRows][kJoinWarps];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int4 seg = p.shared_seg[blockIdx.y];
-  const int row = blockIdx.x;
-  if (seg.x < 0 || seg.w + row >= p.group) return;
-  const int parts = blockIdx.y - seg.x + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const auto slot = [&](int i) { return (static_cast<long long>(seg.x + i) * 2 + (i == 0 ? 1 : 0)) * A::RT + row; };
-  float m = -INFINITY;
-  for (int i = threadIdx.x; i < parts; i += 256) m = fmaxf(m, p.part_ml[slot(i)].x);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if (lane == 0) red[warp] = m;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < 8; ++w) m = fmaxf(m, red[w]);
-  __syncthreads();
-  float l = 0.f;
+  if (seg.x < 0) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, line = warp / kJoinWarps, piece = warp % kJoinWarps;
+  const int row = blockIdx.x * kJoinRows + line;
+  const bool used = row < A::RT && seg.w + row < p.group;
+  const int parts = used ? blockIdx.y - seg.x + 1 : 0;
+  float m = -INFINITY, l = 0.f;
   float4 o[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) o[j] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-  for (int i = warp; i < parts; i += 8) {
-    const float2 x = p.part_ml[slot(i)];
-    const float w = A::weight(x.x, m);
-    l += x.y * w;
+  for (int i = piece; i < parts; i += kJoinWarps) {
+    const long long slot = (static_cast<long long>(seg.x + i) * 2 + (i == 0 ? 1 : 0)) * A::RT + row;
+    const float2 x = p.part_ml[slot];
+    const float top = fmaxf(m, x.x), f = A::weight(m, top), w = A::weight(x.x, top);
+    m = top;
+    l = l * f + x.y * w;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const int dim = (j * 32 + lane) * 4;
       if (lane < LANES && dim < p.d) {
-        const float4 y = *reinterpret_cast<const float4*>(p.part_o + slot(i) * DP + dim);
-        o[j].x += y.x * w, o[j].y += y.y * w, o[j].z += y.z * w, o[j].w += y.w * w;
+        const float4 y = *reinterpret_cast<const float4*>(p.part_o + slot * DP + dim);
+        o[j].x = o[j].x * f + y.x * w, o[j].y = o[j].y * f + y.y * w, o[j].z = o[j].z * f + y.z * w, o[j].w = o[j].w * f + y.w * w;
       }
     }
   }
-  if (lane == 0) red[warp] = l;
 #pragma unroll
   for (int j = 0; j < V; ++j)
-    if (lane < LANES) sums[warp][j * 32 + lane] = o[j];
+    if (lane < LANES) sums[line][piece][j * 32 + lane] = o[j];
+  if (lane == 0) tops[line][piece] = m, totals[line][piece] = l;
   __syncthreads();
-  const int dim = threadIdx.x * 4;
-  if (dim >= p.d) return;
-  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-  l = 0.f;
+  if (!used || piece != 0) return;
+  float w[kJoinWarps];
+  m = -INFINITY, l = 0.f;
 #pragma unroll
-  for (int w = 0; w < 8; ++w) {
-    const float4 y = sums[w][threadIdx.x];
-    s.x += y.x, s.y += y.y, s.z += y.z, s.w += y.w;
-    l += red[w];
-  }
+  for (int i = 0; i < kJoinWarps; ++i) m = fmaxf(m, tops[line][i]);
+#pragma unroll
+  for (int i = 0; i < kJoinWarps; ++i) w[i] = A::weight(tops[line][i], m), l += totals[line][i] * w[i];
   T* out = static_cast<T*>(p.out) + ((static_cast<long long>(seg.y) * p.hkv + seg.z) * p.group + seg.w + row) * p.d;
-  pa_store(out + dim, s, l);
+  for (int x = lane; x * 4 < p.d; x += 32) {
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < kJoinWarps; ++i) {
+      const float4 y = sums[line][i][x];
+      s.x += y.x * w[i], s.y += y.y * w[i], s.z += y.z * w[i], s.w += y.w * w[i];
+    }
+    pa_store(out + x * 4, s, l);
+  }
 }
 
 // What the caller's workspace has to hold for one block of the grid, in bytes.
@@ -541,29 +705,45 @@ constexpr long long part_bytes(int rt, int dp) { return 2ll * rt * (dp * 4 + 8) 
 template <typename T, int DP, bool WIDE, bool MASK>
 struct PagedAttnLaunch {
   using A = PagedAttn<T, DP, WIDE, MASK>;
-  // Blocks that one SM holds at once; negative: an error.
+  // Blocks that one SM holds at once; negative: an error.  Called once before the first launch on a device.
   static int resident() {
     auto kernel = paged_attention_kernel<T, DP, WIDE, MASK>;
-    if (A::kSmem > 48 * 1024 &&
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(A::kSmem)) != cudaSuccess)
+    const int smem = static_cast<int>(A::kSmem);
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+        cudaFuncSetAttribute(paged_attention_cluster_kernel<T, DP, WIDE, MASK>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
       return -2;
     int n = 0;
     if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, 128, A::kSmem) != cudaSuccess || n < 1) return -2;
     return n;
   }
-  static int launch(PagedAttnParams& p, int grid, void* ws, long long ws_bytes, cudaStream_t st) {
+  static int launch(PagedAttnParams& p, int grid, int cluster, void* ws, long long ws_bytes, cudaStream_t st) {
+    p.row_tiles = (p.group + A::RT - 1) / A::RT;
+    if (cluster > 0) {
+      const long long blocks = static_cast<long long>(p.b) * p.s * p.hkv * p.row_tiles * cluster;
+      if (blocks > 0x7fffffffll || cluster > 8) return -1;
+      cudaLaunchConfig_t cfg{};
+      cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+      cfg.blockDim = dim3(128);
+      cfg.dynamicSmemBytes = A::kSmem;
+      cfg.stream = st;
+      cudaLaunchAttribute attr{};
+      attr.id = cudaLaunchAttributeClusterDimension;
+      attr.val.clusterDim.x = cluster, attr.val.clusterDim.y = 1, attr.val.clusterDim.z = 1;
+      cfg.attrs = &attr;
+      cfg.numAttrs = cluster > 1 ? 1 : 0;
+      return cudaLaunchKernelEx(&cfg, paged_attention_cluster_kernel<T, DP, WIDE, MASK>, p, cluster) == cudaSuccess ? 0 : -2;
+    }
     if (grid <= 0 || ws_bytes < grid * part_bytes(A::RT, DP)) return -1;
     char* w = static_cast<char*>(ws);
     p.part_o = reinterpret_cast<float*>(w);
     p.part_ml = reinterpret_cast<float2*>(w + static_cast<long long>(grid) * 2 * A::RT * DP * 4);
     p.shared_seg = reinterpret_cast<int4*>(w + static_cast<long long>(grid) * 2 * A::RT * (DP * 4 + 8));
-    p.row_tiles = (p.group + A::RT - 1) / A::RT;
     paged_attention_kernel<T, DP, WIDE, MASK><<<grid, 128, A::kSmem, st>>>(p);
     if (cudaGetLastError() != cudaSuccess) return -2;
     if (grid == 1) return 0;  // nothing is shared
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(p.group < A::RT ? p.group : A::RT, grid);
-    cfg.blockDim = dim3(256);
+    cfg.gridDim = dim3(((p.group < A::RT ? p.group : A::RT) + kJoinRows - 1) / kJoinRows, grid);
+    cfg.blockDim = dim3(32 * kJoinRows * kJoinWarps);
     cfg.stream = st;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -603,7 +783,7 @@ extern "C" {
 struct OsloPagedAttentionArgs {
   long long q, k_pages, v_pages, table, lens, mask, out, workspace, status, stream;  // addresses; mask may be 0
   long long q_b, q_s, q_h, k_page, k_head, v_page, v_head, table_row, mask_b, mask_s;
-  long long b, s, hkv, group, d, page_size, max_pages, num_pages, mask_len, dtype, grid, workspace_bytes;
+  long long b, s, hkv, group, d, page_size, max_pages, num_pages, mask_len, dtype, grid, cluster, workspace_bytes;  // cluster > 0: one launch, without a workspace
   double scale;
 };
 
@@ -632,7 +812,7 @@ int oslo_paged_attention(const OsloPagedAttentionArgs* a) {
   p.b = a->b, p.s = a->s, p.hkv = a->hkv, p.group = a->group, p.d = a->d, p.page_size = a->page_size, p.max_pages = a->max_pages;
   p.num_pages = a->num_pages, p.mask_len = a->mask_len, p.scale = static_cast<float>(a->scale);
   return paged_attention_dispatch(a->dtype, a->d, a->group, a->mask != 0, [&](auto l) {
-    return decltype(l)::launch(p, static_cast<int>(a->grid), reinterpret_cast<void*>(a->workspace), a->workspace_bytes,
+    return decltype(l)::launch(p, static_cast<int>(a->grid), static_cast<int>(a->cluster), reinterpret_cast<void*>(a->workspace), a->workspace_bytes,
                                reinterpret_cast<cudaStream_t>(a->stream));
   });
 }

@@ -27,11 +27,14 @@ _DT = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # of a device's current stream
 _device = getattr(torch._C, "_cuda_getDevice", None)
 MAX_HEAD_DIM = 256
+#: tokens that a block of the one-launch attention takes at most
+CLUSTER_TOKENS = 1024
+_INFERENCE = "the paged cache is for inference: call it under torch.no_grad() or detach its inputs"
 
 
-def _check_pages(k_pages, v_pages, block_table, b: int, hd: int, dtype, device):
+def _check_pages(k_pages, v_pages, block_table, b: int, hd: int, dtype, device: int):
     """Raises unless pools and table fit ``b`` sequences of this type; returns what the kernels need of their layout."""
-    shape, ks, vs = k_pages.shape, k_pages.stride(), v_pages.stride()
+    shape, ks, vs, table = k_pages.shape, k_pages.stride(), v_pages.stride(), block_table.shape
     if len(shape) != 4 or v_pages.shape != shape:
         raise ValueError(f"k_pages and v_pages are [pages, kv_heads, page_size, head_dim], both alike: got {tuple(shape)} "
                          f"and {tuple(v_pages.shape)}")
@@ -44,39 +47,54 @@ def _check_pages(k_pages, v_pages, block_table, b: int, hd: int, dtype, device):
     if page == 0 or page % 16 or d == 0 or d % 8 or d > MAX_HEAD_DIM or hkv == 0:
         raise ValueError(f"page_size is a multiple of 16 and head_dim a multiple of 8 up to {MAX_HEAD_DIM}: got {page}, {d} "
                          f"({hkv} key heads)")
-    for t, st in ((k_pages, ks), (v_pages, vs)):
-        if st[3] != 1 or st[2] != d or (st[0] | st[1]) % 8 or t.data_ptr() % 16:
-            raise ValueError("the tokens of a head inside a page are contiguous, and pages and heads start on 16-byte boundaries")
-    table = block_table.shape
-    row, col = block_table.stride() if len(table) == 2 else (0, 0)
-    if block_table.dtype != torch.int32 or len(table) != 2 or table[0] != b or (col != 1 and table[1] > 1):
-        raise ValueError(f"block_table is int32 [{b}, pages per sequence] with contiguous rows: got {block_table.dtype} {tuple(table)}")
-    if k_pages.device != device or v_pages.device != device or block_table.device != device:
-        raise ValueError(f"tensors are on {device}, {k_pages.device}, {v_pages.device} and {block_table.device}")
-    if table[1] * page > 0x3FFFFFFF:
+    kp, vp = k_pages.data_ptr(), v_pages.data_ptr()
+    if ks[3] != 1 or vs[3] != 1 or ks[2] != d or vs[2] != d or (ks[0] | ks[1] | vs[0] | vs[1]) % 8 or (kp | vp) % 16:
+        raise ValueError("the tokens of a head inside a page are contiguous, and pages and heads start on 16-byte boundaries: got "
+                         f"strides {ks} and {vs}")
+    if len(table) != 2 or table[0] != b or block_table.dtype != torch.int32:
+        raise ValueError(f"block_table is int32 [{b}, pages per sequence]: got {block_table.dtype} {tuple(table)}")
+    row, col = block_table.stride()
+    width = table[1]
+    if col != 1 and width > 1:
+        raise ValueError(f"the rows of block_table are contiguous: got strides {(row, col)}")
+    if k_pages.get_device() != device or v_pages.get_device() != device or block_table.get_device() != device:
+        raise ValueError(f"tensors are on devices {device}, {k_pages.device}, {v_pages.device} and {block_table.device}")
+    if width * page > 0x3FFFFFFF:
         raise ValueError("block_table spans more than 2**30 tokens")
-    return pages, hkv, page, table[1], row, ks, vs
+    return pages, hkv, page, width, row, ks, vs, kp, vp
 
 
-def _check_ints(name, t, b: int, device):
-    if t.dtype != torch.int32 or t.shape != (b,) or not t.is_contiguous() or t.device != device:
-        raise ValueError(f"{name} is a contiguous int32 tensor [{b}] on {device}: got {t.dtype} {tuple(t.shape)} on {t.device}")
+def _check_ints(name, t, b: int, device: int):
+    if t.dtype != torch.int32 or t.shape != (b,) or not t.is_contiguous() or t.get_device() != device:
+        raise ValueError(f"{name} is a contiguous int32 tensor [{b}] beside the other ones: got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
-def _no_grad(*tensors):
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise RuntimeError("the paged cache is for inference: call it under torch.no_grad() or detach its inputs")
+def _check_rope(rope, hd: int, device: int):
+    cos, sin, rot, neox = rope
+    if rot < 0 or rot % 2 or rot > hd:
+        raise ValueError(f"rot_dim is even and at most {hd}: got {rot}")
+    shape = cos.shape
+    if cos.dtype != torch.float32 or sin.dtype != torch.float32 or len(shape) != 2 or shape[1] != rot // 2 or sin.shape != shape \
+            or not cos.is_contiguous() or not sin.is_contiguous() or cos.get_device() != device or sin.get_device() != device:
+        raise ValueError(f"the rotation's tables are contiguous float32 [positions, {rot // 2}] beside the other tensors: got "
+                         f"{cos.dtype} {tuple(shape)} and {sin.dtype} {tuple(sin.shape)} on {cos.device} and {sin.device}")
+    return cos, sin, rot, 1 if neox else 0, shape[0]
+
+
+def _grad(*tensors):
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            return True
+    return False
 
 
 def _aligned(t):
-    """``t`` with unit inner stride and 16-byte aligned heads (a copy where it has not), and its strides."""
-    st = t.stride()
-    if st[3] == 1 and not ((st[0] | st[1] | st[2]) % (16 // t.element_size()) or t.data_ptr() % 16):
-        return t, st
+    """``t`` with unit inner stride and 16-byte aligned heads (a copy where it has not), its strides and its address."""
+    st, at = t.stride(), t.data_ptr()
+    if st[3] == 1 and not ((st[0] | st[1] | st[2]) % (16 // t.element_size()) or at % 16):
+        return t, st, at
     t = t.clone(memory_format=torch.contiguous_format)
-    return t, t.stride()
+    return t, t.stride(), t.data_ptr()
 
 
 def paged_kv_append(k, v, k_pages, v_pages, block_table, start, count=None, q=None, rope=None):
@@ -91,13 +109,14 @@ def paged_kv_append(k, v, k_pages, v_pages, block_table, start, count=None, q=No
 
     Returns the rotated ``q`` ``[b, s, heads, head_dim]`` as a new tensor (rows of padding are zeros), or ``None`` without ``q``.
     """
-    shape, dtype, dev = k.shape, k.dtype, k.device
-    if len(shape) != 4 or v.shape != shape or v.dtype != dtype or v.device != dev:
+    shape, dtype, dev = k.shape, k.dtype, k.get_device()
+    if len(shape) != 4 or v.shape != shape or v.dtype != dtype or v.get_device() != dev:
         raise ValueError(f"k and v are [b, s, kv_heads, head_dim], both alike: got {tuple(shape)} {dtype} and {tuple(v.shape)} "
                          f"{v.dtype}")
     b, s, hkv, hd = shape
-    _no_grad(k, v, q, k_pages, v_pages)
-    pages, heads, page, width, row, kps, vps = _check_pages(k_pages, v_pages, block_table, b, hd, dtype, dev)
+    if torch.is_grad_enabled() and _grad(k, v, q, k_pages, v_pages):
+        raise RuntimeError(_INFERENCE)
+    pages, heads, page, width, row, kps, vps, kp, vp = _check_pages(k_pages, v_pages, block_table, b, hd, dtype, dev)
     if heads != hkv:
         raise ValueError(f"the pages hold {heads} key heads, the tokens {hkv}")
     _check_ints("start", start, b, dev)
@@ -106,39 +125,28 @@ def paged_kv_append(k, v, k_pages, v_pages, block_table, start, count=None, q=No
     hq = 0
     if q is not None:
         qshape = q.shape
-        if len(qshape) != 4 or qshape[0] != b or qshape[1] != s or qshape[3] != hd or q.dtype != dtype or q.device != dev:
-            raise ValueError(f"q is [{b}, {s}, heads, {hd}] {dtype} on {dev}: got {tuple(qshape)} {q.dtype} on {q.device}")
+        if len(qshape) != 4 or qshape[0] != b or qshape[1] != s or qshape[3] != hd or q.dtype != dtype or q.get_device() != dev:
+            raise ValueError(f"q is [{b}, {s}, heads, {hd}] {dtype} beside k: got {tuple(qshape)} {q.dtype} on {q.device}")
         hq = qshape[2]
-    cos = sin = None
-    rot, neox, positions = 0, True, 0
-    if rope is not None:
-        cos, sin, rot, neox = rope
-        if rot < 0 or rot % 2 or rot > hd:
-            raise ValueError(f"rot_dim is even and at most {hd}: got {rot}")
-        for t in (cos, sin):
-            if t.dtype != torch.float32 or t.dim() != 2 or t.shape != cos.shape or t.shape[1] != rot // 2 or not t.is_contiguous() \
-                    or t.device != dev:
-                raise ValueError(f"the rotation's tables are contiguous float32 [positions, {rot // 2}] on {dev}: got {t.dtype} "
-                                 f"{tuple(t.shape)} on {t.device}")
-        positions = cos.shape[0]
+    cos, sin, rot, neox, positions = _check_rope(rope, hd, dev) if rope is not None else (None, None, 0, 1, 0)
     if not k.is_cuda:
         return _append_reference(k, v, k_pages, v_pages, block_table, start, count, q, rope if rot else None)
-    index = dev.index
-    if index != _device():
+    if dev != _device():
         with torch.cuda.device(dev):
             return paged_kv_append(k, v, k_pages, v_pages, block_table, start, count, q, rope)
-    k, ks = _aligned(k)
-    v, vs = _aligned(v)
-    out, qs = None, ks
+    out, qs, qp, op = None, (0, 0, 0), 0, 0
     if q is not None:
-        out = torch.empty(qshape, dtype=dtype, device=dev)
-        q, qs = _aligned(q)
-    rc = _fn("oslo_paged_kv_append")(_APPEND_ARGS.pack(
-        q.data_ptr() if hq else 0, k.data_ptr(), v.data_ptr(), out.data_ptr() if hq else 0, k_pages.data_ptr(), v_pages.data_ptr(),
-        block_table.data_ptr(), start.data_ptr(), count.data_ptr() if count is not None else 0, cos.data_ptr() if rot else 0,
-        sin.data_ptr() if rot else 0, _status_ptr(index), _raw_stream(index),
+        out = q.new_empty(qshape)
+        if hq:
+            q, qs, qp = _aligned(q)
+            op = out.data_ptr()
+    k, ks, kx = _aligned(k)
+    v, vs, vx = _aligned(v)
+    rc = (_append_fn or _load()[0])(_APPEND_ARGS.pack(
+        qp, kx, vx, op, kp, vp, block_table.data_ptr(), start.data_ptr(), 0 if count is None else count.data_ptr(),
+        cos.data_ptr() if rot else 0, sin.data_ptr() if rot else 0, _status_ptr(dev), _raw_stream(dev),
         qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], kps[0], kps[1], vps[0], vps[1], row,
-        b, s, hq, hkv, hd, rot, 1 if neox else 0, positions, page, width, pages, _DT[dtype]))
+        b, s, hq, hkv, hd, rot, neox, positions, page, width, pages, _DT[dtype]))
     if rc:
         raise RuntimeError(f"oslo_paged_kv_append failed ({rc})")
     return out
@@ -155,32 +163,33 @@ def paged_attention(q, k_pages, v_pages, block_table, lengths, scale: Optional[f
 
     Returns ``[b, s, heads * head_dim]``, like :func:`oslo_b200.ops.attention.attention`.
     """
-    shape, dtype, dev = q.shape, q.dtype, q.device
+    shape, dtype, dev = q.shape, q.dtype, q.get_device()
     if len(shape) != 4:
         raise ValueError(f"q is [b, s, heads, head_dim]: got {tuple(shape)}")
     b, s, hq, hd = shape
-    _no_grad(q, k_pages, v_pages, mask)
-    pages, hkv, page, width, row, ks, vs = _check_pages(k_pages, v_pages, block_table, b, hd, dtype, dev)
+    if torch.is_grad_enabled() and _grad(q, k_pages, v_pages, mask):
+        raise RuntimeError(_INFERENCE)
+    pages, hkv, page, width, row, ks, vs, kp, vp = _check_pages(k_pages, v_pages, block_table, b, hd, dtype, dev)
     _check_ints("lengths", lengths, b, dev)
-    if hq == 0 or hq % hkv:
+    group = hq // hkv
+    if hq == 0 or group * hkv != hq:
         raise ValueError(f"{hq} query heads do not share {hkv} key heads evenly")
-    scale = float(scale) if scale is not None else 1.0 / math.sqrt(hd)
+    scale = hd ** -0.5 if scale is None else float(scale)
     if not math.isfinite(scale):
         raise ValueError(f"scale is a finite number: got {scale}")
     if mask is not None:
-        if mask.dim() != 4 or mask.shape[0] not in (1, b) or mask.shape[1] != 1 or mask.shape[2] not in (1, s) or mask.device != dev \
-                or not mask.is_floating_point():
-            raise ValueError(f"mask is an additive floating tensor [{b} or 1, 1, {s} or 1, tokens] on {dev}: got {mask.dtype} "
+        if mask.dim() != 4 or mask.shape[0] not in (1, b) or mask.shape[1] != 1 or mask.shape[2] not in (1, s) \
+                or mask.get_device() != dev or not mask.is_floating_point():
+            raise ValueError(f"mask is an additive floating tensor [{b} or 1, 1, {s} or 1, tokens] beside q: got {mask.dtype} "
                              f"{tuple(mask.shape)} on {mask.device}")
         mask = mask.float()
     if not q.is_cuda:
         return _attention_reference(q, k_pages, v_pages, block_table, lengths, scale, mask)
-    index = dev.index
-    if index != _device():
+    if dev != _device():
         with torch.cuda.device(dev):
             return paged_attention(q, k_pages, v_pages, block_table, lengths, scale, mask)
-    q, qs = _aligned(q)
-    out = torch.empty((b, s, hq * hd), dtype=dtype, device=dev)
+    q, qs, qp = _aligned(q)
+    out = q.new_empty((b, s, hq * hd))
     most = width * page
     mptr = mb = mt = mlen = 0
     if mask is not None:
@@ -190,16 +199,26 @@ def paged_attention(q, k_pages, v_pages, block_table, lengths, scale: Optional[f
             mask = mask.contiguous()
         mptr, mb, mt = mask.data_ptr(), mask.stride(0), mask.stride(2)
         most = min(most, mlen)
-    group, kind = hq // hkv, _DT[dtype]
-    blocks, block_bytes = _attention_plan(kind, hd, group, mptr != 0, index)
-    # no more blocks than the longest possible sequences have work for (in units of 32 tokens, the smallest of the kernel's)
-    grid = max(1, min(blocks, b * s * hq * -(-most // 32)))
-    room = grid * block_bytes
-    ws = torch.empty(room, dtype=torch.uint8, device=dev)
-    rc = _fn("oslo_paged_attention")(_ATTEND_ARGS.pack(
-        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), lengths.data_ptr(), mptr, out.data_ptr(),
-        ws.data_ptr(), _status_ptr(index), _raw_stream(index), qs[0], qs[1], qs[2], ks[0], ks[1], vs[0], vs[1], row, mb, mt,
-        b, s, hkv, group, hd, page, width, pages, mlen, kind, grid, room, scale))
+    kind = _DT[dtype]
+    blocks, block_bytes = _attention_plan(kind, hd, group, mptr != 0, dev)
+    # Where the table keeps sequences short, a cluster of blocks takes each (query token, key head) and one launch does it.  Else
+    # equal ranges of the work go to as many blocks as the device holds (no more than the longest possible sequences have work
+    # for, in units of 32 tokens, the smallest of the kernel's) and a second launch joins what they share.
+    segments = b * s * hkv * -(-group // (16 if group > 8 else 8))
+    cluster = 8
+    while cluster > 1 and (segments * cluster > blocks or cluster * 32 > most):
+        cluster //= 2
+    grid = room = wp = 0
+    if most > CLUSTER_TOKENS * cluster:
+        cluster = 0
+        grid = max(1, min(blocks, segments * -(-most // 32)))
+        room = grid * block_bytes
+        ws = torch.empty(room, dtype=torch.uint8, device=q.device)
+        wp = ws.data_ptr()
+    rc = (_attend_fn or _load()[1])(_ATTEND_ARGS.pack(
+        qp, kp, vp, block_table.data_ptr(), lengths.data_ptr(), mptr, out.data_ptr(), wp, _status_ptr(dev), _raw_stream(dev),
+        qs[0], qs[1], qs[2], ks[0], ks[1], vs[0], vs[1], row, mb, mt,
+        b, s, hkv, group, hd, page, width, pages, mlen, kind, grid, cluster, room, scale))
     if rc:
         raise RuntimeError(f"oslo_paged_attention failed ({rc})")
     return out
@@ -207,16 +226,16 @@ def paged_attention(q, k_pages, v_pages, block_table, lengths, scale: Optional[f
 
 # arguments travel as one struct of eight-byte fields: ctypes converts one value instead of forty
 _APPEND_ARGS = struct.Struct("=39q")
-_ATTEND_ARGS = struct.Struct("=32qd")
-_fns = {}
+_ATTEND_ARGS = struct.Struct("=33qd")
+_append_fn = _attend_fn = None
 
 
-def _fn(name):
-    fn = _fns.get(name)
-    if fn is None:
-        getattr(_lib._load_cuda_lib(), name).argtypes = [ctypes.c_char_p]
-        fn = _fns[name] = getattr(_lib.cuda_lib(), name)
-    return fn
+def _load():
+    global _append_fn, _attend_fn
+    dll, lib = _lib._load_cuda_lib(), _lib.cuda_lib()
+    dll.oslo_paged_kv_append.argtypes = dll.oslo_paged_attention.argtypes = [ctypes.c_char_p]
+    _append_fn, _attend_fn = lib.oslo_paged_kv_append, lib.oslo_paged_attention
+    return _append_fn, _attend_fn
 
 
 @lru_cache(maxsize=None)
