@@ -1,6 +1,8 @@
 """Text generation for the in-tree causal language models: greedy, top-k / top-p sampling and beam search, with
 n-gram blocking on the fused kernel and a key / value cache: the prompt is run once, after which every step feeds only
-the newest token and attends over the cached keys and values (``oslo_b200.ops.attention.DecodeCache``).
+the newest token and attends over the cached keys and values (``oslo_b200.ops.attention.DecodeCache``, or in pages that
+never move and for prompts of different lengths: ``oslo_b200.ops.paged.PagedDecodeCache``).  Penalties for repeated tokens,
+biases and grammar masks on the logits are one kernel (``oslo_b200.ops.logits.process_logits``).
 
 A compact counterpart of LightSeq's inference engine entry points (oslo/lightseq2/inference/pywrapper/*, sampling and
 beam-search kernels in inference/kernels/transformerKernels.cc.cu): the model forward runs on this repository's
@@ -8,13 +10,15 @@ training kernels; the decoding bookkeeping is vectorised torch code on the devic
 """
 from __future__ import annotations
 
-from typing import Optional
+from typing import Callable, Mapping, Optional, Sequence, Union
 
 import torch
 import torch.nn.functional as F
 
 from oslo_b200.nn.ngram_repeat_block import NGramRepeatBlock
 from oslo_b200.ops.attention import DecodeCache, decode_cache
+from oslo_b200.ops.logits import pack_token_mask, process_logits
+from oslo_b200.ops.paged import PagedDecodeCache
 
 
 def _logits(model, ids, cache: Optional[DecodeCache] = None):
@@ -74,13 +78,68 @@ def _filter(logits, top_k: int, top_p: float):
     return logits
 
 
+class _LogitsRules:
+    """The penalties, biases and grammar of one generation, applied to the next-token logits of a step."""
+
+    def __init__(self, repetition_penalty, presence_penalty, frequency_penalty, logit_bias, allowed_tokens):
+        self.penalties = dict(repetition_penalty=repetition_penalty, presence_penalty=presence_penalty,
+                              frequency_penalty=frequency_penalty)
+        self.counts = repetition_penalty != 1.0 or presence_penalty != 0.0 or frequency_penalty != 0.0
+        self.bias, self.allowed_tokens = logit_bias, allowed_tokens
+        self.active = self.counts or logit_bias is not None or allowed_tokens is not None
+
+    def __call__(self, logits, ids, lengths, prompts):
+        """``ids [rows, >= lengths]``, of which ``lengths`` (int32 ``[rows]``; ``None``: all) count and ``prompts`` are the prompt."""
+        if not self.active:
+            return logits
+        rows, vocab = logits.shape
+        if self.bias is not None and not isinstance(self.bias, torch.Tensor):
+            pairs = list(self.bias.items() if isinstance(self.bias, Mapping) else self.bias)
+            bias = torch.zeros(vocab)
+            for token, value in pairs:
+                if not 0 <= int(token) < vocab:
+                    raise ValueError(f"logit_bias names token {token}, the vocabulary has {vocab}")
+                bias[int(token)] = float(value)
+            self.bias = bias
+        if self.bias is not None:
+            self.bias = self.bias.to(logits.device)
+        allowed = None
+        if self.allowed_tokens is not None:
+            allowed = self.allowed_tokens(ids, lengths)
+            if allowed is not None and allowed.dtype == torch.bool:
+                allowed = pack_token_mask(allowed)
+        history = dict(tokens=ids, token_lengths=lengths, prompt_lengths=prompts, **self.penalties) if self.counts else {}
+        return process_logits(logits, bias=self.bias, allowed=allowed, **history)
+
+
 @torch.no_grad()
 def generate(model, input_ids: torch.Tensor, max_new_tokens: int = 32, do_sample: bool = False, top_k: int = 0,
              top_p: float = 1.0, temperature: float = 1.0, num_beams: int = 1, no_repeat_ngram_size: int = 0,
              eos_token_id: Optional[int] = None, length_penalty: float = 1.0, pad_multiple: int = 1,
-             use_cache: bool = True):
+             use_cache: bool = True, paged_cache: bool = False, page_size: int = 64,
+             prompt_lengths: Optional[Sequence[int]] = None, repetition_penalty: float = 1.0, presence_penalty: float = 0.0,
+             frequency_penalty: float = 0.0, logit_bias: Union[None, torch.Tensor, Mapping, Sequence] = None,
+             allowed_tokens: Optional[Callable] = None):
     """Returns ``[batch, prompt + new]`` token ids (best beam when ``num_beams > 1``).  ``use_cache=False`` re-runs the
-    whole prefix every step (the reference behaviour for models whose attention does not go through ``oslo_b200.ops``)."""
+    whole prefix every step (the reference behaviour for models whose attention does not go through ``oslo_b200.ops``).
+
+    ``paged_cache``: keep keys and values in pages of ``page_size`` tokens and attend with the paged kernel (no beams).  With it,
+    ``prompt_lengths`` gives the number of tokens of each right-padded prompt; row ``i`` of the result is then its prompt,
+    what was generated, and padding (``eos_token_id`` or 0).
+    ``repetition_penalty`` (of prompt and generated tokens), ``presence_penalty``, ``frequency_penalty`` (of generated tokens),
+    ``logit_bias`` (a tensor ``[vocab]``, a mapping or pairs token -> value) and ``allowed_tokens`` change the logits before
+    temperature and sampling (of beams: their log-probabilities), see :func:`oslo_b200.ops.logits.process_logits`.
+    ``allowed_tokens(ids, lengths)`` is called every step with the tokens so far (``lengths``: int32 ``[rows]`` of those that
+    count, ``None``: all) and returns ``[rows, vocab]`` booleans, packed words, or ``None`` for no restriction."""
+    if paged_cache and not use_cache:
+        raise ValueError("paged_cache is a kind of cache: it needs use_cache")
+    if paged_cache and num_beams > 1:
+        raise ValueError("the paged cache does not follow beams: use the dense cache for num_beams > 1")
+    if prompt_lengths is not None and not paged_cache:
+        raise ValueError("prompts of different lengths need paged_cache=True")
+    if repetition_penalty <= 0:
+        raise ValueError(f"repetition_penalty is positive: got {repetition_penalty}")
+    rules = _LogitsRules(repetition_penalty, presence_penalty, frequency_penalty, logit_bias, allowed_tokens)
     model.eval()
     pc = getattr(model, "parallel_context", None)
     if num_beams > 1 and use_cache and pc is not None and getattr(pc, "tensor_parallel_size", 1) > 1:
@@ -92,21 +151,25 @@ def generate(model, input_ids: torch.Tensor, max_new_tokens: int = 32, do_sample
             use_cache = False
     if num_beams > 1:
         return _beam_search(model, input_ids, max_new_tokens, num_beams, no_repeat_ngram_size, eos_token_id, length_penalty,
-                            use_cache)
+                            use_cache, rules)
+    pick = _picker(do_sample, top_k, top_p)
+    if prompt_lengths is not None:
+        if no_repeat_ngram_size > 0:
+            raise ValueError("n-gram blocking takes prompts of one length")
+        return _generate_ragged(model, input_ids, [int(n) for n in prompt_lengths], max_new_tokens, pick, temperature, eos_token_id,
+                                page_size, rules)
     ids = input_ids
     blocker = NGramRepeatBlock()
     done = torch.zeros(ids.shape[0], dtype=torch.bool, device=ids.device)
-    cache = DecodeCache() if use_cache else None
+    cache = None
+    if use_cache:
+        cache = PagedDecodeCache(ids.shape[1] + max_new_tokens, page_size) if paged_cache else DecodeCache()
+    prompts = torch.full((ids.shape[0],), ids.shape[1], dtype=torch.int32, device=ids.device) if rules.counts else None
     for _ in range(max_new_tokens):
-        logits = _logits(model, ids, cache) / max(temperature, 1e-6)
+        logits = rules(_logits(model, ids, cache), ids, None, prompts) / max(temperature, 1e-6)
         if no_repeat_ngram_size > 0:
             logits = blocker(ids, logits.contiguous(), ids.shape[0], ids.shape[1] - 1, 1, no_repeat_ngram_size)
-        if do_sample:
-            from .kernels import sample_tokens
-
-            nxt = sample_tokens(logits, top_k, top_p)  # the device kernel on CUDA (no vocabulary sort)
-        else:
-            nxt = logits.argmax(-1, keepdim=True)
+        nxt = pick(logits)
         if eos_token_id is not None:
             nxt = torch.where(done.unsqueeze(1), torch.full_like(nxt, eos_token_id), nxt)
             done |= nxt.squeeze(1) == eos_token_id
@@ -116,7 +179,54 @@ def generate(model, input_ids: torch.Tensor, max_new_tokens: int = 32, do_sample
     return ids
 
 
-def _beam_search(model, input_ids, max_new_tokens, beams, ngram, eos, length_penalty, use_cache=True):
+def _picker(do_sample, top_k, top_p):
+    """Next tokens ``[rows, 1]`` from logits ``[rows, vocab]``."""
+    if not do_sample:
+        return lambda logits: logits.argmax(-1, keepdim=True)
+    from .kernels import sample_tokens
+
+    return lambda logits: sample_tokens(logits, top_k, top_p)  # the device kernel on CUDA (no vocabulary sort)
+
+
+def _generate_ragged(model, input_ids, lengths, max_new_tokens, pick, temperature, eos, page_size, rules):
+    """Generation from right-padded prompts of different lengths over the paged cache."""
+    if not getattr(getattr(model, "module", model), "ragged_prompts", False):
+        raise ValueError(f"{type(model).__name__} takes prompts of one length")
+    b, width = input_ids.shape
+    if len(lengths) != b or min(lengths) < 1 or max(lengths) > width:
+        raise ValueError(f"prompt_lengths has a number from 1 to {width} for each of the {b} prompts: got {lengths}")
+    dev = input_ids.device
+    pad = 0 if eos is None else eos
+    length = torch.tensor(lengths, dtype=torch.int32, device=dev)
+    out = input_ids.new_full((b, width + max_new_tokens), pad)
+    out[:, :width] = torch.where(torch.arange(width, device=dev) < length[:, None], input_ids, out[:, :width])
+    cache = PagedDecodeCache(max(lengths) + max_new_tokens, page_size)
+    prompts = length if rules.counts else None
+    done = torch.zeros(b, dtype=torch.bool, device=dev)
+    rows = torch.arange(b, device=dev)
+    feed, counts, last = out[:, : max(lengths)], lengths, (length - 1).long()
+    new = 0
+    for new in range(1, max_new_tokens + 1):
+        cache.begin_forward(counts)
+        with decode_cache(cache):
+            logits = model(input_ids=feed)
+        cache.advance(feed.shape[1])
+        logits = logits.logits if hasattr(logits, "logits") else logits[0]
+        logits = _whole_logits(model, logits[rows, last]).float()
+        logits = rules(logits, out, length, prompts) / max(temperature, 1e-6)
+        nxt = pick(logits).squeeze(1)
+        if eos is not None:
+            nxt = torch.where(done, torch.full_like(nxt, eos), nxt)
+            done |= nxt == eos
+        out[rows, length.long()] = nxt
+        length = length + 1
+        feed, counts, last = nxt[:, None], None, torch.zeros_like(last)
+        if eos is not None and bool(done.all()):
+            break
+    return out[:, : width + new]
+
+
+def _beam_search(model, input_ids, max_new_tokens, beams, ngram, eos, length_penalty, use_cache=True, rules=None):
     b, prompt = input_ids.shape
     dev = input_ids.device
     ids = input_ids.repeat_interleave(beams, dim=0)  # [b * beams, t]
@@ -125,8 +235,11 @@ def _beam_search(model, input_ids, max_new_tokens, beams, ngram, eos, length_pen
     finished = torch.zeros(b * beams, dtype=torch.bool, device=dev)
     blocker = NGramRepeatBlock()
     cache = DecodeCache() if use_cache else None
+    prompts = torch.full((b * beams,), prompt, dtype=torch.int32, device=dev) if rules is not None and rules.counts else None
     for _ in range(max_new_tokens):
         lp = F.log_softmax(_logits(model, ids, cache), dim=-1)
+        if rules is not None:
+            lp = rules(lp, ids, None, prompts)
         if ngram > 0:
             lp = blocker(ids, lp.contiguous(), b, ids.shape[1] - 1, beams, ngram)
         vocab = lp.shape[-1]

@@ -14,8 +14,8 @@ FastAPI application:
   back end needs a URL change only.
 
 Requests wait in a queue; a single worker takes up to ``max_batch`` requests that arrive within ``max_wait_ms`` of the
-first one and runs those with the same prompt length and sampling settings as one batch (prompts of other lengths in the
-window run in their own batches: generation here takes no padding mask).  The model runs in a worker thread so the event
+first one and runs those with the same prompt length and sampling settings as one batch.  Requests with ``"paged_cache": true``
+share a batch whatever their prompts' lengths, where the model takes such prompts (GPT-2, GPT-NeoX, Llama).  The model runs in a worker thread so the event
 loop keeps accepting requests while the GPU is busy.
 """
 from __future__ import annotations
@@ -39,8 +39,9 @@ class _Request:
 class DynamicBatcher:
     """Groups queued requests into batches and runs them through ``generate_fn(ids [b, s], **params) -> [b, s + new]``."""
 
-    def __init__(self, generate_fn, max_batch: int = 8, max_wait_ms: float = 5.0):
+    def __init__(self, generate_fn, max_batch: int = 8, max_wait_ms: float = 5.0, ragged: bool = False):
         self.generate_fn, self.max_batch, self.max_wait = generate_fn, max_batch, max_wait_ms / 1000.0
+        self.ragged = ragged  # generate_fn takes prompt_lengths with paged_cache
         self.queue: "asyncio.Queue[_Request]" = None
         self.batches = self.requests = 0
         self.batch_sizes: List[int] = []
@@ -83,15 +84,20 @@ class DynamicBatcher:
                     break
             groups: Dict[Any, List[_Request]] = {}
             for r in window:
-                groups.setdefault((len(r.input_ids), tuple(sorted(r.params.items()))), []).append(r)
+                mixed = self.ragged and r.params.get("paged_cache") and not r.params.get("no_repeat_ngram_size")
+                groups.setdefault((None if mixed else len(r.input_ids), tuple(sorted(r.params.items()))), []).append(r)
             for (_, _), reqs in groups.items():
                 await self._run(reqs)
 
     async def _run(self, reqs: List[_Request]):
-        ids = torch.tensor([r.input_ids for r in reqs], dtype=torch.long)
+        lengths = [len(r.input_ids) for r in reqs]
+        width, params = max(lengths), dict(reqs[0].params)
+        ids = torch.tensor([r.input_ids + [0] * (width - n) for r, n in zip(reqs, lengths)], dtype=torch.long)
+        if min(lengths) < width:
+            params["prompt_lengths"] = lengths
         try:
-            out = await asyncio.get_running_loop().run_in_executor(None, lambda: self.generate_fn(ids, **reqs[0].params))
-            rows = out.tolist()
+            out = await asyncio.get_running_loop().run_in_executor(None, lambda: self.generate_fn(ids, **params))
+            rows = [row[: len(row) - width + n] for row, n in zip(out.tolist(), lengths)]
             now = time.perf_counter()
             self.batches += 1
             self.requests += len(reqs)
@@ -116,18 +122,25 @@ def create_app(model, tokenizer=None, device=None, max_batch: int = 8, max_wait_
 
     device = device or next(model.parameters()).device
     allowed = {"max_new_tokens", "do_sample", "top_k", "top_p", "temperature", "num_beams", "no_repeat_ngram_size",
-               "eos_token_id", "length_penalty"}
+               "eos_token_id", "length_penalty", "paged_cache", "page_size", "repetition_penalty", "presence_penalty",
+               "frequency_penalty", "logit_bias"}
+
+    def settings(given: Dict[str, Any]) -> Dict[str, Any]:
+        params = {k: v for k, v in given.items() if k in allowed}
+        if isinstance(params.get("logit_bias"), dict):  # hashable, so that requests with the same biases share a batch
+            params["logit_bias"] = tuple(sorted((int(k), float(v)) for k, v in params["logit_bias"].items()))
+        return params
 
     def run(ids, **params):
         return generate(model, ids.to(device), **params).cpu()
 
-    batcher = DynamicBatcher(run, max_batch, max_wait_ms)
+    batcher = DynamicBatcher(run, max_batch, max_wait_ms, ragged=getattr(getattr(model, "module", model), "ragged_prompts", False))
     app = FastAPI(title="oslo_b200 inference")
     app.state.batcher = batcher
 
     @app.post("/generate")
     async def _generate(body: Dict[str, Any]):
-        params = {k: v for k, v in body.items() if k in allowed}
+        params = settings(body)
         if "input_ids" in body:
             prompts = body["input_ids"]
             if prompts and isinstance(prompts[0], int):
@@ -192,7 +205,7 @@ def create_app(model, tokenizer=None, device=None, max_batch: int = 8, max_wait_
         b, sl = int(shape[0]), int(shape[1])
         if b <= 0 or sl <= 0 or len(flat) != b * sl:
             raise HTTPException(status_code=400, detail=f"data holds {len(flat)} elements, shape says {b} x {sl}")
-        params = {k: v for k, v in (body.get("parameters") or {}).items() if k in allowed}
+        params = settings(body.get("parameters") or {})
         pad = int((body.get("parameters") or {}).get("pad_token_id", 0))
         try:
             results = await asyncio.gather(*[batcher.submit([int(x) for x in flat[i * sl : (i + 1) * sl]], **params) for i in range(b)])

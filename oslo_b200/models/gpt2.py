@@ -79,9 +79,9 @@ class GPT2Model(PreTrainedModel):
     def forward(self, input_ids, attention_mask=None, position_ids=None):
         s = input_ids.shape[-1]
         if position_ids is None:
-            from oslo_b200.ops.attention import decode_offset
+            from oslo_b200.ops.attention import decode_positions
 
-            position_ids = (torch.arange(s, device=input_ids.device) + decode_offset()).unsqueeze(0)
+            position_ids = decode_positions(s, input_ids.device)
         x = self.wte(input_ids)
         pos = self.wpe(position_ids)
         if pos.shape[:-1] != x.shape[:-1] and pos.shape[0] != 1:
@@ -103,6 +103,7 @@ class GPT2Model(PreTrainedModel):
 
 class GPT2LMHeadModel(PreTrainedModel):
     config_class = GPT2Config
+    ragged_prompts = True  # positions follow each sequence of the decode cache
     base_model_prefix = "transformer"
 
     def __init__(self, config):
@@ -177,6 +178,8 @@ class GPT2LMHeadModel(PreTrainedModel):
 class MoEGPTLMHeadModel(GPT2LMHeadModel):
     """GPT-2 style decoder intended for :class:`oslo_b200.parallel.ExpertParallel`, which turns the FFN of the layers
     chosen by ``config.moe_every`` into mixtures of ``config.num_experts`` experts."""
+
+    ragged_prompts = False  # padding would take places in the experts' buffers
 
     def moe_layer_ids(self):
         every = getattr(self.config, "moe_every", 2)

@@ -55,9 +55,9 @@ class GPTNeoXAttention(nn.Module):
         heads = qkv.shape[-1] // (3 * self.head_size)
         rope = None
         if self.rotary_ndims > 0:
-            from oslo_b200.ops.attention import decode_offset
+            from oslo_b200.ops.attention import decode_limit
 
-            cos, sin = self._tables(s + decode_offset(), qkv.device)  # incremental decoding rotates at offset positions
+            cos, sin = self._tables(s + decode_limit(), qkv.device)  # incremental decoding rotates at offset positions
             rope = (cos, sin, self.rotary_ndims, True)
         return OF.qkv_attention(qkv, heads, self.head_size, layout="h3d", causal=True, rope=rope, mask=attention_mask)
 
@@ -200,6 +200,7 @@ class GPTNeoXModel(PreTrainedModel):
 
 class GPTNeoXForCausalLM(PreTrainedModel):
     config_class = GPTNeoXConfig
+    ragged_prompts = True  # positions follow each sequence of the decode cache
     base_model_prefix = "gpt_neox"
 
     def __init__(self, config):

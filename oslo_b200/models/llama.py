@@ -45,8 +45,12 @@ class LlamaAttention(nn.Module):
         b, s = q.shape[0], q.shape[1]  # from the projection: under sequence parallelism it has gathered the token shards
         hq, hkv = q.shape[-1] // self.head_dim, k.shape[-1] // self.head_dim
         q, k, v = q.view(b, s, hq, self.head_dim), k.view(b, s, hkv, self.head_dim), v.view(b, s, hkv, self.head_dim)
-        from oslo_b200.ops.attention import decode_offset
+        from oslo_b200.ops.attention import decode_limit, decode_offset, paged_cache
 
+        cache = paged_cache()
+        if cache is not None:  # the pages hold the key heads once, and sequences may differ in length
+            cos, sin = self._tables(s + decode_limit(), x.device)
+            return self.o_proj(cache.attend(q, k, v, rope=(cos, sin, self.head_dim, True), mask=attention_mask))
         off = decode_offset()
         cos, sin = self._tables(s + off, x.device)
         pos = (torch.arange(s, device=x.device) + off).repeat(b) if off else None  # incremental decoding
@@ -109,6 +113,7 @@ class LlamaModel(PreTrainedModel):
 
 class LlamaForCausalLM(PreTrainedModel):
     config_class = LlamaConfig
+    ragged_prompts = True  # positions follow each sequence of the decode cache
     base_model_prefix = "model"
 
     def __init__(self, config):

@@ -17,6 +17,7 @@ import torch
 
 from . import _lib
 from .gemm import gemm, supported
+from .paged import PagedDecodeCache
 from .softmax import softmax_backward_, softmax_inplace_, softmax_reference
 
 
@@ -122,13 +123,14 @@ class DecodeCache:
         return self.k[i], self.v[i]
 
 
-_CACHE: Optional[DecodeCache] = None
+_CACHE = None  # the active DecodeCache or PagedDecodeCache
 
 
 class decode_cache:
-    """Context manager that makes ``cache`` the active :class:`DecodeCache` (inference only)."""
+    """Context manager that makes ``cache``, a :class:`DecodeCache` or a :class:`oslo_b200.ops.paged.PagedDecodeCache`, the active
+    one (inference only)."""
 
-    def __init__(self, cache: DecodeCache):
+    def __init__(self, cache):
         self.cache = cache
 
     def __enter__(self):
@@ -144,6 +146,23 @@ class decode_cache:
 def decode_offset() -> int:
     """Tokens already held by the active decode cache (0 without one): the position of the first new token."""
     return _CACHE.offset if _CACHE is not None else 0
+
+
+def decode_limit() -> int:
+    """Tokens held by the longest sequence of the active decode cache (0 without one)."""
+    return _CACHE.longest if isinstance(_CACHE, PagedDecodeCache) else decode_offset()
+
+
+def decode_positions(s: int, device) -> torch.Tensor:
+    """Positions of the next ``s`` tokens under the active decode cache: ``[1, s]``, or ``[batch, s]`` where sequences differ."""
+    if isinstance(_CACHE, PagedDecodeCache):
+        return _CACHE.positions(s, device)
+    return (torch.arange(s, device=device) + decode_offset()).unsqueeze(0)
+
+
+def paged_cache() -> Optional[PagedDecodeCache]:
+    """The active decode cache if it is a paged one and no gradient is recorded."""
+    return _CACHE if isinstance(_CACHE, PagedDecodeCache) and not torch.is_grad_enabled() else None
 
 
 def _cached_attention(q, k, v, scale, mask=None):
@@ -166,7 +185,16 @@ def attention(q, k, v, causal: bool = True, scale: Optional[float] = None, mask=
     b, s, nh, hd = q.shape
     scale = scale if scale is not None else 1.0 / math.sqrt(hd)
     if _CACHE is not None and causal and not torch.is_grad_enabled():
+        if isinstance(_CACHE, PagedDecodeCache):
+            return _CACHE.attend(q, k, v, scale, mask=mask)
         return _cached_attention(q, k, v, scale, mask)
+    return dense_attention(q, k, v, causal, scale, mask)
+
+
+def dense_attention(q, k, v, causal: bool = True, scale: Optional[float] = None, mask=None):
+    """:func:`attention` over the given keys and values alone, whatever decode cache is active."""
+    b, s, nh, hd = q.shape
+    scale = scale if scale is not None else 1.0 / math.sqrt(hd)
     if mask is None and flash_supported(q, k, v):
         return _FlashAttentionFn.apply(q, k, v, causal, float(scale))
     if mask is None and supported(q, k) and s % 8 == 0 and hd % 8 == 0 and k.shape[1] == s:
@@ -380,6 +408,8 @@ def qkv_attention(qkv, heads: int, head_dim: int, layout: str = "h3d", causal: b
     if _CACHE is not None and causal and not torch.is_grad_enabled():
         shape5 = (b, s, heads, 3, head_dim) if layout == "h3d" else (b, s, 3, heads, head_dim)
         q, k, v = _split_qkv(qkv.view(shape5), layout)
+        if isinstance(_CACHE, PagedDecodeCache):
+            return _CACHE.attend(q, k, v, scale, rope, mask)
         if rope is not None:
             cos, sin, rot, neox = rope
             pos = (torch.arange(s, device=qkv.device) + _CACHE.offset).repeat(b)

@@ -255,6 +255,130 @@ def _attention_plan(dtype: int, hd: int, group: int, masked: bool, device: int):
     return n * _lib.num_sms(device), lib.oslo_paged_attention_block_bytes(hd, group)
 
 
+# ------------------------------------------------------------------------------------------------ the cache of a generation
+class PagedDecodeCache:
+    """Keys and values of the tokens a model has already seen, in pages (``with decode_cache(cache): model(ids)``).
+
+    A drop-in for :class:`oslo_b200.ops.attention.DecodeCache` except for beam search: pages of ``page_size`` tokens are taken
+    from a pool as sequences grow, nothing is copied when they do, and the sequences of the batch may have different lengths.
+    The first forward takes the prompts, padded on the right; ``begin_forward(counts)`` says how many tokens of each row are real.
+    Its attention runs over the prompts themselves; every later forward stores its tokens and attends over the pages.  The
+    pools ``[pages, kv_heads, page_size, head_dim]`` of a layer are made when its first keys come.
+
+    ``max_tokens``: tokens a sequence may reach; ``num_pages``: pages of a layer's pool (default: enough for every sequence).
+    """
+
+    def __init__(self, max_tokens: int, page_size: int = 64, num_pages: Optional[int] = None):
+        if page_size <= 0 or page_size % 16:
+            raise ValueError(f"page_size is a positive multiple of 16: got {page_size}")
+        if max_tokens <= 0:
+            raise ValueError(f"max_tokens is positive: got {max_tokens}")
+        self.max_tokens, self.page_size, self.num_pages = max_tokens, page_size, num_pages
+        self.k_pages: List[torch.Tensor] = []
+        self.v_pages: List[torch.Tensor] = []
+        self.lengths: List[int] = []  # tokens of each sequence
+        self.pages: List[List[int]] = []  # pages of each sequence, in order
+        self.block_table: Optional[torch.Tensor] = None  # int32 [batch, pages of max_tokens], on the device
+        self._free: List[int] = []
+        self._held = self._after = None  # int32 [batch] on the device: tokens before and after this forward
+        self._counts: Optional[List[int]] = None
+        self._layer = self._new = 0
+
+    @property
+    def offset(self) -> int:
+        """Tokens of every sequence, where all have as many."""
+        if len(set(self.lengths)) > 1:
+            raise RuntimeError("the sequences of this cache have different lengths: this model takes one position for all of them")
+        return self.lengths[0] if self.lengths else 0
+
+    @property
+    def longest(self) -> int:
+        return max(self.lengths, default=0)
+
+    def positions(self, s: int, device) -> torch.Tensor:
+        """Positions of the next ``s`` tokens: ``[batch, s]``, or ``[1, s]`` before the first forward."""
+        new = torch.arange(s, device=device)
+        return new.unsqueeze(0) if self._held is None else self._held.unsqueeze(1) + new
+
+    def begin_forward(self, counts: Optional[Sequence[int]] = None):
+        self._layer, self._counts = 0, None if counts is None else [int(c) for c in counts]
+
+    def advance(self, n: int):
+        """After a forward over ``n`` tokens a row."""
+        self.lengths = [have + new for have, new in zip(self.lengths, self._counts or [n] * len(self.lengths))]
+        self._held, self._counts = self._after, None
+
+    def reorder(self, index: torch.Tensor):
+        raise RuntimeError("the paged cache does not follow beams: search beams over the dense cache")
+
+    def _grow(self, b: int, s: int, device):
+        """Pages for the tokens of this forward (once per forward, before its first layer stores any)."""
+        if self.block_table is None:
+            width = -(-self.max_tokens // self.page_size)
+            if self.num_pages is None:
+                self.num_pages = b * width
+            self.lengths, self.pages = [0] * b, [[] for _ in range(b)]
+            self._free = list(range(self.num_pages - 1, -1, -1))
+            self._rows = torch.zeros(b, width, dtype=torch.int32)
+            self.block_table = self._rows.to(device)
+            self._held = torch.zeros(b, dtype=torch.int32, device=device)
+        counts = self._counts if self._counts is not None else [s] * b
+        if len(self.lengths) != b or len(counts) != b or min(counts) < 0 or max(counts) > s:
+            raise ValueError(f"the cache holds {len(self.lengths)} sequences; this forward has {b} rows of {s} tokens, of which {counts} "
+                             "are real")
+        need = [-(-(have + new) // self.page_size) - len(own) for have, new, own in zip(self.lengths, counts, self.pages)]
+        if max(have + new for have, new in zip(self.lengths, counts)) > self.max_tokens:
+            raise ValueError(f"a sequence would pass max_tokens = {self.max_tokens}")
+        if sum(n for n in need if n > 0) > len(self._free):
+            raise RuntimeError(f"the page pool is exhausted: {sum(n for n in need if n > 0)} pages are needed, {len(self._free)} of "
+                               f"{self.num_pages} are free")
+        for row, n in enumerate(need):
+            for _ in range(n):
+                self._rows[row, len(self.pages[row])] = self._free[-1]
+                self.pages[row].append(self._free.pop())
+        if any(n > 0 for n in need):
+            self.block_table = self._rows.to(device)
+        self._new = s
+        if self._counts is None:
+            self._count, self._after = None, self._held + s
+        else:
+            self._count = torch.tensor(counts, dtype=torch.int32, device=device)
+            self._after = self._held + self._count
+
+    def attend(self, q, k, v, scale: Optional[float] = None, rope=None, mask=None):
+        """What a layer's causal attention calls: ``q [b, s, heads, head_dim]``, ``k``, ``v`` ``[b, s, kv_heads, head_dim]`` of the
+        new tokens -> ``[b, s, heads * head_dim]``.  ``rope = (cos, sin, rot_dim, neox)`` rotates queries and keys first; ``mask`` is
+        additive over all tokens so far.  Layers are told apart by the order of their calls."""
+        from .attention import dense_attention
+        from .softmax import apply_rope
+
+        b, s, hq, hd = q.shape
+        if self._layer == 0:
+            self._grow(b, s, q.device)
+        i = self._layer
+        self._layer += 1
+        if i == len(self.k_pages):
+            for pools in (self.k_pages, self.v_pages):
+                pools.append(torch.zeros(self.num_pages, k.shape[2], self.page_size, hd, dtype=k.dtype, device=k.device))
+        pools = self.k_pages[i], self.v_pages[i]
+        if self.longest == 0:  # the prompts attend to themselves
+            if rope is not None:
+                cos, sin, rot, neox = rope
+                pos = torch.arange(s, device=q.device).repeat(b)
+                q = apply_rope(q.contiguous(), cos, sin, rot, neox, positions=pos)
+                k = apply_rope(k.contiguous(), cos, sin, rot, neox, positions=pos)
+            paged_kv_append(k, v, *pools, self.block_table, self._held, count=self._count)
+            if k.shape[2] != hq:
+                k, v = (t.repeat_interleave(hq // t.shape[2], dim=2) for t in (k, v))
+            return dense_attention(q, k, v, True, scale, mask)
+        if self._count is not None and min(self._counts) < s:
+            raise ValueError("only prompts may be padded: a later forward takes as many tokens of every row")
+        turned = paged_kv_append(k, v, *pools, self.block_table, self._held, q=q, rope=rope)
+        if mask is not None:
+            mask = mask[..., -s:, :]
+        return paged_attention(turned, *pools, self.block_table, self._after, scale, mask)
+
+
 # ------------------------------------------------------------------------------------------------ plain forms
 def _rows_of(block_table, page: int, pages: int, row: int, n: int):
     """Page and row in it of tokens ``0 .. n`` of one sequence."""
