@@ -8,6 +8,9 @@ Two shared objects are produced next to this file's package:
   Python through ``ctypes`` (no libtorch dependency, so a rebuild takes seconds).
 * ``oslo_b200/_lib/liboslo_b200_cpu.so``   ``csrc/cpu/*.cpp`` compiled by g++ with
   AVX-512/AVX2 + OpenMP (CPU Adam / Adagrad, memory planner, partitioner core).
+* ``oslo_b200/_lib/_oslo_b200_step.so``  ``csrc/torch/*.cpp`` against the installed PyTorch: a Python module that calls
+  the decoding step's entry points of the CUDA library without Python's per-argument cost (optional: the same calls go
+  through ``ctypes`` without it).
 
 Replaces the reference's per-extension JIT ``Binder`` (``oslo/torch/_C/__init__.py:249-680``).
 Run as ``python -m oslo_b200.csrc.build`` or call :func:`build_all`.
@@ -107,8 +110,37 @@ def build_cpu() -> Path:
     return out
 
 
+def build_step() -> Path:
+    """The module of ``csrc/torch``, compiled against this interpreter's PyTorch."""
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+
+    OBJ_DIR.mkdir(parents=True, exist_ok=True)
+    src, out, stamp_file = CSRC / "torch" / "step_calls.cpp", LIB_DIR / "_oslo_b200_step.so", OBJ_DIR / "step_calls.stamp"
+    flags = ["-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    stamp = _stamp(src, flags + [torch.__version__, sys.version])
+    if out.exists() and stamp_file.exists() and stamp_file.read_text() == stamp:
+        return out
+    cmd = ["g++", *flags]
+    for path in [*include_paths(device_type="cuda"), sysconfig.get_paths()["include"]]:
+        cmd += ["-isystem", path]
+    cmd += [str(src), "-o", str(out)]
+    for path in library_paths():
+        cmd += [f"-L{path}", f"-Wl,-rpath,{path}"]
+    cmd += ["-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed:\n{res.stdout}\n{res.stderr}")
+    stamp_file.write_text(stamp)
+    return out
+
+
 def build_all(verbose: bool = False):
-    return build_cuda(verbose), build_cpu()
+    built = build_cuda(verbose), build_cpu()
+    build_step()
+    return built
 
 
 if __name__ == "__main__":

@@ -13,6 +13,7 @@
 // every element's mask is two instructions (10 us).  Adding a cluster's tokens to each other's counters through distributed
 // shared memory, so that a row reads its history once, was slower (105 us): frequent tokens serialise the remote atomics.
 #include "common.cuh"
+#include "step_args.h"
 
 namespace oslo {
 
@@ -220,13 +221,6 @@ int process_logits_launch(LogitsParams& p, cudaStream_t st) {
 }
 
 }  // namespace oslo
-
-// Everything a call needs, eight bytes each.  Strides in elements.
-struct OsloProcessLogitsArgs {
-  long long x, y, tokens, token_lens, prompt_lens, rep, pres, freq, bias, allowed, stream;  // addresses; from tokens on they may be 0
-  long long x_stride, y_stride, tok_stride, bias_stride, allowed_stride, rows, vocab, history, tok64, dtype;
-  double rep_s, pres_s, freq_s;
-};
 
 extern "C" int oslo_process_logits(const OsloProcessLogitsArgs* a) {
   using namespace oslo;

@@ -8,6 +8,7 @@
 // Pools are [pages, kv_heads, page_size, head_dim]: the tokens of one head inside a page are contiguous, which is what the
 // attention over the pages streams.
 #include "common.cuh"
+#include "step_args.h"
 
 namespace oslo {
 
@@ -235,13 +236,6 @@ int paged_append_launch(const PagedAppendParams& p, cudaStream_t st) {
 }
 
 }  // namespace oslo
-
-// Everything a call needs, eight bytes each.  Strides in elements.
-struct OsloPagedAppendArgs {
-  long long q, k, v, q_out, k_pages, v_pages, table, start, count, cosb, sinb, status, stream;  // addresses; q, count, cosb may be 0
-  long long q_b, q_s, q_h, k_b, k_s, k_h, v_b, v_s, v_h, k_page, k_head, v_page, v_head, table_row;
-  long long b, s, hq, hkv, d, rot, neox, positions, page_size, max_pages, num_pages, dtype;
-};
 
 extern "C" int oslo_paged_kv_append(const OsloPagedAppendArgs* a) {
   using namespace oslo;

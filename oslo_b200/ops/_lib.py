@@ -8,7 +8,10 @@ library is not needed.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
+import warnings
 from functools import lru_cache
 from pathlib import Path
 
@@ -68,6 +71,28 @@ def _load_cuda_lib() -> ctypes.CDLL:
                 f"{path} not found: run `python -m oslo_b200.csrc.build` (needs nvcc) before using the CUDA ops"
             )
     return ctypes.CDLL(str(path))
+
+
+@lru_cache(maxsize=None)
+def step_calls():
+    """The module that launches a decoding step's kernels without Python's per-argument cost, bound to the kernel library, or
+    ``None`` where it is not built for this PyTorch (the same kernels are then called through ``ctypes``)."""
+    path = _LIB_DIR / "_oslo_b200_step.so"
+    try:
+        if not path.exists() and os.environ.get("OSLO_B200_AUTOBUILD", "1") == "1":
+            from oslo_b200.csrc.build import build_step
+
+            build_step()
+        loader = importlib.machinery.ExtensionFileLoader("_oslo_b200_step", str(path))
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_oslo_b200_step", loader))
+        loader.exec_module(module)
+    except (ImportError, OSError, RuntimeError) as e:
+        warnings.warn(f"the step module is not available, its calls go through ctypes: {e}")
+        return None
+    dll = _load_cuda_lib()
+    module.bind(*(ctypes.cast(getattr(dll, name), ctypes.c_void_p).value for name in (
+        "oslo_paged_kv_append", "oslo_paged_attention", "oslo_paged_attention_workspace_bytes", "oslo_process_logits")))
+    return module
 
 
 @lru_cache(maxsize=None)

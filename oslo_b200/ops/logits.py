@@ -57,6 +57,10 @@ def process_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     ``allowed``: int32 ``[rows or 1, ceil(vocab / 32)]`` from :func:`pack_token_mask`; a row that allows nothing is all ``-inf``.
     The result is a new tensor, or ``out`` (which may be ``logits``).  For inference: no gradient.
     """
+    if logits.is_cuda and out is None:
+        y = _step(logits, tokens, token_lengths, prompt_lengths, repetition_penalty, presence_penalty, frequency_penalty, bias, allowed)
+        if y is not NotImplemented:
+            return y
     dtype, dev = logits.dtype, logits.device
     if logits.dim() != 2 or dtype not in _DT:
         raise ValueError(f"logits are float32, float16 or bfloat16 [rows, vocab]: got {dtype} {tuple(logits.shape)}")
@@ -127,6 +131,21 @@ def process_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
         freq_s))
     if rc:
         raise RuntimeError(f"oslo_process_logits failed ({rc})")
+    return y
+
+
+_direct = None
+
+
+def _step(*args):
+    """The call through the step module, where its arguments are ordinary; else ``NotImplemented``."""
+    global _direct
+    if _direct is None:
+        module = _lib.step_calls()
+        _direct = module.process_logits if module is not None else lambda *args: NotImplemented
+    y = _direct(*args)
+    if y is not NotImplemented:
+        _lib.native_calls += 1
     return y
 
 

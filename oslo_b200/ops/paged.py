@@ -27,8 +27,6 @@ _DT = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # of a device's current stream
 _device = getattr(torch._C, "_cuda_getDevice", None)
 MAX_HEAD_DIM = 256
-#: tokens that a block of the one-launch attention takes at most
-CLUSTER_TOKENS = 1024
 _INFERENCE = "the paged cache is for inference: call it under torch.no_grad() or detach its inputs"
 
 
@@ -109,6 +107,10 @@ def paged_kv_append(k, v, k_pages, v_pages, block_table, start, count=None, q=No
 
     Returns the rotated ``q`` ``[b, s, heads, head_dim]`` as a new tensor (rows of padding are zeros), or ``None`` without ``q``.
     """
+    if k.is_cuda:
+        out = _step(0, k, v, k_pages, v_pages, block_table, start, count, q, rope)
+        if out is not NotImplemented:
+            return out
     shape, dtype, dev = k.shape, k.dtype, k.get_device()
     if len(shape) != 4 or v.shape != shape or v.dtype != dtype or v.get_device() != dev:
         raise ValueError(f"k and v are [b, s, kv_heads, head_dim], both alike: got {tuple(shape)} {dtype} and {tuple(v.shape)} "
@@ -142,7 +144,7 @@ def paged_kv_append(k, v, k_pages, v_pages, block_table, start, count=None, q=No
             op = out.data_ptr()
     k, ks, kx = _aligned(k)
     v, vs, vx = _aligned(v)
-    rc = (_append_fn or _load()[0])(_APPEND_ARGS.pack(
+    rc = _load()[0](_APPEND_ARGS.pack(
         qp, kx, vx, op, kp, vp, block_table.data_ptr(), start.data_ptr(), 0 if count is None else count.data_ptr(),
         cos.data_ptr() if rot else 0, sin.data_ptr() if rot else 0, _status_ptr(dev), _raw_stream(dev),
         qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], kps[0], kps[1], vps[0], vps[1], row,
@@ -163,6 +165,10 @@ def paged_attention(q, k_pages, v_pages, block_table, lengths, scale: Optional[f
 
     Returns ``[b, s, heads * head_dim]``, like :func:`oslo_b200.ops.attention.attention`.
     """
+    if q.is_cuda:
+        out = _step(1, q, k_pages, v_pages, block_table, lengths, scale, mask)
+        if out is not NotImplemented:
+            return out
     shape, dtype, dev = q.shape, q.dtype, q.get_device()
     if len(shape) != 4:
         raise ValueError(f"q is [b, s, heads, head_dim]: got {tuple(shape)}")
@@ -190,7 +196,6 @@ def paged_attention(q, k_pages, v_pages, block_table, lengths, scale: Optional[f
             return paged_attention(q, k_pages, v_pages, block_table, lengths, scale, mask)
     q, qs, qp = _aligned(q)
     out = q.new_empty((b, s, hq * hd))
-    most = width * page
     mptr = mb = mt = mlen = 0
     if mask is not None:
         mlen = mask.shape[3]
@@ -198,61 +203,58 @@ def paged_attention(q, k_pages, v_pages, block_table, lengths, scale: Optional[f
         if mask.stride(3) != 1:
             mask = mask.contiguous()
         mptr, mb, mt = mask.data_ptr(), mask.stride(0), mask.stride(2)
-        most = min(most, mlen)
-    kind = _DT[dtype]
-    blocks, block_bytes = _attention_plan(kind, hd, group, mptr != 0, dev)
-    # Where the table keeps sequences short and the GPU holds all of it at once, a cluster of blocks takes each (query token, key
-    # head) and one launch does it (200 tokens, 16 heads: 5.5 us, against 8.4 us for two launches).  Else
-    # equal ranges of the work go to as many blocks as the device holds (no more than the longest possible sequences have work
-    # for, in units of 32 tokens, the smallest of the kernel's) and a second launch joins what they share.
-    segments = b * s * hkv * -(-group // (16 if group > 8 else 8))
-    cluster = 8
-    while cluster > 1 and (segments * cluster > blocks or cluster * 32 > most):
-        cluster //= 2
-    grid = room = wp = 0
-    if most > CLUSTER_TOKENS * cluster or segments > blocks:
-        cluster = 0
-        grid = max(1, min(blocks, segments * -(-most // 32)))
-        room = grid * block_bytes
+    args = [qp, kp, vp, block_table.data_ptr(), lengths.data_ptr(), mptr, out.data_ptr(), 0, _status_ptr(dev), _raw_stream(dev),
+            qs[0], qs[1], qs[2], ks[0], ks[1], vs[0], vs[1], row, mb, mt,
+            b, s, hkv, group, hd, page, width, pages, mlen, _DT[dtype], scale]
+    _, attend, workspace = _load()
+    room = workspace(_ATTEND_ARGS.pack(*args))
+    if room > 0:
         ws = torch.empty(room, dtype=torch.uint8, device=q.device)
-        wp = ws.data_ptr()
-    rc = (_attend_fn or _load()[1])(_ATTEND_ARGS.pack(
-        qp, kp, vp, block_table.data_ptr(), lengths.data_ptr(), mptr, out.data_ptr(), wp, _status_ptr(dev), _raw_stream(dev),
-        qs[0], qs[1], qs[2], ks[0], ks[1], vs[0], vs[1], row, mb, mt,
-        b, s, hkv, group, hd, page, width, pages, mlen, kind, grid, cluster, room, scale))
+        args[7] = ws.data_ptr()
+    rc = attend(_ATTEND_ARGS.pack(*args)) if room >= 0 else room
     if rc:
         raise RuntimeError(f"oslo_paged_attention failed ({rc})")
     return out
 
 
+_direct = None
+
+
+def _step(which, *args):
+    """The call through the step module, where its arguments are ordinary; else ``NotImplemented``."""
+    global _direct
+    if _direct is None:
+        module = _lib.step_calls()
+        _direct = (module.paged_kv_append, module.paged_attention) if module is not None else (_not_built, _not_built)
+    out = _direct[which](*args)
+    if out is not NotImplemented:
+        _lib.native_calls += 1
+    return out
+
+
+def _not_built(*args):
+    return NotImplemented
+
+
 # arguments travel as one struct of eight-byte fields: ctypes converts one value instead of forty
 _APPEND_ARGS = struct.Struct("=39q")
-_ATTEND_ARGS = struct.Struct("=33qd")
-_append_fn = _attend_fn = None
-
-
+_ATTEND_ARGS = struct.Struct("=30qd")
+@lru_cache(maxsize=None)
 def _load():
-    global _append_fn, _attend_fn
     dll, lib = _lib._load_cuda_lib(), _lib.cuda_lib()
-    dll.oslo_paged_kv_append.argtypes = dll.oslo_paged_attention.argtypes = [ctypes.c_char_p]
-    _append_fn, _attend_fn = lib.oslo_paged_kv_append, lib.oslo_paged_attention
-    return _append_fn, _attend_fn
+    for name in ("oslo_paged_kv_append", "oslo_paged_attention", "oslo_paged_attention_workspace_bytes"):
+        getattr(dll, name).argtypes = [ctypes.c_char_p]
+    dll.oslo_paged_attention_workspace_bytes.restype = ctypes.c_longlong
+    return lib.oslo_paged_kv_append, lib.oslo_paged_attention, lib.oslo_paged_attention_workspace_bytes
 
 
 @lru_cache(maxsize=None)
 def _status_ptr(device: int) -> int:
-    return _lib.status_word(torch.device("cuda", device)).data_ptr()
-
-
-@lru_cache(maxsize=None)
-def _attention_plan(dtype: int, hd: int, group: int, masked: bool, device: int):
-    """(blocks that the device holds at once, workspace bytes of a block) of the attention kernel for these types and sizes."""
-    lib = _lib._load_cuda_lib()
-    lib.oslo_paged_attention_block_bytes.restype = ctypes.c_longlong
-    n = lib.oslo_paged_attention_resident_parts(dtype, hd, group, 1 if masked else 0)
-    if n <= 0:
-        raise RuntimeError(f"oslo_paged_attention_resident_parts failed ({n})")
-    return n * _lib.num_sms(device), lib.oslo_paged_attention_block_bytes(hd, group)
+    ptr = _lib.status_word(torch.device("cuda", device)).data_ptr()
+    module = _lib.step_calls()
+    if module is not None:
+        module.status(device, ptr)  # from now on the step module takes this device's calls
+    return ptr
 
 
 # ------------------------------------------------------------------------------------------------ the cache of a generation

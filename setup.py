@@ -24,6 +24,7 @@ class BuildWithNative(build_py):
                 native.build_cpu()
                 try:
                     native.build_cuda()
+                    native.build_step()
                 except Exception as e:  # no nvcc on this machine: the host library is still useful (CPU ranks, tests)
                     print(f"[oslo_b200] CUDA kernels not built at install time: {e}", file=sys.stderr)
             finally:
@@ -45,7 +46,8 @@ setup(
     long_description=open(os.path.join(ROOT, "README.md"), encoding="utf-8").read(),
     long_description_content_type="text/markdown",
     packages=find_packages(include=["oslo_b200", "oslo_b200.*"]),
-    package_data={"oslo_b200": ["_lib/*.so", "csrc/*.cu", "csrc/*.cuh", "csrc/*.h", "csrc/cpu/*.cpp", "csrc/cpu/*.h"]},
+    package_data={"oslo_b200": ["_lib/*.so", "csrc/*.cu", "csrc/*.cuh", "csrc/*.h", "csrc/cpu/*.cpp", "csrc/cpu/*.h",
+                                "csrc/torch/*.cpp"]},
     python_requires=">=3.10",
     install_requires=["torch>=2.4", "numpy"],
     extras_require={"hf": ["transformers", "tokenizers"], "serve": ["fastapi", "uvicorn"], "test": ["pytest"]},

@@ -333,3 +333,66 @@ def test_generation_in_16_bits_follows_the_dense_cache(dtype):
     # 2 layers x 2 residual additions and projections, each rounding both runs: 16 half steps, and their spread over later layers
     assert rel <= 16 * eps, rel
     assert math.isfinite(rel)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_calls_with_and_without_the_step_module_agree(dtype, monkeypatch):
+    from oslo_b200.ops import _lib, logits as logits_ops, paged as paged_ops
+
+    module = _lib.step_calls()
+    assert module is not None
+    taken = []
+
+    def through(f):
+        def call(*args):
+            out = f(*args)
+            taken.append(out is not NotImplemented)
+            return out
+
+        return call
+
+    def run(width, most):
+        torch.manual_seed(0)  # both sides get the same inputs
+        q, k, v, kp, vp, table, held, rope, x, tokens, lens = _state(40, width=width, most=most, dtype=dtype)
+        b = q.shape[0]
+        mask = torch.randn(b, 1, 1, width * 16, device="cuda")
+        kp, vp = kp.clone(), vp.clone()
+        none = torch.zeros_like(held)
+        out = [OF.paged_kv_append(k, v, kp, vp, table, held, count=none + 1, q=q, rope=rope),
+               OF.paged_kv_append(k, v, kp, vp, table, held)]
+        out += [OF.paged_attention(q, kp, vp, table, held + 1, **kw)
+                for kw in (dict(), dict(scale=0.2), dict(mask=mask), dict(mask=mask[:1]), dict(mask=mask.double()))]
+        rates = torch.rand(b, device="cuda") + 0.5
+        allowed = OF.pack_token_mask(torch.rand(b, 5000, device="cuda", generator=torch.Generator("cuda").manual_seed(1)) < 0.5)
+        for kw in (dict(), dict(tokens=tokens, repetition_penalty=1.5), dict(tokens=tokens.int(), presence_penalty=rates * 0 + 0.3),
+                   dict(tokens=tokens, token_lengths=lens, prompt_lengths=lens // 2, frequency_penalty=1),
+                   dict(bias=x[0]), dict(bias=x * 2, allowed=allowed), dict(allowed=allowed[:1]), dict(bias=x[0].half())):
+            out.append(OF.process_logits(x.to(dtype), **kw))
+        return out + [kp, vp]
+
+    for width, most in ((40, 600), (400, 6000)):
+        run(width, most)
+        monkeypatch.setattr(paged_ops, "_direct", tuple(through(f) for f in (module.paged_kv_append, module.paged_attention)))
+        monkeypatch.setattr(logits_ops, "_direct", through(module.process_logits))
+        before = _lib.native_calls
+        a = run(width, most)
+        assert _lib.native_calls - before >= 15 and sum(taken) >= 11 and not all(taken)
+        monkeypatch.setattr(paged_ops, "_direct", (paged_ops._not_built,) * 2)
+        monkeypatch.setattr(logits_ops, "_direct", lambda *args: NotImplemented)
+        b = run(width, most)
+        for i, (x, y) in enumerate(zip(a, b)):
+            assert (x is None and y is None) or torch.equal(x.nan_to_num(), y.nan_to_num()), i
+        taken.clear()
+
+
+def test_step_module_leaves_what_is_not_ordinary():
+    from oslo_b200.csrc.build import build_step
+    from oslo_b200.ops import _lib
+
+    build_step()
+    module = _lib.step_calls()
+    t = torch.zeros(2, 1, 4, 64)
+    for args in ((), (t,) * 7, (t, t, t, t, t, None, None), (None,) * 9, (t,) * 9, (1,) * 9, ("q",) * 7):
+        for f in (module.paged_kv_append, module.paged_attention, module.process_logits):
+            assert f(*args) is NotImplemented
