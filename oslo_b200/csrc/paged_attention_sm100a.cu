@@ -24,7 +24,7 @@
 // (Rows of the ring are 16 bytes longer than a head, which keeps the value loads free of bank conflicts.)  tcgen05 would
 // multiply 128 rows where there are 1 to 16: the tensor cores are not what bounds this.
 // The probabilities enter the second product as the sum of two 16-bit numbers (high part and remainder), which keeps 16 bits
-// and more of each; fp32 inputs are split in the same way into tf32 parts (three products), which keeps 21 bits.
+// and more of each.
 #include "common.cuh"
 #include "step_args.h"
 
@@ -104,26 +104,6 @@ struct Mma16<__half> {
   static OSLO_DEVINL float low(uint32_t r) { return __low2float(reinterpret_cast<const __half2&>(r)); }
   static OSLO_DEVINL float high(uint32_t r) { return __high2float(reinterpret_cast<const __half2&>(r)); }
 };
-// D[16 x 8] += A[16 x 8] B[8 x 8], tf32 operands
-OSLO_DEVINL void mma_tf32(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-OSLO_DEVINL uint32_t tf32_hi(float x) {
-  uint32_t r;
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
-  return r;
-}
-OSLO_DEVINL uint32_t tf32_lo(float x, uint32_t hi) { return tf32_hi(x - __uint_as_float(hi)); }
-// a * b with both split: the product of the two remainders (2^-22 relative) is left out
-OSLO_DEVINL void mma_3xtf32(float (&c)[4], const float (&a)[4], float b0, float b1) {
-  const uint32_t h0 = tf32_hi(a[0]), h1 = tf32_hi(a[1]), h2 = tf32_hi(a[2]), h3 = tf32_hi(a[3]);
-  const uint32_t g0 = tf32_hi(b0), g1 = tf32_hi(b1);
-  mma_tf32(c, tf32_lo(a[0], h0), tf32_lo(a[1], h1), tf32_lo(a[2], h2), tf32_lo(a[3], h3), g0, g1);
-  mma_tf32(c, h0, h1, h2, h3, tf32_lo(b0, g0), tf32_lo(b1, g1));
-  mma_tf32(c, h0, h1, h2, h3, g0, g1);
-}
-
 // s / l, zeros where nothing was seen
 OSLO_DEVINL void pa_store(float* dst, float4 s, float l) {
   const float inv = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
@@ -137,11 +117,27 @@ OSLO_DEVINL void pa_store(T* dst, float4 s, float l) {
   *reinterpret_cast<uint2*>(dst) = r;
 }
 
-// T: element type; DP: head_dim rounded up to 64, 128 or 256; WIDE: 9 to 16 query heads per block instead of up to 8
+// Scores and weights of one mask mode.  With a mask the scores stay in natural units: a mask of the type's lowest value times
+// log2(e) would leave its range.
+template <bool MASK>
+struct AttnMath {
+  static OSLO_DEVINL float score(const PagedAttnParams& p, float s, float add) {
+    return MASK ? fmaf(s, p.scale, add) : s * (p.scale * kLog2e);
+  }
+  // exp(x - m); m = -inf: nothing was seen yet
+  static OSLO_DEVINL float weight(float x, float m) {
+    const float mm = m == -INFINITY ? 0.f : m;
+    return ex2(MASK ? (x - mm) * kLog2e : x - mm);
+  }
+};
+
+// What a warp keeps of a segment and does with a tile.  T: element type; DP: head_dim rounded up to 64, 128 or 256; WIDE: 9 to
+// 16 query heads per block instead of up to 8.  This one: 16-bit types on the tensor cores.
 template <typename T, int DP, bool WIDE, bool MASK>
-struct PagedAttn {
-  static constexpr int E = 16 / sizeof(T);           // elements of one load
-  static constexpr int TT = sizeof(T) == 2 ? 16 : 8;  // tokens of one tile
+struct AttnWarp {
+  using Math = AttnMath<MASK>;
+  static constexpr int E = 8;   // elements of one load
+  static constexpr int TT = 16;  // tokens of one tile
   static constexpr int NT = TT / 8;
   static constexpr int KC = DP / (4 * E);   // loads per key and lane
   static constexpr int VC = DP / (8 * E);   // loads per value and lane
@@ -150,20 +146,14 @@ struct PagedAttn {
   static constexpr int ROW = DP + 4;        // padded row of the joining buffer
   static constexpr int WARPS = 4;
   static constexpr int PITCH = DP + E;  // elements between two rows of a tile in the ring
-  static constexpr int TILE = TT * PITCH * 2;  // keys, then values
-  static constexpr int STAGES = DP == 64 ? 3 : 2;
-  // Blocks an SM should hold; the ring's size is chosen for it.
-  static constexpr int BLOCKS = (DP == 64 ? 4 : DP == 128 ? 3 : 2) - (sizeof(T) == 4 || DP == 256 ? 1 : 0);
-  static constexpr size_t kRing = sizeof(T) * TILE * STAGES;  // of one warp; the joining buffer takes its place at the end
-  static constexpr size_t kSmem = kRing * WARPS + sizeof(float) * 2 * WARPS * RT;
-  static_assert(kRing >= sizeof(float) * RT * ROW, "a warp's part of the joining buffer fits its ring");
-  static_assert((kSmem + 1024) * BLOCKS <= 227 * 1024 + 1024, "shared memory of the blocks of an SM");
+  static constexpr int BLOCKS = DP == 64 ? 4 : DP == 128 ? 3 : 1;  // blocks an SM should hold; the ring's size is chosen for it
+  static constexpr int SCRATCH = 0;  // floats of shared memory of the block, beside the rings
 
   uint4 q0[KC], q1[WIDE ? KC : 1];
   float o[VC][E][WIDE ? 4 : 2];
   float m0, m1, l0, l1;
 
-  OSLO_DEVINL void load_q(const PagedAttnParams& p, const T* q, int row0) {
+  OSLO_DEVINL void load_q(const PagedAttnParams& p, const T* q, int row0, float*) {
     const int r = (threadIdx.x & 31) >> 2, quad = threadIdx.x & 3;
 #pragma unroll
     for (int c = 0; c < KC; ++c) {
@@ -184,23 +174,6 @@ struct PagedAttn {
         for (int x = 0; x < (WIDE ? 4 : 2); ++x) o[j][e][x] = 0.f;
   }
 
-  // Starts the copy of one tile, `rows` of whose tokens are seen, into the ring.
-  static OSLO_DEVINL void fill(const PagedAttnParams& p, T* ring, const T* k, const T* v, int rows) {
-    constexpr int CHUNKS = DP / E;
-    const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const T* src = half ? v : k;
-      T* dst = ring + half * TT * PITCH;
-#pragma unroll
-      for (int i = 0; i < TT * CHUNKS / 32; ++i) {
-        const int row = (i * 32 + lane) / CHUNKS, c = (i * 32 + lane) % CHUNKS;
-        const bool valid = row < rows && c * E < p.d;
-        copy16(dst + row * PITCH + c * E, valid ? src + row * p.d + c * E : src, valid);
-      }
-    }
-  }
-
   // Block j of the values of this lane's tokens.
   static OSLO_DEVINL void load_v(uint4 (&vr)[VT], const T* ring, int j, const bool (&seen)[NT][2]) {
     const int lane = threadIdx.x & 31, r = lane >> 2, quad = lane & 3;
@@ -214,7 +187,7 @@ struct PagedAttn {
   }
 
   // One tile of the ring: its TT tokens start at `token`; tokens at or past `limit` are not seen.
-  OSLO_DEVINL void tile(const PagedAttnParams& p, const T* ring, int token, int limit, const float* mask) {
+  OSLO_DEVINL void tile(const PagedAttnParams& p, const T* ring, int token, int limit, const float* mask, float*) {
     const int lane = threadIdx.x & 31, r = lane >> 2, quad = lane & 3;
     float add[NT][2];
     bool seen[NT][2];
@@ -238,15 +211,8 @@ struct PagedAttn {
       for (int c = 0; c < KC; ++c) {
         const uint4 qa = q0[c], qb = WIDE ? q1[WIDE ? c : 0] : make_uint4(0, 0, 0, 0);
         const uint4 kr = *reinterpret_cast<const uint4*>(ring + (n * 8 + r) * PITCH + c * 4 * E + quad * E);
-        if constexpr (sizeof(T) == 2) {
-          Mma16<T>::run(sc[n], qa.x, qb.x, qa.y, qb.y, kr.x, kr.y);
-          Mma16<T>::run(sc[n], qa.z, qb.z, qa.w, qb.w, kr.z, kr.w);
-        } else {
-          const float a[4] = {__uint_as_float(qa.x), __uint_as_float(qb.x), __uint_as_float(qa.y), __uint_as_float(qb.y)};
-          const float b[4] = {__uint_as_float(qa.z), __uint_as_float(qb.z), __uint_as_float(qa.w), __uint_as_float(qb.w)};
-          mma_3xtf32(sc[n], a, __uint_as_float(kr.x), __uint_as_float(kr.y));
-          mma_3xtf32(sc[n], b, __uint_as_float(kr.z), __uint_as_float(kr.w));
-        }
+        Mma16<T>::run(sc[n], qa.x, qb.x, qa.y, qb.y, kr.x, kr.y);
+        Mma16<T>::run(sc[n], qa.z, qb.z, qa.w, qb.w, kr.z, kr.w);
       }
     }
     float t0 = -INFINITY, t1 = -INFINITY;
@@ -254,10 +220,10 @@ struct PagedAttn {
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        sc[n][x] = seen[n][x] ? score(p, sc[n][x], add[n][x]) : -INFINITY;
+        sc[n][x] = seen[n][x] ? Math::score(p, sc[n][x], add[n][x]) : -INFINITY;
         t0 = fmaxf(t0, sc[n][x]);
         if constexpr (WIDE) {
-          sc[n][2 + x] = seen[n][x] ? score(p, sc[n][2 + x], add[n][x]) : -INFINITY;
+          sc[n][2 + x] = seen[n][x] ? Math::score(p, sc[n][2 + x], add[n][x]) : -INFINITY;
           t1 = fmaxf(t1, sc[n][2 + x]);
         }
       }
@@ -269,7 +235,7 @@ struct PagedAttn {
     }
     if (__any_sync(0xffffffffu, t0 > m0 || (WIDE && t1 > m1))) {  // a new maximum: what was summed is scaled to it
       const float n0 = fmaxf(m0, t0), n1 = fmaxf(m1, t1);
-      const float f0 = weight(m0, n0), f1 = WIDE ? weight(m1, n1) : 0.f;
+      const float f0 = Math::weight(m0, n0), f1 = WIDE ? Math::weight(m1, n1) : 0.f;
       m0 = n0, m1 = n1;
       l0 *= f0, l1 *= f1;
 #pragma unroll
@@ -284,71 +250,300 @@ struct PagedAttn {
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        sc[n][x] = weight(sc[n][x], m0);
+        sc[n][x] = Math::weight(sc[n][x], m0);
         l0 += sc[n][x];
         if constexpr (WIDE) {
-          sc[n][2 + x] = weight(sc[n][2 + x], m1);
+          sc[n][2 + x] = Math::weight(sc[n][2 + x], m1);
           l1 += sc[n][2 + x];
         }
       }
-    if constexpr (sizeof(T) == 2) {
-      uint32_t hi[4], lo[4];  // A operand: rows r / r + 8 of tokens 2q.. and 8 + 2q..
+    uint32_t hi[4], lo[4];  // A operand: rows r / r + 8 of tokens 2q.. and 8 + 2q..
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+    for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int x = 0; x < (WIDE ? 2 : 1); ++x) {
-          const float a = sc[n][2 * x], b = sc[n][2 * x + 1];
-          const uint32_t h = Mma16<T>::pack(a, b);
-          hi[2 * n + x] = h;
-          lo[2 * n + x] = Mma16<T>::pack(a - Mma16<T>::low(h), b - Mma16<T>::high(h));
-        }
-      if constexpr (!WIDE) hi[1] = hi[3] = lo[1] = lo[3] = 0;
-#pragma unroll
-      for (int j = 0; j < VC; ++j) {
-        uint4 vr[VT];
-        load_v(vr, ring, j, seen);
-        const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&vr[0]);
-        const uint32_t* w1 = reinterpret_cast<const uint32_t*>(&vr[1]);
-        const uint32_t* w2 = reinterpret_cast<const uint32_t*>(&vr[2]);
-        const uint32_t* w3 = reinterpret_cast<const uint32_t*>(&vr[3]);
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const uint32_t sel = e & 1 ? 0x7632 : 0x5410;
-          const uint32_t b0 = __byte_perm(w0[e / 2], w1[e / 2], sel), b1 = __byte_perm(w2[e / 2], w3[e / 2], sel);
-          float c[4] = {o[j][e][0], o[j][e][1], WIDE ? o[j][e][WIDE ? 2 : 0] : 0.f, WIDE ? o[j][e][WIDE ? 3 : 0] : 0.f};
-          Mma16<T>::run(c, hi[0], hi[1], hi[2], hi[3], b0, b1);
-          Mma16<T>::run(c, lo[0], lo[1], lo[2], lo[3], b0, b1);
-          o[j][e][0] = c[0], o[j][e][1] = c[1];
-          if constexpr (WIDE) o[j][e][2] = c[2], o[j][e][3] = c[3];
-        }
+      for (int x = 0; x < (WIDE ? 2 : 1); ++x) {
+        const float a = sc[n][2 * x], b = sc[n][2 * x + 1];
+        const uint32_t h = Mma16<T>::pack(a, b);
+        hi[2 * n + x] = h;
+        lo[2 * n + x] = Mma16<T>::pack(a - Mma16<T>::low(h), b - Mma16<T>::high(h));
       }
-    } else {
-      const float a[4] = {sc[0][0], WIDE ? sc[0][2] : 0.f, sc[0][1], WIDE ? sc[0][3] : 0.f};
+    if constexpr (!WIDE) hi[1] = hi[3] = lo[1] = lo[3] = 0;
 #pragma unroll
-      for (int j = 0; j < VC; ++j) {
-        uint4 vr[VT];
-        load_v(vr, ring, j, seen);
-        const float* w0 = reinterpret_cast<const float*>(&vr[0]);
-        const float* w1 = reinterpret_cast<const float*>(&vr[1]);
+    for (int j = 0; j < VC; ++j) {
+      uint4 vr[VT];
+      load_v(vr, ring, j, seen);
+      const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&vr[0]);
+      const uint32_t* w1 = reinterpret_cast<const uint32_t*>(&vr[1]);
+      const uint32_t* w2 = reinterpret_cast<const uint32_t*>(&vr[2]);
+      const uint32_t* w3 = reinterpret_cast<const uint32_t*>(&vr[3]);
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          float c[4] = {o[j][e][0], o[j][e][1], WIDE ? o[j][e][WIDE ? 2 : 0] : 0.f, WIDE ? o[j][e][WIDE ? 3 : 0] : 0.f};
-          mma_3xtf32(c, a, w0[e], w1[e]);
-          o[j][e][0] = c[0], o[j][e][1] = c[1];
-          if constexpr (WIDE) o[j][e][2] = c[2], o[j][e][3] = c[3];
-        }
+      for (int e = 0; e < E; ++e) {
+        const uint32_t sel = e & 1 ? 0x7632 : 0x5410;
+        const uint32_t b0 = __byte_perm(w0[e / 2], w1[e / 2], sel), b1 = __byte_perm(w2[e / 2], w3[e / 2], sel);
+        float c[4] = {o[j][e][0], o[j][e][1], WIDE ? o[j][e][WIDE ? 2 : 0] : 0.f, WIDE ? o[j][e][WIDE ? 3 : 0] : 0.f};
+        Mma16<T>::run(c, hi[0], hi[1], hi[2], hi[3], b0, b1);
+        Mma16<T>::run(c, lo[0], lo[1], lo[2], lo[3], b0, b1);
+        o[j][e][0] = c[0], o[j][e][1] = c[1];
+        if constexpr (WIDE) o[j][e][2] = c[2], o[j][e][3] = c[3];
       }
     }
   }
 
-  // With a mask the scores stay in natural units: a mask of the type's lowest value times log2(e) would leave its range.
-  static OSLO_DEVINL float score(const PagedAttnParams& p, float s, float add) {
-    return MASK ? fmaf(s, p.scale, add) : s * (p.scale * kLog2e);
+  OSLO_DEVINL void join(T* ring, float* ml) {
+    float* buf = reinterpret_cast<float*>(ring);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, quad = lane & 3;
+    l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
+    l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+    if (quad == 0) {
+      ml[warp * RT + r] = m0;
+      if constexpr (WIDE) ml[warp * RT + 8 + r] = m1;
+    }
+    __syncthreads();
+    float top0 = -INFINITY, top1 = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      top0 = fmaxf(top0, ml[w * RT + r]);
+      if constexpr (WIDE) top1 = fmaxf(top1, ml[w * RT + 8 + r]);
+    }
+    const float f0 = Math::weight(m0, top0), f1 = WIDE ? Math::weight(m1, top1) : 0.f;
+    if (quad == 0) {
+      ml[WARPS * RT + warp * RT + r] = l0 * f0;
+      if constexpr (WIDE) ml[WARPS * RT + warp * RT + 8 + r] = l1 * f1;
+    }
+#pragma unroll
+    for (int j = 0; j < VC; ++j)
+#pragma unroll
+      for (int x = 0; x < (WIDE ? 4 : 2); ++x) {
+        float* dst = buf + (r + (x >> 1) * 8) * ROW + j * 8 * E + (quad * 2 + (x & 1)) * E;
+        const float f = x >> 1 ? f1 : f0;
+#pragma unroll
+        for (int e = 0; e < E; e += 4)
+          *reinterpret_cast<float4*>(dst + e) = make_float4(o[j][e][x] * f, o[j][e + 1][x] * f, o[j][e + 2][x] * f, o[j][e + 3][x] * f);
+      }
+    __syncthreads();
   }
-  // exp(x - m); m = -inf: nothing was seen yet
-  static OSLO_DEVINL float weight(float x, float m) {
-    const float mm = m == -INFINITY ? 0.f : m;
-    return ex2(MASK ? (x - mm) * kLog2e : x - mm);
+};
+
+// 32-bit inputs, on the FMA units: tensor cores would round them to 10 bits, and splitting each into three products was both
+// less exact (2e-6 against 7e-7 for 32-bit sums at 256 dims) and slower.  Lane (r, q) multiplies its quarter of key r with every
+// query row; a reduce-scatter leaves a quarter of the rows' scores with each of the four lanes.  For the output a lane owns four
+// dims (eight of 256) and walks over the tile's tokens; the weights come from shared memory.
+template <int DP, bool WIDE, bool MASK>
+struct AttnWarp<float, DP, WIDE, MASK> {
+  using Math = AttnMath<MASK>;
+  static constexpr int E = 4;
+  static constexpr int TT = 8;
+  static constexpr int RT = WIDE ? 16 : 8;
+  static constexpr int OWN = RT / 4;  // rows whose scores a lane holds
+  static constexpr int ROW = DP + 4;
+  static constexpr int WARPS = 4;
+  static constexpr int PITCH = DP + 16;  // eight lanes of a key load then touch all banks
+  static constexpr int BLOCKS = DP == 64 ? 3 : DP == 128 ? 2 : 1;
+  static constexpr int KC = DP / 16;              // loads per key and lane
+  static constexpr int VC = DP < 128 ? 1 : DP / 128;  // loads per value and lane
+  static constexpr int HALVES = DP == 64 ? 2 : 1;  // 16 lanes cover 64 dims: the two halves of the warp take alternate tokens
+  static constexpr int WEIGHTS = RT * TT + RT;     // of a warp: weights [RT][TT], then factors [RT]
+  static constexpr int SCRATCH = RT * DP + WARPS * WEIGHTS;  // the block's queries, then each warp's weights
+
+  float4 o[RT][VC];
+  float m[OWN], l[OWN];
+  int rows;
+
+  static OSLO_DEVINL int own_row(int i) {
+    const int quad = threadIdx.x & 3;
+    return (quad & 1) * (RT / 2) + (quad >> 1) * (RT / 4) + i;
+  }
+  OSLO_DEVINL void load_q(const PagedAttnParams& p, const float* q, int row0, float* scratch) {
+    rows = min(RT, p.group - row0);
+    for (int x = threadIdx.x; x < rows * (DP / 4); x += 32 * WARPS) {
+      const int row = x / (DP / 4), dim = x % (DP / 4) * 4;
+      reinterpret_cast<uint4*>(scratch)[x] = dim < p.d ? ldg16(q + (row0 + row) * p.q_sh + dim) : make_uint4(0, 0, 0, 0);
+    }
+    __syncthreads();
+  }
+  OSLO_DEVINL void clear() {
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) m[i] = -INFINITY, l[i] = 0.f;
+#pragma unroll
+    for (int g = 0; g < RT; ++g)
+#pragma unroll
+      for (int j = 0; j < VC; ++j) o[g][j] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+
+  OSLO_DEVINL void tile(const PagedAttnParams& p, const float* ring, int token, int limit, const float* mask, float* scratch) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, quad = lane & 3;
+    float* const weights = scratch + RT * DP + warp * WEIGHTS;
+    float* const factors = weights + RT * TT;
+    bool seen = token + r < limit;
+    float add = 0.f;
+    if constexpr (MASK) {
+      if (seen) add = mask[token + r];
+      seen = seen && add != -INFINITY;
+    }
+    const unsigned visible = __ballot_sync(0xffffffffu, seen);  // token t: bit 4 t
+    float part[RT];
+#pragma unroll
+    for (int g = 0; g < RT; ++g) part[g] = 0.f;
+#pragma unroll
+    for (int c0 = 0; c0 < KC; c0 += 4) {
+      float4 k[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) k[c] = *reinterpret_cast<const float4*>(ring + r * PITCH + (c0 + c) * 16 + quad * 4);
+#pragma unroll
+      for (int g = 0; g < RT; ++g) {
+        if (g >= rows) break;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float4 q = *reinterpret_cast<const float4*>(scratch + g * DP + (c0 + c) * 16 + quad * 4);
+          part[g] = fmaf(q.x, k[c].x, fmaf(q.y, k[c].y, fmaf(q.z, k[c].z, fmaf(q.w, k[c].w, part[g]))));
+        }
+      }
+    }
+    // of each pair of lanes one goes on with the first half of the rows, the other with the second
+#pragma unroll
+    for (int i = 0; i < RT / 2; ++i) {
+      const bool up = quad & 1;
+      const float keep = up ? part[i + RT / 2] : part[i], give = up ? part[i] : part[i + RT / 2];
+      part[i] = keep + __shfl_xor_sync(0xffffffffu, give, 1);
+    }
+#pragma unroll
+    for (int i = 0; i < RT / 4; ++i) {
+      const bool up = quad & 2;
+      const float keep = up ? part[i + RT / 4] : part[i], give = up ? part[i] : part[i + RT / 4];
+      part[i] = keep + __shfl_xor_sync(0xffffffffu, give, 2);
+    }
+    float top[OWN];
+    bool higher = false;
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) {
+      part[i] = seen ? Math::score(p, part[i], add) : -INFINITY;
+      top[i] = part[i];
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], x));
+      higher = higher || top[i] > m[i];
+    }
+    const bool rescale = __any_sync(0xffffffffu, higher);
+    if (rescale) {
+#pragma unroll
+      for (int i = 0; i < OWN; ++i) {
+        const float n = fmaxf(m[i], top[i]), f = Math::weight(m[i], n);
+        m[i] = n, l[i] *= f;
+        if (r == 0) factors[own_row(i)] = f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) {
+      const float w = Math::weight(part[i], m[i]);
+      l[i] += w;
+      // tokens of one half of the warp lie side by side
+      weights[own_row(i) * TT + (HALVES == 2 ? (r & 1) * 4 + (r >> 1) : r)] = w;
+    }
+    __syncwarp();
+    if (rescale) {
+#pragma unroll
+      for (int g = 0; g < RT; ++g) {
+        if (g >= rows) break;
+        const float f = factors[g];
+#pragma unroll
+        for (int j = 0; j < VC; ++j) o[g][j].x *= f, o[g][j].y *= f, o[g][j].z *= f, o[g][j].w *= f;
+      }
+    }
+    constexpr int N = TT / HALVES;  // tokens of a lane
+    const int half = HALVES == 2 ? lane >> 4 : 0, column = (HALVES == 2 ? lane & 15 : lane) * 4;
+#pragma unroll
+    for (int j = 0; j < VC; ++j)
+#pragma unroll
+      for (int t0 = 0; t0 < N; t0 += 4) {
+        float4 v[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const int at = HALVES == 2 ? 2 * (t0 + t) + half : t0 + t;
+          v[t] = *reinterpret_cast<const float4*>(ring + TT * PITCH + at * PITCH + j * 128 + column);
+          if constexpr (MASK) {  // a masked token may hold anything: its values do not enter the product
+            if (!((visible >> (4 * at)) & 1)) v[t] = make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+        }
+#pragma unroll
+        for (int g = 0; g < RT; ++g) {
+          if (g >= rows) break;
+          const float4 w = *reinterpret_cast<const float4*>(weights + g * TT + half * 4 + t0);
+          float4& y = o[g][j];
+          y.x = fmaf(w.x, v[0].x, fmaf(w.y, v[1].x, fmaf(w.z, v[2].x, fmaf(w.w, v[3].x, y.x))));
+          y.y = fmaf(w.x, v[0].y, fmaf(w.y, v[1].y, fmaf(w.z, v[2].y, fmaf(w.w, v[3].y, y.y))));
+          y.z = fmaf(w.x, v[0].z, fmaf(w.y, v[1].z, fmaf(w.z, v[2].z, fmaf(w.w, v[3].z, y.z))));
+          y.w = fmaf(w.x, v[0].w, fmaf(w.y, v[1].w, fmaf(w.z, v[2].w, fmaf(w.w, v[3].w, y.w))));
+        }
+      }
+  }
+
+  OSLO_DEVINL void join(float* buf, float* ml) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2;
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) {
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], x);
+      if (r == 0) ml[warp * RT + own_row(i)] = m[i];
+    }
+    __syncthreads();
+    const auto factor = [&](int g) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) top = fmaxf(top, ml[w * RT + g]);
+      return Math::weight(ml[warp * RT + g], top);
+    };
+#pragma unroll
+    for (int i = 0; i < OWN; ++i)
+      if (r == 0) ml[WARPS * RT + warp * RT + own_row(i)] = l[i] * factor(own_row(i));
+#pragma unroll
+    for (int g = 0; g < RT; ++g) {
+      if (g >= rows) break;
+      const float f = factor(g);
+#pragma unroll
+      for (int j = 0; j < VC; ++j) {
+        float4 y = o[g][j];
+        if constexpr (HALVES == 2) {
+          y.x += __shfl_xor_sync(0xffffffffu, y.x, 16), y.y += __shfl_xor_sync(0xffffffffu, y.y, 16);
+          y.z += __shfl_xor_sync(0xffffffffu, y.z, 16), y.w += __shfl_xor_sync(0xffffffffu, y.w, 16);
+        }
+        if (HALVES == 1 || lane < 16)
+          *reinterpret_cast<float4*>(buf + g * ROW + j * 128 + lane * 4) = make_float4(y.x * f, y.y * f, y.z * f, y.w * f);
+      }
+    }
+    __syncthreads();
+  }
+};
+
+// The block's side of it: rings of tiles in shared memory, and the walk over a segment's tokens.
+template <typename T, int DP, bool WIDE, bool MASK>
+struct PagedAttn : AttnWarp<T, DP, WIDE, MASK> {
+  using W = AttnWarp<T, DP, WIDE, MASK>;
+  using W::BLOCKS, W::E, W::PITCH, W::ROW, W::RT, W::SCRATCH, W::TT, W::WARPS;
+  static constexpr int TILE = TT * PITCH * 2;  // keys, then values
+  static constexpr int STAGES = DP == 64 ? 3 : 2;
+  static constexpr size_t kRing = sizeof(T) * TILE * STAGES;  // of one warp; the joining buffer takes its place at the end
+  static constexpr size_t kSmem = kRing * WARPS + sizeof(float) * (2 * WARPS * RT + SCRATCH);
+  static_assert(kRing >= sizeof(float) * RT * ROW, "a warp's part of the joining buffer fits its ring");
+  static_assert((kSmem + 1024) * BLOCKS <= 228 * 1024, "shared memory of the blocks of an SM");
+
+  static OSLO_DEVINL float weight(float x, float m) { return W::Math::weight(x, m); }
+
+  // Starts the copy of one tile, `rows` of whose tokens are seen, into the ring.
+  static OSLO_DEVINL void fill(const PagedAttnParams& p, T* ring, const T* k, const T* v, int rows) {
+    constexpr int CHUNKS = DP / E;
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const T* src = half ? v : k;
+      T* dst = ring + half * TT * PITCH;
+#pragma unroll
+      for (int i = 0; i < TT * CHUNKS / 32; ++i) {
+        const int row = (i * 32 + lane) / CHUNKS, c = (i * 32 + lane) % CHUNKS;
+        const bool valid = row < rows && c * E < p.d;
+        copy16(dst + row * PITCH + c * E, valid ? src + row * p.d + c * E : src, valid);
+      }
+    }
   }
 
   // Row maxima of the four warps, then their row sums.
@@ -382,58 +577,22 @@ struct PagedAttn {
     int t = ahead;
 #pragma unroll
     for (int x = 0; x < STAGES; ++x) advance(x);
-    load_q(p, static_cast<const T*>(p.q) + b * p.q_sb + i * p.q_ss + static_cast<long long>(h) * p.group * p.q_sh, row0);
-    clear();
+    float* const scratch = ml_of(smem) + 2 * WARPS * RT;
+    this->load_q(p, static_cast<const T*>(p.q) + b * p.q_sb + i * p.q_ss + static_cast<long long>(h) * p.group * p.q_sh, row0, scratch);
+    this->clear();
     for (int slot = 0; t < end; t += STEP) {
       copy_wait<STAGES - 1>();
       __syncwarp();
-      tile(p, ring + slot * TILE, t, (missing >> slot) & 1 ? 0 : limit, mask);
+      this->tile(p, ring + slot * TILE, t, (missing >> slot) & 1 ? 0 : limit, mask, scratch);
       __syncwarp();
       advance(slot);
       slot = slot + 1 == STAGES ? 0 : slot + 1;
     }
     copy_wait<0>();
     __syncwarp();
-    join(ring, ml_of(smem));
+    this->join(ring, ml_of(smem));  // then every thread may read row sums, maxima and the warps' outputs, scaled to one maximum
   }
 
-  // Joins the warps' sums.  Afterwards every thread may read row sums / maxima (ml) and the warps' outputs, scaled to the same
-  // maximum, at the start of their rings.
-  OSLO_DEVINL void join(T* ring, float* ml) {
-    float* buf = reinterpret_cast<float*>(ring);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, quad = lane & 3;
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-    l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-    if (quad == 0) {
-      ml[warp * RT + r] = m0;
-      if constexpr (WIDE) ml[warp * RT + 8 + r] = m1;
-    }
-    __syncthreads();
-    float top0 = -INFINITY, top1 = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      top0 = fmaxf(top0, ml[w * RT + r]);
-      if constexpr (WIDE) top1 = fmaxf(top1, ml[w * RT + 8 + r]);
-    }
-    const float f0 = weight(m0, top0), f1 = WIDE ? weight(m1, top1) : 0.f;
-    if (quad == 0) {
-      ml[WARPS * RT + warp * RT + r] = l0 * f0;
-      if constexpr (WIDE) ml[WARPS * RT + warp * RT + 8 + r] = l1 * f1;
-    }
-#pragma unroll
-    for (int j = 0; j < VC; ++j)
-#pragma unroll
-      for (int x = 0; x < (WIDE ? 4 : 2); ++x) {
-        float* dst = buf + (r + (x >> 1) * 8) * ROW + j * 8 * E + (quad * 2 + (x & 1)) * E;
-        const float f = x >> 1 ? f1 : f0;
-#pragma unroll
-        for (int e = 0; e < E; e += 4)
-          *reinterpret_cast<float4*>(dst + e) = make_float4(o[j][e][x] * f, o[j][e + 1][x] * f, o[j][e + 2][x] * f, o[j][e + 3][x] * f);
-      }
-    __syncthreads();
-  }
 };
 
 // The tokens a query sees, as far as the table (and the mask) reach.
