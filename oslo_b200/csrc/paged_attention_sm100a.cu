@@ -45,8 +45,26 @@ struct PagedAttnParams {
   float* part_o;   // [grid, 2, RT, DP] unnormalised outputs of shared segments: 0 = begun by an earlier block, 1 = begun here
   float2* part_ml;  // [grid, 2, RT] their maxima and sums
   int4* shared_seg;  // [grid] of the segment begun earlier that ends here: (first block, query, key head, first row); x < 0: none
-  int b, s, hkv, group, d, page_size, max_pages, num_pages, mask_len, row_tiles;
+  int b, s, hkv, group, d, page_size, max_pages, num_pages, mask_len;
+  int queries, rows, row_tiles;  // groups of query rows of a sequence; rows of a group and key head, and how many blocks' worth
   float scale;
+};
+
+// Rows of a segment.  The query tokens of a sequence that share a mask form one group: its row r is query head r % group of token
+// first + r / group, so one pass over the keys serves several proposed tokens.  Tokens with masks of their own are groups.
+struct Segment {
+  int b, h, first, row0, rows;  // sequence, key head, first query token of the group, first row, rows in this block
+  int length;                   // tokens that query token i of the sequence sees: length + i
+  OSLO_DEVINL Segment(const PagedAttnParams& p, int query, int head, int row, int most) {
+    b = query / p.queries, h = head, first = query - b * p.queries, row0 = row, rows = min(most, p.rows - row);
+    length = 0;
+  }
+  OSLO_DEVINL int token(const PagedAttnParams& p, int r) const { return first + (row0 + r) / p.group; }
+  OSLO_DEVINL int q_head(const PagedAttnParams& p, int r) const { return h * p.group + (row0 + r) % p.group; }
+  OSLO_DEVINL long long q_at(const PagedAttnParams& p, int r) const { return b * p.q_sb + token(p, r) * p.q_ss + q_head(p, r) * p.q_sh; }
+  OSLO_DEVINL long long out_at(const PagedAttnParams& p, int r) const {
+    return ((static_cast<long long>(b) * p.s + token(p, r)) * p.hkv * p.group + q_head(p, r)) * p.d;
+  }
 };
 
 // Starting a segment costs a block about as long as two units: each segment has that many units without tokens at its front.
@@ -81,7 +99,7 @@ struct Mma16;  // D[16 x 8] += A[16 x 16] B[16 x 8], 16-bit operands
 template <>
 struct Mma16<__nv_bfloat16> {
   static OSLO_DEVINL void run(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   }
   static OSLO_DEVINL uint32_t pack(float lo, float hi) {
@@ -94,7 +112,7 @@ struct Mma16<__nv_bfloat16> {
 template <>
 struct Mma16<__half> {
   static OSLO_DEVINL void run(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   }
   static OSLO_DEVINL uint32_t pack(float lo, float hi) {
@@ -146,22 +164,29 @@ struct AttnWarp {
   static constexpr int ROW = DP + 4;        // padded row of the joining buffer
   static constexpr int WARPS = 4;
   static constexpr int PITCH = DP + E;  // elements between two rows of a tile in the ring
-  static constexpr int BLOCKS = DP == 64 ? 4 : DP == 128 ? 3 : 1;  // blocks an SM should hold; the ring's size is chosen for it
+  // Blocks an SM should hold; the ring's size is chosen for it.  128 dims: two blocks with three tiles a warp (one sequence of
+  // 131071 tokens 100 us, ragged batch 30 us) against three blocks with two (105 and 32 us) and one with four (120 and 42 us).
+  // 64 dims: three blocks with three tiles (64 x 4000 tokens, 12 heads: 116 us) against four (124 us) and two with five (137 us).
+  static constexpr int BLOCKS = DP == 64 ? 3 : DP == 128 ? 2 : 1;
   static constexpr int SCRATCH = 0;  // floats of shared memory of the block, beside the rings
 
   uint4 q0[KC], q1[WIDE ? KC : 1];
-  float o[VC][E][WIDE ? 4 : 2];
+  float o[VC][E][4];  // rows r and r + 8; with up to 8 rows the second pair holds what the remainders of the weights add
   float m0, m1, l0, l1;
+  int end0, end1, least, most;  // tokens that rows r and r + 8 see; of all rows, the least and the most
 
-  OSLO_DEVINL void load_q(const PagedAttnParams& p, const T* q, int row0, float*) {
+  OSLO_DEVINL void load_q(const PagedAttnParams& p, const Segment& seg, float*) {
     const int r = (threadIdx.x & 31) >> 2, quad = threadIdx.x & 3;
+    const T* q = static_cast<const T*>(p.q);
+    const long long a0 = r < seg.rows ? seg.q_at(p, r) : 0, a1 = WIDE && r + 8 < seg.rows ? seg.q_at(p, r + 8) : 0;
 #pragma unroll
     for (int c = 0; c < KC; ++c) {
       const int dim = c * 4 * E + quad * E;
-      q0[c] = row0 + r < p.group && dim < p.d ? ldg16(q + (row0 + r) * p.q_sh + dim) : make_uint4(0, 0, 0, 0);
-      if constexpr (WIDE)
-        q1[c] = row0 + r + 8 < p.group && dim < p.d ? ldg16(q + (row0 + r + 8) * p.q_sh + dim) : make_uint4(0, 0, 0, 0);
+      q0[c] = r < seg.rows && dim < p.d ? ldg16(q + a0 + dim) : make_uint4(0, 0, 0, 0);
+      if constexpr (WIDE) q1[c] = r + 8 < seg.rows && dim < p.d ? ldg16(q + a1 + dim) : make_uint4(0, 0, 0, 0);
     }
+    end0 = seg.length + seg.token(p, min(r, seg.rows - 1)), end1 = seg.length + seg.token(p, min(r + 8, seg.rows - 1));
+    least = seg.length + seg.token(p, 0), most = seg.length + seg.token(p, seg.rows - 1);
   }
   OSLO_DEVINL void clear() {
     m0 = m1 = -INFINITY;
@@ -171,19 +196,26 @@ struct AttnWarp {
 #pragma unroll
       for (int e = 0; e < E; ++e)
 #pragma unroll
-        for (int x = 0; x < (WIDE ? 4 : 2); ++x) o[j][e][x] = 0.f;
+        for (int x = 0; x < 4; ++x) o[j][e][x] = 0.f;
   }
 
-  // Block j of the values of this lane's tokens.
-  static OSLO_DEVINL void load_v(uint4 (&vr)[VT], const T* ring, int j, const bool (&seen)[NT][2]) {
+  // Block j of the values of this lane's tokens; zeros for those that are masked or, where `end` is given, at or past it.
+  template <bool END>
+  static OSLO_DEVINL void load_v(uint4 (&vr)[VT], const T* ring, int j, const bool (&seen)[NT][2], int end) {
     const int lane = threadIdx.x & 31, r = lane >> 2, quad = lane & 3;
 #pragma unroll
     for (int t = 0; t < VT; ++t) {
       vr[t] = *reinterpret_cast<const uint4*>(ring + TT * PITCH + ((t >> 1) * 8 + quad * 2 + (t & 1)) * PITCH + j * 8 * E + r * E);
-      if constexpr (MASK) {  // a masked token may hold anything: its values do not enter the product
-        if (!seen[t >> 1][t & 1]) vr[t] = make_uint4(0, 0, 0, 0);
+      if constexpr (MASK || END) {  // a token that is not seen may hold anything: its values do not enter the product
+        if (!seen[t >> 1][t & 1] || (END && (t >> 1) * 8 + quad * 2 + (t & 1) >= end)) vr[t] = make_uint4(0, 0, 0, 0);
       }
     }
+  }
+  // 16-bit B operands of column e from the values of the lane's four tokens
+  static OSLO_DEVINL void columns(const uint4 (&vr)[VT], int e, uint32_t& b0, uint32_t& b1) {
+    const uint32_t sel = e & 1 ? 0x7632 : 0x5410;
+    b0 = __byte_perm(reinterpret_cast<const uint32_t*>(&vr[0])[e / 2], reinterpret_cast<const uint32_t*>(&vr[1])[e / 2], sel);
+    b1 = __byte_perm(reinterpret_cast<const uint32_t*>(&vr[2])[e / 2], reinterpret_cast<const uint32_t*>(&vr[3])[e / 2], sel);
   }
 
   // One tile of the ring: its TT tokens start at `token`; tokens at or past `limit` are not seen.
@@ -207,23 +239,27 @@ struct AttnWarp {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+      float odd[4] = {0.f, 0.f, 0.f, 0.f};  // two chains of products, each half as long
 #pragma unroll
       for (int c = 0; c < KC; ++c) {
         const uint4 qa = q0[c], qb = WIDE ? q1[WIDE ? c : 0] : make_uint4(0, 0, 0, 0);
         const uint4 kr = *reinterpret_cast<const uint4*>(ring + (n * 8 + r) * PITCH + c * 4 * E + quad * E);
         Mma16<T>::run(sc[n], qa.x, qb.x, qa.y, qb.y, kr.x, kr.y);
-        Mma16<T>::run(sc[n], qa.z, qb.z, qa.w, qb.w, kr.z, kr.w);
+        Mma16<T>::run(odd, qa.z, qb.z, qa.w, qb.w, kr.z, kr.w);
       }
+#pragma unroll
+      for (int x = 0; x < 4; ++x) sc[n][x] += odd[x];
     }
     float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        sc[n][x] = seen[n][x] ? Math::score(p, sc[n][x], add[n][x]) : -INFINITY;
+        const int t = token + n * 8 + quad * 2 + x;
+        sc[n][x] = seen[n][x] && t < end0 ? Math::score(p, sc[n][x], add[n][x]) : -INFINITY;
         t0 = fmaxf(t0, sc[n][x]);
         if constexpr (WIDE) {
-          sc[n][2 + x] = seen[n][x] ? Math::score(p, sc[n][2 + x], add[n][x]) : -INFINITY;
+          sc[n][2 + x] = seen[n][x] && t < end1 ? Math::score(p, sc[n][2 + x], add[n][x]) : -INFINITY;
           t1 = fmaxf(t1, sc[n][2 + x]);
         }
       }
@@ -243,7 +279,7 @@ struct AttnWarp {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
           o[j][e][0] *= f0, o[j][e][1] *= f0;
-          if constexpr (WIDE) o[j][e][2] *= f1, o[j][e][3] *= f1;
+          o[j][e][2] *= WIDE ? f1 : f0, o[j][e][3] *= WIDE ? f1 : f0;
         }
     }
 #pragma unroll
@@ -267,26 +303,42 @@ struct AttnWarp {
         hi[2 * n + x] = h;
         lo[2 * n + x] = Mma16<T>::pack(a - Mma16<T>::low(h), b - Mma16<T>::high(h));
       }
-    if constexpr (!WIDE) hi[1] = hi[3] = lo[1] = lo[3] = 0;
+    if constexpr (!WIDE) hi[1] = lo[0], hi[3] = lo[2];  // the remainders take the empty rows
+    if (least == most || token + TT <= least) {
 #pragma unroll
-    for (int j = 0; j < VC; ++j) {
-      uint4 vr[VT];
-      load_v(vr, ring, j, seen);
-      const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&vr[0]);
-      const uint32_t* w1 = reinterpret_cast<const uint32_t*>(&vr[1]);
-      const uint32_t* w2 = reinterpret_cast<const uint32_t*>(&vr[2]);
-      const uint32_t* w3 = reinterpret_cast<const uint32_t*>(&vr[3]);
+      for (int j = 0; j < VC; ++j) {
+        uint4 vr[VT];
+        load_v<false>(vr, ring, j, seen, 0);
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const uint32_t sel = e & 1 ? 0x7632 : 0x5410;
-        const uint32_t b0 = __byte_perm(w0[e / 2], w1[e / 2], sel), b1 = __byte_perm(w2[e / 2], w3[e / 2], sel);
-        float c[4] = {o[j][e][0], o[j][e][1], WIDE ? o[j][e][WIDE ? 2 : 0] : 0.f, WIDE ? o[j][e][WIDE ? 3 : 0] : 0.f};
-        Mma16<T>::run(c, hi[0], hi[1], hi[2], hi[3], b0, b1);
-        Mma16<T>::run(c, lo[0], lo[1], lo[2], lo[3], b0, b1);
-        o[j][e][0] = c[0], o[j][e][1] = c[1];
-        if constexpr (WIDE) o[j][e][2] = c[2], o[j][e][3] = c[3];
+        for (int part = 0; part < (WIDE ? 2 : 1); ++part)  // all high parts, then all remainders: neighbours do not wait for each other
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            uint32_t b0, b1;
+            columns(vr, e, b0, b1);
+            const uint32_t(&a)[4] = part ? lo : hi;
+            Mma16<T>::run(o[j][e], a[0], a[1], a[2], a[3], b0, b1);
+          }
       }
+      return;
     }
+    // Some of the tile's tokens are seen by some rows only; what they hold must not reach the others, not even times zero.  Each
+    // query token of the group gets a product of its own, over the tokens that it sees.
+    for (int end = least; end <= most; ++end)
+#pragma unroll
+      for (int j = 0; j < VC; ++j) {
+        uint4 vr[VT];
+        load_v<true>(vr, ring, j, seen, end - token);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          uint32_t b0, b1;
+          columns(vr, e, b0, b1);
+          float c[4] = {0.f, 0.f, 0.f, 0.f};
+          Mma16<T>::run(c, hi[0], hi[1], hi[2], hi[3], b0, b1);
+          if constexpr (WIDE) Mma16<T>::run(c, lo[0], lo[1], lo[2], lo[3], b0, b1);
+          if (end0 == end) o[j][e][0] += c[0], o[j][e][1] += c[1];
+          if ((WIDE ? end1 : end0) == end) o[j][e][2] += c[2], o[j][e][3] += c[3];
+        }
+      }
   }
 
   OSLO_DEVINL void join(T* ring, float* ml) {
@@ -318,9 +370,9 @@ struct AttnWarp {
       for (int x = 0; x < (WIDE ? 4 : 2); ++x) {
         float* dst = buf + (r + (x >> 1) * 8) * ROW + j * 8 * E + (quad * 2 + (x & 1)) * E;
         const float f = x >> 1 ? f1 : f0;
+        const auto sum = [&](int e) { return (WIDE ? o[j][e][x] : o[j][e][x] + o[j][e][(x + 2) & 3]) * f; };
 #pragma unroll
-        for (int e = 0; e < E; e += 4)
-          *reinterpret_cast<float4*>(dst + e) = make_float4(o[j][e][x] * f, o[j][e + 1][x] * f, o[j][e + 2][x] * f, o[j][e + 3][x] * f);
+        for (int e = 0; e < E; e += 4) *reinterpret_cast<float4*>(dst + e) = make_float4(sum(e), sum(e + 1), sum(e + 2), sum(e + 3));
       }
     __syncthreads();
   }
@@ -349,18 +401,23 @@ struct AttnWarp<float, DP, WIDE, MASK> {
 
   float4 o[RT][VC];
   float m[OWN], l[OWN];
-  int rows;
+  int end[OWN];  // tokens that the lane's rows see
+  int rows, first, group, least, most;  // row g sees least + (first + g) / group tokens
 
   static OSLO_DEVINL int own_row(int i) {
     const int quad = threadIdx.x & 3;
     return (quad & 1) * (RT / 2) + (quad >> 1) * (RT / 4) + i;
   }
-  OSLO_DEVINL void load_q(const PagedAttnParams& p, const float* q, int row0, float* scratch) {
-    rows = min(RT, p.group - row0);
+  OSLO_DEVINL void load_q(const PagedAttnParams& p, const Segment& seg, float* scratch) {
+    rows = seg.rows;
     for (int x = threadIdx.x; x < rows * (DP / 4); x += 32 * WARPS) {
       const int row = x / (DP / 4), dim = x % (DP / 4) * 4;
-      reinterpret_cast<uint4*>(scratch)[x] = dim < p.d ? ldg16(q + (row0 + row) * p.q_sh + dim) : make_uint4(0, 0, 0, 0);
+      reinterpret_cast<uint4*>(scratch)[x] = dim < p.d ? ldg16(static_cast<const float*>(p.q) + seg.q_at(p, row) + dim) : make_uint4(0, 0, 0, 0);
     }
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) end[i] = seg.length + seg.token(p, min(own_row(i), rows - 1));
+    first = seg.row0 % p.group, group = p.group;
+    least = seg.length + seg.token(p, 0), most = seg.length + seg.token(p, rows - 1);
     __syncthreads();
   }
   OSLO_DEVINL void clear() {
@@ -418,7 +475,7 @@ struct AttnWarp<float, DP, WIDE, MASK> {
     bool higher = false;
 #pragma unroll
     for (int i = 0; i < OWN; ++i) {
-      part[i] = seen ? Math::score(p, part[i], add) : -INFINITY;
+      part[i] = seen && token + r < end[i] ? Math::score(p, part[i], add) : -INFINITY;
       top[i] = part[i];
 #pragma unroll
       for (int x = 4; x < 32; x <<= 1) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], x));
@@ -452,6 +509,7 @@ struct AttnWarp<float, DP, WIDE, MASK> {
     }
     constexpr int N = TT / HALVES;  // tokens of a lane
     const int half = HALVES == 2 ? lane >> 4 : 0, column = (HALVES == 2 ? lane & 15 : lane) * 4;
+    const bool mixed = least != most && token + TT > least;
 #pragma unroll
     for (int j = 0; j < VC; ++j)
 #pragma unroll
@@ -464,6 +522,21 @@ struct AttnWarp<float, DP, WIDE, MASK> {
           if constexpr (MASK) {  // a masked token may hold anything: its values do not enter the product
             if (!((visible >> (4 * at)) & 1)) v[t] = make_float4(0.f, 0.f, 0.f, 0.f);
           }
+        }
+        if (mixed) {  // nor do those of a token that the row does not see
+#pragma unroll
+          for (int g = 0; g < RT; ++g) {
+            if (g >= rows) break;
+            const int sees = least + (first + g) / group - token;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+              if ((HALVES == 2 ? 2 * (t0 + t) + half : t0 + t) >= sees) continue;
+              const float w = weights[g * TT + half * 4 + t0 + t];
+              float4& y = o[g][j];
+              y.x = fmaf(w, v[t].x, y.x), y.y = fmaf(w, v[t].y, y.y), y.z = fmaf(w, v[t].z, y.z), y.w = fmaf(w, v[t].w, y.w);
+            }
+          }
+          continue;
         }
 #pragma unroll
         for (int g = 0; g < RT; ++g) {
@@ -521,7 +594,7 @@ struct PagedAttn : AttnWarp<T, DP, WIDE, MASK> {
   using W = AttnWarp<T, DP, WIDE, MASK>;
   using W::BLOCKS, W::E, W::PITCH, W::ROW, W::RT, W::SCRATCH, W::TT, W::WARPS;
   static constexpr int TILE = TT * PITCH * 2;  // keys, then values
-  static constexpr int STAGES = DP == 64 ? 3 : 2;
+  static constexpr int STAGES = DP == 64 || (DP == 128 && sizeof(T) == 2) ? 3 : 2;
   static constexpr size_t kRing = sizeof(T) * TILE * STAGES;  // of one warp; the joining buffer takes its place at the end
   static constexpr size_t kSmem = kRing * WARPS + sizeof(float) * (2 * WARPS * RT + SCRATCH);
   static_assert(kRing >= sizeof(float) * RT * ROW, "a warp's part of the joining buffer fits its ring");
@@ -550,11 +623,11 @@ struct PagedAttn : AttnWarp<T, DP, WIDE, MASK> {
   static OSLO_DEVINL float* ml_of(char* smem) { return reinterpret_cast<float*>(smem + kRing * WARPS); }
 
   // Attends over tokens [begin, end) of a segment with all warps of the block and joins them.
-  OSLO_DEVINL void walk(const PagedAttnParams& p, char* smem, int query, int h, int row0, int limit, int begin, int end) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int b = query / p.s, i = query - b * p.s;
-    const float* mask = MASK ? p.mask + b * p.m_sb + i * p.m_ss : nullptr;
-    const int* table = p.table + b * p.table_stride;
+  OSLO_DEVINL void walk(const PagedAttnParams& p, char* smem, Segment& seg, int limit, int begin, int end) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h = seg.h;
+    const float* mask = MASK ? p.mask + seg.b * p.m_sb + seg.first * p.m_ss : nullptr;
+    const int* table = p.table + seg.b * p.table_stride;
+    seg.length = p.lens[seg.b] - p.s + 1;
     T* ring = reinterpret_cast<T*>(smem + kRing * warp);
     const T* k = static_cast<const T*>(p.k) + h * p.k_head;
     const T* v = static_cast<const T*>(p.v) + h * p.v_head;
@@ -578,7 +651,7 @@ struct PagedAttn : AttnWarp<T, DP, WIDE, MASK> {
 #pragma unroll
     for (int x = 0; x < STAGES; ++x) advance(x);
     float* const scratch = ml_of(smem) + 2 * WARPS * RT;
-    this->load_q(p, static_cast<const T*>(p.q) + b * p.q_sb + i * p.q_ss + static_cast<long long>(h) * p.group * p.q_sh, row0, scratch);
+    this->load_q(p, seg, scratch);
     this->clear();
     for (int slot = 0; t < end; t += STEP) {
       copy_wait<STAGES - 1>();
@@ -595,11 +668,11 @@ struct PagedAttn : AttnWarp<T, DP, WIDE, MASK> {
 
 };
 
-// The tokens a query sees, as far as the table (and the mask) reach.
+// The tokens that a group's last query token sees, as far as the table (and the mask) reach.
 template <bool MASK>
 OSLO_DEVINL int query_limit(const PagedAttnParams& p, int query, bool report) {
-  const int b = query / p.s, i = query - b * p.s;
-  const long long limit = static_cast<long long>(p.lens[b]) - p.s + 1 + i;
+  const int b = query / p.queries;
+  const long long limit = static_cast<long long>(p.lens[b]) + (query - b * p.queries) - (p.queries - 1);
   const int cap = MASK ? min(p.mask_len, p.max_pages * p.page_size) : p.max_pages * p.page_size;
   if (limit > cap && report) atomicCAS(p.status, kStatusOk, kStatusPageRange);
   return static_cast<int>(min(max(limit, 0ll), static_cast<long long>(cap)));
@@ -635,7 +708,7 @@ __global__ void __launch_bounds__(128, PagedAttn<T, DP, WIDE, MASK>::BLOCKS) pag
 
   // This block's range of units: an exclusive prefix sum of the queries' units over the block's threads, each of which owns a
   // contiguous run of queries.  A query without tokens is one unit, so that its zeros are written.
-  const int queries = p.b * p.s, run = (queries + 127) / 128;
+  const int queries = p.b * p.queries, run = (queries + 127) / 128;
   const int first = min(queries, static_cast<int>(threadIdx.x) * run), last = min(queries, first + run);
   long long mine = 0;
   for (int i = first; i < last; ++i) mine += segment_units<UNIT>(query_limit<MASK>(p, i, false));
@@ -691,18 +764,18 @@ __global__ void __launch_bounds__(128, PagedAttn<T, DP, WIDE, MASK>::BLOCKS) pag
     const int h = seg / p.row_tiles, row0 = (seg - h * p.row_tiles) * A::RT;
 
     A acc;
-    acc.walk(p, reinterpret_cast<char*>(smem4), query, h, row0, limit, max(0, a - kSegmentUnits) * UNIT, min(limit, (e - kSegmentUnits) * UNIT));
+    Segment rows(p, query, h, row0, A::RT);
+    acc.walk(p, reinterpret_cast<char*>(smem4), rows, limit, max(0, a - kSegmentUnits) * UNIT, min(limit, (e - kSegmentUnits) * UNIT));
 
     const bool whole = a == 0 && e == n_units;
     const long long slot = static_cast<long long>(blockIdx.x) * 2 + (a == 0 ? 1 : 0);
-    T* out = static_cast<T*>(p.out) + (static_cast<long long>(query) * p.hkv + h) * p.group * p.d;
     for (int x = threadIdx.x; x < A::RT * (DP / 4); x += blockDim.x) {
       const int row = x / (DP / 4), dim = x % (DP / 4) * 4;
-      if (row0 + row >= p.group || dim >= p.d) continue;
+      if (row >= rows.rows || dim >= p.d) continue;
       float l, m;
       const float4 s = block_sum<A>(reinterpret_cast<const char*>(smem4), row, dim, l, m);
       if (whole) {
-        pa_store(out + (row0 + row) * p.d + dim, s, l);
+        pa_store(static_cast<T*>(p.out) + rows.out_at(p, row) + dim, s, l);
       } else {
         *reinterpret_cast<float4*>(p.part_o + (slot * A::RT + row) * DP + dim) = s;
         if (dim == 0) p.part_ml[slot * A::RT + row] = make_float2(m, l);
@@ -751,15 +824,16 @@ __global__ void __launch_bounds__(128, PagedAttn<T, DP, WIDE, MASK>::BLOCKS) pag
   const int limit = query_limit<MASK>(p, query, threadIdx.x == 0);
   const int units = (limit + UNIT - 1) / UNIT;
   A acc;
-  acc.walk(p, smem, query, h, row0, limit, units * rank / cluster * UNIT, min(limit, units * (rank + 1) / cluster * UNIT));
-  T* out = static_cast<T*>(p.out) + ((static_cast<long long>(query) * p.hkv + h) * p.group + row0) * p.d;
-  const int rows = min(A::RT, p.group - row0), quads = p.d / 4;
+  Segment part(p, query, h, row0, A::RT);
+  acc.walk(p, smem, part, limit, units * rank / cluster * UNIT, min(limit, units * (rank + 1) / cluster * UNIT));
+  T* out = static_cast<T*>(p.out);
+  const int rows = part.rows, quads = p.d / 4;
   if (cluster == 1) {
     for (int x = threadIdx.x; x < rows * quads; x += 128) {
       const int row = x / quads, dim = (x - row * quads) * 4;
       float l, m;
       const float4 s = block_sum<A>(smem, row, dim, l, m);
-      pa_store(out + row * p.d + dim, s, l);
+      pa_store(out + part.out_at(p, row) + dim, s, l);
     }
     return;
   }
@@ -792,7 +866,7 @@ __global__ void __launch_bounds__(128, PagedAttn<T, DP, WIDE, MASK>::BLOCKS) pag
         l += t[i].y * w;
         s.x += y[i].x * w, s.y += y[i].y * w, s.z += y[i].z * w, s.w += y[i].w * w;
       }
-    pa_store(out + row * p.d + dim, s, l);
+    pa_store(out + part.out_at(p, row) + dim, s, l);
   }
   cluster_barrier();  // a block's shared memory stays until all have read it
 }
@@ -813,7 +887,8 @@ __global__ void __launch_bounds__(32 * kJoinRows * kJoinWarps) paged_attention_j
   if (seg.x < 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, line = warp / kJoinWarps, piece = warp % kJoinWarps;
   const int row = blockIdx.x * kJoinRows + line;
-  const bool used = row < A::RT && seg.w + row < p.group;
+  const Segment rows(p, seg.y, seg.z, seg.w, A::RT);
+  const bool used = row < rows.rows;
   const int parts = used ? blockIdx.y - seg.x + 1 : 0;
   float m = -INFINITY, l = 0.f;
   float4 o[V];
@@ -847,7 +922,7 @@ __global__ void __launch_bounds__(32 * kJoinRows * kJoinWarps) paged_attention_j
   for (int i = 0; i < kJoinWarps; ++i) m = fmaxf(m, tops[line][i]);
 #pragma unroll
   for (int i = 0; i < kJoinWarps; ++i) w[i] = A::weight(tops[line][i], m), l += totals[line][i] * w[i];
-  T* out = static_cast<T*>(p.out) + ((static_cast<long long>(seg.y) * p.hkv + seg.z) * p.group + seg.w + row) * p.d;
+  T* out = static_cast<T*>(p.out) + rows.out_at(p, row);
   for (int x = lane; x * 4 < p.d; x += 32) {
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
@@ -864,8 +939,8 @@ struct PagedAttnPlan {
   int cluster, grid, resident;
   long long bytes;
 };
-// Tokens that a block of the one-launch form takes at most.
-constexpr int kClusterTokens = 1024;
+// Tokens that a block of the one-launch form takes at most (8 sequences of up to 4000 tokens: 20 us with 512, 26 us with 1024).
+constexpr int kClusterTokens = 512;
 
 template <typename T, int DP, bool WIDE, bool MASK>
 struct PagedAttnLaunch {
@@ -895,7 +970,7 @@ struct PagedAttnLaunch {
     PagedAttnPlan x{8, 0, resident(), 0};
     if (x.resident < 0) return x;
     const int most = MASK ? min(p.mask_len, p.max_pages * p.page_size) : p.max_pages * p.page_size;
-    const long long segments = static_cast<long long>(p.b) * p.s * p.hkv * p.row_tiles;
+    const long long segments = static_cast<long long>(p.b) * p.queries * p.hkv * p.row_tiles;
     while (x.cluster > 1 && (segments * x.cluster > x.resident || x.cluster * 32 > most)) x.cluster /= 2;
     if (segments <= x.resident && most <= static_cast<long long>(kClusterTokens) * x.cluster) return x;
     x.cluster = 0;
@@ -907,7 +982,7 @@ struct PagedAttnLaunch {
   static int launch(PagedAttnParams& p, const PagedAttnPlan& plan, void* ws, cudaStream_t st) {
     if (plan.cluster > 0) {
       cudaLaunchConfig_t cfg{};
-      cfg.gridDim = dim3(static_cast<unsigned>(p.b) * p.s * p.hkv * p.row_tiles * plan.cluster);
+      cfg.gridDim = dim3(static_cast<unsigned>(p.b) * p.queries * p.hkv * p.row_tiles * plan.cluster);
       cfg.blockDim = dim3(128);
       cfg.dynamicSmemBytes = A::kSmem;
       cfg.stream = st;
@@ -927,7 +1002,7 @@ struct PagedAttnLaunch {
     if (cudaGetLastError() != cudaSuccess) return -2;
     if (plan.grid == 1) return 0;  // nothing is shared
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(((p.group < A::RT ? p.group : A::RT) + kJoinRows - 1) / kJoinRows, plan.grid);
+    cfg.gridDim = dim3(((p.rows < A::RT ? p.rows : A::RT) + kJoinRows - 1) / kJoinRows, plan.grid);
     cfg.blockDim = dim3(32 * kJoinRows * kJoinWarps);
     cfg.stream = st;
     cudaLaunchAttribute attr{};
@@ -938,6 +1013,10 @@ struct PagedAttnLaunch {
     return cudaLaunchKernelEx(&cfg, paged_attention_join_kernel<T, DP, WIDE, MASK>, p) == cudaSuccess ? 0 : -2;
   }
 };
+
+// Whether a block takes 16 query rows instead of 8.  32-bit rows of 256 dims do not fit the registers twice: 24 rows took 1297 us
+// in two blocks' worth of 16 and 671 us in three of 8.
+inline bool paged_attention_wide(int dtype, int d, int rows) { return rows > 8 && !(dtype == 0 && d > 128); }
 
 // Calls f with the PagedAttnLaunch of these types and sizes.
 template <typename T, int DP, typename F>
@@ -952,8 +1031,8 @@ int paged_attention_type(int d, bool wide, bool mask, F f) {
   return paged_attention_dp<T, 256>(wide, mask, f);
 }
 template <typename F>
-int paged_attention_dispatch(int dtype, int d, int group, bool mask, F f) {
-  const bool wide = group > 8;
+int paged_attention_dispatch(int dtype, int d, int rows, bool mask, F f) {
+  const bool wide = paged_attention_wide(dtype, d, rows);
   if (dtype == 0) return paged_attention_type<float>(d, wide, mask, f);
   if (dtype == 1) return paged_attention_type<__half>(d, wide, mask, f);
   if (dtype == 2) return paged_attention_type<__nv_bfloat16>(d, wide, mask, f);
@@ -966,8 +1045,11 @@ extern "C" {
 
 static bool paged_attention_params(const OsloPagedAttentionArgs* a, oslo::PagedAttnParams& p) {
   if (a->hkv <= 0 || a->group <= 0 || a->d <= 0 || a->d > 256 || a->d % 8 || a->page_size <= 0 || a->page_size % 16) return false;
-  const long long tiles = a->group > 8 ? (a->group + 15) / 16 : 1;
-  if (a->b * a->s > 0x3fffffff || a->max_pages * a->page_size > 0x3fffffff || a->b * a->s * a->hkv * tiles > 0x3fffffff) return false;
+  if (a->b > 0x3fffffff || a->s > 0x3fffffff || a->group > 0x3fffffff || a->s * a->group > 0x3fffffff) return false;
+  const bool together = a->mask == 0 || a->mask_s == 0;  // the query tokens of a sequence share what they see but for the last ones
+  const long long rows = together ? a->s * a->group : a->group, most = oslo::paged_attention_wide(a->dtype, a->d, rows > 16 ? 16 : rows) ? 16 : 8,
+                  tiles = (rows + most - 1) / most;
+  if (a->b * a->s > 0x3fffffff || a->max_pages * a->page_size > 0x3fffffff || a->b * a->s * a->hkv * tiles * 8 > 0x3fffffff) return false;
   p.q = reinterpret_cast<const void*>(a->q), p.k = reinterpret_cast<const void*>(a->k_pages), p.v = reinterpret_cast<const void*>(a->v_pages);
   p.mask = reinterpret_cast<const float*>(a->mask), p.out = reinterpret_cast<void*>(a->out);
   p.table = reinterpret_cast<const int*>(a->table), p.lens = reinterpret_cast<const int*>(a->lens);
@@ -976,6 +1058,7 @@ static bool paged_attention_params(const OsloPagedAttentionArgs* a, oslo::PagedA
   p.v_head = a->v_head, p.table_stride = a->table_row, p.m_sb = a->mask_b, p.m_ss = a->mask_s;
   p.b = a->b, p.s = a->s, p.hkv = a->hkv, p.group = a->group, p.d = a->d, p.page_size = a->page_size, p.max_pages = a->max_pages;
   p.num_pages = a->num_pages, p.mask_len = a->mask_len, p.scale = static_cast<float>(a->scale), p.row_tiles = static_cast<int>(tiles);
+  p.queries = together ? 1 : static_cast<int>(a->s), p.rows = static_cast<int>(rows);
   return true;
 }
 
@@ -986,7 +1069,7 @@ long long oslo_paged_attention_workspace_bytes(const OsloPagedAttentionArgs* a) 
   PagedAttnParams p{};
   if (!paged_attention_params(a, p)) return -1;
   long long bytes = 0;
-  const int rc = paged_attention_dispatch(a->dtype, a->d, a->group, a->mask != 0, [&](auto l) {
+  const int rc = paged_attention_dispatch(a->dtype, a->d, p.rows, a->mask != 0, [&](auto l) {
     const PagedAttnPlan plan = decltype(l)::plan(p);
     bytes = plan.bytes;
     return plan.resident < 0 ? plan.resident : 0;
@@ -999,7 +1082,7 @@ int oslo_paged_attention(const OsloPagedAttentionArgs* a) {
   if (a->b <= 0 || a->s <= 0) return 0;
   PagedAttnParams p{};
   if (!paged_attention_params(a, p)) return -1;
-  return paged_attention_dispatch(a->dtype, a->d, a->group, a->mask != 0, [&](auto l) {
+  return paged_attention_dispatch(a->dtype, a->d, p.rows, a->mask != 0, [&](auto l) {
     const PagedAttnPlan plan = decltype(l)::plan(p);
     if (plan.resident < 0) return plan.resident;
     return decltype(l)::launch(p, plan, reinterpret_cast<void*>(a->workspace), reinterpret_cast<cudaStream_t>(a->stream));
