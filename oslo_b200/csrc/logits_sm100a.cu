@@ -62,6 +62,10 @@ struct LogitsRow {
   }
 };
 
+// Room for a slice's counters and for their shift to a 16-byte boundary, by up to seven of them.
+template <typename C>
+__host__ __device__ constexpr int counter_bytes(int slice) { return (slice + 8) * static_cast<int>(sizeof(C)); }
+
 // Adds the history's tokens in [v0, v0 + n) to their counters.
 template <typename I, typename C>
 OSLO_DEVINL void count_tokens(const I* tokens, int len, int prompt, int v0, int n, C* seen) {
@@ -111,7 +115,7 @@ __global__ void __launch_bounds__(kLogitsThreads, 5) process_logits_kernel(const
   fetch(threadIdx.x);
   LogitsRow<C> pen{p.rep_s, 1.f, p.pres_s, p.freq_s};
   if constexpr (HISTORY) {
-    for (int i = threadIdx.x; i < static_cast<int>(p.slice * sizeof(C) / 16) + 1; i += kLogitsThreads) counters4[i] = make_uint4(0, 0, 0, 0);
+    for (int i = threadIdx.x; i < counter_bytes<C>(p.slice) / 16; i += kLogitsThreads) counters4[i] = make_uint4(0, 0, 0, 0);
     if (p.rep) pen.rep = p.rep[row];
     if (p.pres) pen.pres = p.pres[row];
     if (p.freq) pen.freq = p.freq[row];
@@ -215,8 +219,8 @@ int process_logits_launch(LogitsParams& p, cudaStream_t st) {
   if (grid > 0x7fffffffll) return -1;
   const unsigned blocks = static_cast<unsigned>(grid);
   if (!p.tokens) process_logits_kernel<T, char><<<blocks, kLogitsThreads, 0, st>>>(p);
-  else if (small) process_logits_kernel<T, uint16_t><<<blocks, kLogitsThreads, p.slice * 2 + 16, st>>>(p);
-  else process_logits_kernel<T, uint32_t><<<blocks, kLogitsThreads, p.slice * 4 + 16, st>>>(p);
+  else if (small) process_logits_kernel<T, uint16_t><<<blocks, kLogitsThreads, counter_bytes<uint16_t>(p.slice), st>>>(p);
+  else process_logits_kernel<T, uint32_t><<<blocks, kLogitsThreads, counter_bytes<uint32_t>(p.slice), st>>>(p);
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
 

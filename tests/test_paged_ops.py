@@ -504,6 +504,9 @@ def test_logits(dev, dtype, rows, v, t, kw):
     (5, 250112, 700, dict(allowed="shared", inplace=True, ids=torch.int32)),
     (200, 8193, 33, dict(allowed="rows", bias="shared")),
     (2, 300001, 100, dict(bias="shared", prompts=False)),
+    (3, 8191, 32767, dict(spread=40, bias="shared")),             # the longest history of 16-bit counters
+    (7, 8191, 32768, dict(spread=40, allowed="rows", strided=True)),  # 32-bit counters, rows off the 16-byte grid
+    (3, 70001, 40000, dict(spread=2, prompts=False, lens=False)),
 ])
 def test_logits_large(dtype, rows, v, t, kw):
     _logits_case("cuda", dtype, rows, v, t, **kw)
