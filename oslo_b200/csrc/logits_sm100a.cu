@@ -8,12 +8,14 @@
 // of that slice in shared memory (integer atomics: their order does not matter), while its first logits are already on their
 // way; then it streams the slice, 16 bytes a thread.  Counters have 16 bits for histories of less than 32768 tokens: a group of
 // eight 16-bit logits then meets one 16-byte load of counters, most of them zero.  Plain streaming runs at the copy bandwidth
-// (192 x 250112 bf16: 35 us); with a history of 4095 tokens, a bias and a mask the same logits take 66 us, bound by
-// issue and latency: the history is read by each of a row's 16 slices (11 us), the bias comes from L2 (15 us), and
-// every element's mask is two instructions (10 us).  Adding a cluster's tokens to each other's counters through distributed
+// (192 x 250112 bf16: 35 us); with a history of 4095 tokens, a bias and a mask the same logits take 58 us, bound by
+// issue and latency: the history is read by each of a row's 16 slices, the bias comes from L2 (as many bytes as the logits twice
+// over), and every element's mask is two instructions.  Adding a cluster's tokens to each other's counters through distributed
 // shared memory, so that a row reads its history once, was slower (105 us): frequent tokens serialise the remote atomics.
 #include "common.cuh"
 #include "step_args.h"
+
+#include <type_traits>
 
 namespace oslo {
 
@@ -34,7 +36,8 @@ struct LogitsParams {
 };
 
 constexpr int kLogitsThreads = 256;
-constexpr int kLogitsAhead = 2;             // 16-byte groups of a thread in flight
+template <typename T>
+constexpr int kLogitsAhead = sizeof(T) / 2 * 2;  // 16-byte groups of a thread in flight: sixteen logits
 constexpr int kLogitsCounters = 32 * 1024;  // bytes of counters of a block
 constexpr int kLogitsLeast = 2048;          // tokens of a slice at least
 
@@ -87,10 +90,10 @@ OSLO_DEVINL void count_tokens(const I* tokens, int len, int prompt, int v0, int 
 }
 
 // C: counter type, uint16_t for histories of less than 32768 tokens, uint32_t for longer ones, void without a history
-template <typename T, typename C>
+template <typename T, typename C, bool BIAS, bool ALLOWED>
 __global__ void __launch_bounds__(kLogitsThreads, 5) process_logits_kernel(const LogitsParams p) {
   constexpr bool HISTORY = sizeof(C) > 1;
-  constexpr int E = 16 / sizeof(T);
+  constexpr int E = 16 / sizeof(T), AHEAD = kLogitsAhead<T>;
   extern __shared__ uint4 counters4[];
   C* const counters = reinterpret_cast<C*>(counters4);
   const int row = blockIdx.x / p.slices, v0 = (blockIdx.x - row * p.slices) * p.slice;
@@ -104,10 +107,10 @@ __global__ void __launch_bounds__(kLogitsThreads, 5) process_logits_kernel(const
   const bool aligned = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(y)) & 15) == 0;
   const int groups = aligned ? (n - head) / E : 0;
   // the first logits are on their way while the history is counted
-  uint4 ahead[kLogitsAhead];
+  uint4 ahead[AHEAD];
   const auto fetch = [&](int g0) {
 #pragma unroll
-    for (int j = 0; j < kLogitsAhead; ++j)
+    for (int j = 0; j < AHEAD; ++j)
       if (g0 + j * kLogitsThreads < groups)
         asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
                      : "=r"(ahead[j].x), "=r"(ahead[j].y), "=r"(ahead[j].z), "=r"(ahead[j].w) : "l"(x + head + (g0 + j * kLogitsThreads) * E));
@@ -132,8 +135,8 @@ __global__ void __launch_bounds__(kLogitsThreads, 5) process_logits_kernel(const
   const auto one = [&](int i) {
     float f = lg_f(x[i]);
     if constexpr (HISTORY) f = pen(f, seen[i]);
-    if (bias) f += bias[i];
-    if (allowed && !((allowed[(v0 + i) >> 5] >> ((v0 + i) & 31)) & 1)) f = -INFINITY;
+    if (BIAS) f += bias[i];
+    if (ALLOWED && !((allowed[(v0 + i) >> 5] >> ((v0 + i) & 31)) & 1)) f = -INFINITY;
     lg_st(y[i], f);
   };
   if (!aligned) {
@@ -143,63 +146,71 @@ __global__ void __launch_bounds__(kLogitsThreads, 5) process_logits_kernel(const
   const int tail = head + groups * E;
   if (threadIdx.x < head) one(threadIdx.x);
   if (threadIdx.x < n - tail) one(tail + threadIdx.x);
-  const bool bias16 = bias && (reinterpret_cast<uintptr_t>(bias + head) & 15) == 0;
-  const auto group = [&](int i, const uint4& u) {
-    union {
-      uint4 u;
-      T t[E];
-    } in, out;
-    in.u = u;
-    float f[E];
+  const bool bias16 = BIAS && (reinterpret_cast<uintptr_t>(bias + head) & 15) == 0;
+  for (int g0 = threadIdx.x; g0 < groups; g0 += AHEAD * kLogitsThreads) {
+    // all operands of the groups in flight are requested before the first is used
+    float4 b[AHEAD][E / 4];
+    unsigned lo[AHEAD], hi[AHEAD];
 #pragma unroll
-    for (int e = 0; e < E; ++e) f[e] = lg_f(in.t[e]);
-    if constexpr (HISTORY) {
-      constexpr int W = E * sizeof(C) / 4;  // words of the group's counters
-      unsigned w[W];
-      if constexpr (W == 2) {
-        *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(seen + i);
-      } else {
+    for (int j = 0; j < AHEAD; ++j) {
+      const int g = g0 + j * kLogitsThreads, i = head + g * E, at = v0 + i;
+      if (g >= groups) break;
+      if constexpr (BIAS) {
 #pragma unroll
-        for (int k = 0; k < W; k += 4) *reinterpret_cast<uint4*>(w + k) = *reinterpret_cast<const uint4*>(seen + i + k * (4 / sizeof(C)));
+        for (int e = 0; e < E; e += 4)
+          b[j][e / 4] = bias16 ? __ldg(reinterpret_cast<const float4*>(bias + i + e))
+                               : make_float4(__ldg(bias + i + e), __ldg(bias + i + e + 1), __ldg(bias + i + e + 2), __ldg(bias + i + e + 3));
       }
-      unsigned any = 0;
+      if constexpr (ALLOWED) {
+        lo[j] = __ldg(allowed + (at >> 5));
+        hi[j] = (at & 31) + E > 32 ? __ldg(allowed + (at >> 5) + 1) : 0u;  // the last group ends inside the last word
+      }
+    }
 #pragma unroll
-      for (int k = 0; k < W; ++k) any |= w[k];
-      if (any) {
+    for (int j = 0; j < AHEAD; ++j) {
+      const int g = g0 + j * kLogitsThreads, i = head + g * E;
+      if (g >= groups) break;
+      union {
+        uint4 u;
+        T t[E];
+      } in, out;
+      in.u = ahead[j];
+      float f[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) f[e] = lg_f(in.t[e]);
+      if constexpr (HISTORY) {
+        constexpr int W = E * sizeof(C) / 4;  // words of the group's counters
+        unsigned w[W];
+        if constexpr (W == 2) {
+          *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(seen + i);
+        } else {
+#pragma unroll
+          for (int k = 0; k < W; k += 4) *reinterpret_cast<uint4*>(w + k) = *reinterpret_cast<const uint4*>(seen + i + k * (4 / sizeof(C)));
+        }
+        unsigned any = 0;
+#pragma unroll
+        for (int k = 0; k < W; ++k) any |= w[k];
+        if (any) {
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            f[e] = pen(f[e], sizeof(C) == 4 ? w[e * sizeof(C) / 4] : (w[e * sizeof(C) / 4] >> (e % (4 / sizeof(C)) * 16)) & 0xffffu);
+        }
+      }
+      if constexpr (BIAS) {
+#pragma unroll
+        for (int e = 0; e < E; e += 4) f[e] += b[j][e / 4].x, f[e + 1] += b[j][e / 4].y, f[e + 2] += b[j][e / 4].z, f[e + 3] += b[j][e / 4].w;
+      }
+      if constexpr (ALLOWED) {
+        const unsigned bits = __funnelshift_r(lo[j], hi[j], (v0 + i) & 31);
 #pragma unroll
         for (int e = 0; e < E; ++e)
-          f[e] = pen(f[e], sizeof(C) == 4 ? w[e * sizeof(C) / 4] : (w[e * sizeof(C) / 4] >> (e % (4 / sizeof(C)) * 16)) & 0xffffu);
+          if (!((bits >> e) & 1)) f[e] = -INFINITY;
       }
+#pragma unroll
+      for (int e = 0; e < E; ++e) lg_st(out.t[e], f[e]);
+      *reinterpret_cast<uint4*>(y + i) = out.u;
     }
-    if (bias) {
-      if (bias16) {
-#pragma unroll
-        for (int e = 0; e < E; e += 4) {
-          const float4 b = __ldg(reinterpret_cast<const float4*>(bias + i + e));
-          f[e] += b.x, f[e + 1] += b.y, f[e + 2] += b.z, f[e + 3] += b.w;
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e) f[e] += __ldg(bias + i + e);
-      }
-    }
-    if (allowed) {
-      const int at = v0 + i, w = at >> 5, sh = at & 31;
-      const unsigned lo = __ldg(allowed + w), hi = sh + E > 32 ? __ldg(allowed + w + 1) : 0u;  // the last group ends inside the last word
-      const unsigned bits = __funnelshift_r(lo, hi, sh);
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (!((bits >> e) & 1)) f[e] = -INFINITY;
-    }
-#pragma unroll
-    for (int e = 0; e < E; ++e) lg_st(out.t[e], f[e]);
-    *reinterpret_cast<uint4*>(y + i) = out.u;
-  };
-  for (int g0 = threadIdx.x; g0 < groups; g0 += kLogitsAhead * kLogitsThreads) {
-#pragma unroll
-    for (int j = 0; j < kLogitsAhead; ++j)
-      if (g0 + j * kLogitsThreads < groups) group(head + (g0 + j * kLogitsThreads) * E, ahead[j]);
-    fetch(g0 + kLogitsAhead * kLogitsThreads);
+    fetch(g0 + AHEAD * kLogitsThreads);
   }
 }
 
@@ -218,9 +229,16 @@ int process_logits_launch(LogitsParams& p, cudaStream_t st) {
   const long long grid = static_cast<long long>(p.rows) * p.slices;
   if (grid > 0x7fffffffll) return -1;
   const unsigned blocks = static_cast<unsigned>(grid);
-  if (!p.tokens) process_logits_kernel<T, char><<<blocks, kLogitsThreads, 0, st>>>(p);
-  else if (small) process_logits_kernel<T, uint16_t><<<blocks, kLogitsThreads, counter_bytes<uint16_t>(p.slice), st>>>(p);
-  else process_logits_kernel<T, uint32_t><<<blocks, kLogitsThreads, counter_bytes<uint32_t>(p.slice), st>>>(p);
+  const auto go = [&](auto bias, auto allowed) {
+    constexpr bool B = decltype(bias)::value, A = decltype(allowed)::value;
+    if (!p.tokens) process_logits_kernel<T, char, B, A><<<blocks, kLogitsThreads, 0, st>>>(p);
+    else if (small) process_logits_kernel<T, uint16_t, B, A><<<blocks, kLogitsThreads, counter_bytes<uint16_t>(p.slice), st>>>(p);
+    else process_logits_kernel<T, uint32_t, B, A><<<blocks, kLogitsThreads, counter_bytes<uint32_t>(p.slice), st>>>(p);
+  };
+  if (p.bias && p.allowed) go(std::true_type(), std::true_type());
+  else if (p.bias) go(std::true_type(), std::false_type());
+  else if (p.allowed) go(std::false_type(), std::true_type());
+  else go(std::false_type(), std::false_type());
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
 
