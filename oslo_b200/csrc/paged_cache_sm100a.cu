@@ -118,14 +118,16 @@ struct HeadTurn {
   }
 };
 
-constexpr int kAppendThreads = 256;
+// Small blocks: 8 prompts of up to 1999 tokens, 32 heads of 128, take 100 us with 64 or 128 threads a block, 110 us with 256 and
+// 169 us with 512 (the copy bandwidth gives 92 us); with 8 key heads of 64 and neighbouring pairs 34, 39, 67 and 123 us.
+constexpr int kAppendThreads = 64;
 constexpr int kAppendRows = 2;  // heads of a thread in flight
 
 // Block (token, part of its heads).  A thread keeps one column (chunk or pair of chunks) and walks over the heads of queries and
 // keys, so it reads its angles once; the values are copied in the same way.  The chain start -> page -> store is three
 // trips to memory: the first heads and values of a real token are read before it, the angles beside it.
 template <typename T, int MODE>
-__global__ void __launch_bounds__(kAppendThreads, MODE == kRotateElements ? 2 : 4) paged_append_kernel(const PagedAppendParams p, int parts) {
+__global__ void __launch_bounds__(kAppendThreads, MODE == kRotateElements ? 12 : 16) paged_append_kernel(const PagedAppendParams p, int parts) {
   using H = HeadTurn<T, MODE>;
   constexpr int E = PagedVec<T>::E;
   const int token = blockIdx.x / parts, part = blockIdx.x - token * parts;
