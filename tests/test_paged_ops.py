@@ -226,6 +226,10 @@ SHAPES = [  # s, hq, hkv, d, page, lens
     (1, 3, 3, 136, 16, [50]),
     (4, 6, 2, 64, 16, [4, 90, 3, 1, 0]),   # new tokens that lie before the sequence's first one see nothing
     (3, 12, 1, 128, 32, [130, 31]),
+    (1, 48, 1, 64, 16, [77, 0, 5]),        # 33 to 64 rows of a key head
+    (5, 20, 2, 128, 16, [90, 4, 65]),
+    (7, 11, 1, 256, 16, [33, 200]),        # more than 64
+    (4, 34, 2, 40, 32, [3, 61]),
 ]
 
 
@@ -247,6 +251,12 @@ def test_attention(dev, dtype, s, hq, hkv, d, page, lens):
     (5, 71, 1, 64, 32, [1500, 33]),
     (1, 4, 2, 256, 16, [2500, 17]),
     (1, 12, 12, 64, 16, [10, 200] * 100),
+    (6, 96, 6, 128, 32, [900, 33, 5000, 6, 0]),
+    (4, 24, 1, 64, 32, [6001, 700, 4]),
+    (150, 4, 2, 128, 64, [151, 1000]),
+    (5, 40, 2, 128, 16, [300, 5, 0, 17, 1200] * 8),    # many groups of more than 32 rows
+    (3, 96, 4, 64, 32, [65, 3, 700] * 6),
+    (1, 70, 2, 256, 16, [40, 41] * 16),
 ])
 def test_attention_long_and_ragged(dtype, s, hq, hkv, d, page, lens):
     _attend_case("cuda", dtype, s, hq, hkv, d, page, lens)
