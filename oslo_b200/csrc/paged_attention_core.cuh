@@ -102,6 +102,8 @@ struct Mma16<__nv_bfloat16> {
     const __nv_bfloat162 r = __floats2bfloat162_rn(lo, hi);
     return reinterpret_cast<const uint32_t&>(r);
   }
+  // one of the two has all exponent bits set
+  static OSLO_DEVINL bool wild(uint32_t r) { return (r & 0x7f80u) == 0x7f80u || (r & 0x7f800000u) == 0x7f800000u; }
   static OSLO_DEVINL float low(uint32_t r) { return __uint_as_float(r << 16); }
   static OSLO_DEVINL float high(uint32_t r) { return __uint_as_float(r & 0xffff0000u); }
 };
@@ -115,6 +117,7 @@ struct Mma16<__half> {
     const __half2 r = __floats2half2_rn(lo, hi);
     return reinterpret_cast<const uint32_t&>(r);
   }
+  static OSLO_DEVINL bool wild(uint32_t r) { return (r & 0x7c00u) == 0x7c00u || (r & 0x7c000000u) == 0x7c000000u; }
   static OSLO_DEVINL float low(uint32_t r) { return __low2float(reinterpret_cast<const __half2&>(r)); }
   static OSLO_DEVINL float high(uint32_t r) { return __high2float(reinterpret_cast<const __half2&>(r)); }
 };
@@ -300,7 +303,9 @@ struct AttnWarp {
         lo[2 * n + x] = Mma16<T>::pack(a - Mma16<T>::low(h), b - Mma16<T>::high(h));
       }
     if constexpr (!WIDE) hi[1] = lo[0], hi[3] = lo[2];  // the remainders take the empty rows
-    if (least == most || token + TT <= least) {
+    // Some tokens of a group's last tiles are seen by some rows only.  Their weights are zero for the others, which is enough where
+    // the values are finite; where one is not, each query token gets a product of its own, over the tokens that it sees.
+    if (least == most || token + TT <= least || !wild(ring)) {
 #pragma unroll
       for (int j = 0; j < VC; ++j) {
         uint4 vr[VT];
@@ -317,8 +322,7 @@ struct AttnWarp {
       }
       return;
     }
-    // Some of the tile's tokens are seen by some rows only; what they hold must not reach the others, not even times zero.  Each
-    // query token of the group gets a product of its own, over the tokens that it sees.
+#pragma unroll 1
     for (int end = least; end <= most; ++end)
 #pragma unroll
       for (int j = 0; j < VC; ++j) {
@@ -328,13 +332,24 @@ struct AttnWarp {
         for (int e = 0; e < E; ++e) {
           uint32_t b0, b1;
           columns(vr, e, b0, b1);
-          float c[4] = {0.f, 0.f, 0.f, 0.f};
+          float c[4] = {o[j][e][0], o[j][e][1], o[j][e][2], o[j][e][3]};
           Mma16<T>::run(c, hi[0], hi[1], hi[2], hi[3], b0, b1);
           if constexpr (WIDE) Mma16<T>::run(c, lo[0], lo[1], lo[2], lo[3], b0, b1);
-          if (end0 == end) o[j][e][0] += c[0], o[j][e][1] += c[1];
-          if ((WIDE ? end1 : end0) == end) o[j][e][2] += c[2], o[j][e][3] += c[3];
+          if (end0 == end) o[j][e][0] = c[0], o[j][e][1] = c[1];
+          if ((WIDE ? end1 : end0) == end) o[j][e][2] = c[2], o[j][e][3] = c[3];
         }
       }
+  }
+
+  // Whether a value of the tile is infinite or not a number.
+  static OSLO_DEVINL bool wild(const T* ring) {
+    const int lane = threadIdx.x & 31;
+    bool any = false;
+    for (int x = lane; x < TT * (DP / E); x += 32) {
+      const uint4 v = *reinterpret_cast<const uint4*>(ring + TT * PITCH + x / (DP / E) * PITCH + x % (DP / E) * E);
+      any = any || Mma16<T>::wild(v.x) || Mma16<T>::wild(v.y) || Mma16<T>::wild(v.z) || Mma16<T>::wild(v.w);
+    }
+    return __any_sync(0xffffffffu, any);
   }
 
   OSLO_DEVINL void join(T* ring, float* ml) {
@@ -540,20 +555,29 @@ struct AttnWarp<float, DP, WIDE, MASK> {
             if (!((visible >> (4 * at)) & 1)) v[t] = make_float4(0.f, 0.f, 0.f, 0.f);
           }
         }
-        if (mixed) {  // nor do those of a token that the row does not see
+        if (mixed) {  // tokens that only some rows see have weight zero for the others, which is enough where the values are finite
+          bool wild = false;
 #pragma unroll
-          for (int g = 0; g < RT; ++g) {
-            if (g >= rows) break;
-            const int sees = least + (first + g) / group - token;
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-              if ((HALVES == 2 ? 2 * (t0 + t) + half : t0 + t) >= sees) continue;
-              const float w = weights[g * TT + half * 4 + t0 + t];
-              float4& y = o[g][j];
-              y.x = fmaf(w, v[t].x, y.x), y.y = fmaf(w, v[t].y, y.y), y.z = fmaf(w, v[t].z, y.z), y.w = fmaf(w, v[t].w, y.w);
-            }
+          for (int t = 0; t < 4; ++t) {
+            const uint32_t most_bits = 0x7f800000u;
+            wild = wild || (__float_as_uint(v[t].x) & most_bits) == most_bits || (__float_as_uint(v[t].y) & most_bits) == most_bits ||
+                   (__float_as_uint(v[t].z) & most_bits) == most_bits || (__float_as_uint(v[t].w) & most_bits) == most_bits;
           }
-          continue;
+          if (__any_sync(0xffffffffu, wild)) {
+#pragma unroll
+            for (int g = 0; g < RT; ++g) {
+              if (g >= rows) break;
+              const int sees = least + (first + g) / group - token;
+#pragma unroll
+              for (int t = 3; t >= 0; --t) {  // the order of the sums below
+                if ((HALVES == 2 ? 2 * (t0 + t) + half : t0 + t) >= sees) continue;
+                const float w = weights[g * TT + half * 4 + t0 + t];
+                float4& y = o[g][j];
+                y.x = fmaf(w, v[t].x, y.x), y.y = fmaf(w, v[t].y, y.y), y.z = fmaf(w, v[t].z, y.z), y.w = fmaf(w, v[t].w, y.w);
+              }
+            }
+            continue;
+          }
         }
 #pragma unroll
         for (int g = 0; g < RT; ++g) {

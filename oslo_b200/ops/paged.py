@@ -250,6 +250,8 @@ def _load():
 
 @lru_cache(maxsize=None)
 def _status_ptr(device: int) -> int:
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("call the paged cache's functions once on a device before capturing them: their status word is made then")
     ptr = _lib.status_word(torch.device("cuda", device)).data_ptr()
     module = _lib.step_calls()
     if module is not None:

@@ -361,6 +361,24 @@ def test_pools_inside_a_larger_tensor(dev):
     assert ((got.double() - want).abs() <= tol).all()
 
 
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_pools_of_more_than_two_billion_elements(dtype):
+    torch.manual_seed(8)
+    pages, hkv, page, d = 140_000, 2, 64, 128  # 2.3e9 elements
+    kp, vp = (torch.empty(pages, hkv, page, d, dtype=dtype, device="cuda") for _ in range(2))
+    table = torch.tensor([[pages - 1, 131_072, 0], [139_000, 5, pages - 2]], dtype=torch.int32, device="cuda")
+    k, v = (torch.randn(2, 150, hkv, d, device="cuda").to(dtype) for _ in range(2))
+    OF.paged_kv_append(k, v, kp, vp, table, torch.zeros(2, dtype=torch.int32, device="cuda"))
+    for r in range(2):
+        assert torch.equal(_seq(kp, table, r, 150), k[r]) and torch.equal(_seq(vp, table, r, 150), v[r])
+    q = torch.randn(2, 1, 8, d, device="cuda").to(dtype)
+    got = OF.paged_attention(q, kp, vp, table, torch.tensor([150, 131], dtype=torch.int32, device="cuda"))
+    _sync_status("cuda")
+    want, tol = _attend_exact(q, kp, vp, table, [150, 131], d ** -0.5, None)
+    assert ((got.double() - want).abs() <= tol).all()
+
+
 def test_refusals_of_the_cache():
     kp, vp, table = _pool([20, 20], 16, 2, 64, torch.float32, "cpu")
     q, k, v = (torch.randn(2, 1, n, 64) for n in (4, 2, 2))
@@ -520,6 +538,17 @@ def test_logits(dev, dtype, rows, v, t, kw):
 ])
 def test_logits_large(dtype, rows, v, t, kw):
     _logits_case("cuda", dtype, rows, v, t, **kw)
+
+
+@gpu
+def test_logits_of_more_than_two_billion_elements():
+    rows, v = 8700, 250_112
+    x = torch.empty(rows, v, dtype=torch.bfloat16, device="cuda")
+    some = torch.tensor([0, 1, 4000, 8586, 8587, 8699], device="cuda")
+    x[some] = torch.randn(6, v, device="cuda").bfloat16()
+    tokens = torch.randint(0, v, (rows, 20), device="cuda")
+    got = OF.process_logits(x, tokens, repetition_penalty=1.2, frequency_penalty=0.1)
+    assert torch.equal(got[some], OF.process_logits(x[some], tokens[some], repetition_penalty=1.2, frequency_penalty=0.1))
 
 
 @pytest.mark.parametrize("dev", DEVICES)
