@@ -192,6 +192,12 @@ def _generate_ragged(model, input_ids, lengths, max_new_tokens, pick, temperatur
     """Generation from right-padded prompts of different lengths over the paged cache."""
     if not getattr(getattr(model, "module", model), "ragged_prompts", False):
         raise ValueError(f"{type(model).__name__} takes prompts of one length")
+    pc = getattr(model, "parallel_context", None)
+    if pc is not None and getattr(pc, "tensor_parallel_size", 1) > 1:
+        from oslo_b200.distributed import ParallelMode
+
+        if pc.tensor_parallel_mode != ParallelMode.TENSOR_1D:
+            raise ValueError("layouts that split the batch over ranks take prompts of one length")
     b, width = input_ids.shape
     if len(lengths) != b or min(lengths) < 1 or max(lengths) > width:
         raise ValueError(f"prompt_lengths has a number from 1 to {width} for each of the {b} prompts: got {lengths}")

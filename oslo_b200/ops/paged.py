@@ -300,9 +300,9 @@ class PagedDecodeCache:
         return max(self.lengths, default=0)
 
     def positions(self, s: int, device) -> torch.Tensor:
-        """Positions of the next ``s`` tokens: ``[batch, s]``, or ``[1, s]`` before the first forward."""
+        """Positions of the next ``s`` tokens: ``[1, s]`` where all sequences have as many, else ``[batch, s]``."""
         new = torch.arange(s, device=device)
-        return new.unsqueeze(0) if self._held is None else self._held.unsqueeze(1) + new
+        return (new + self.offset).unsqueeze(0) if len(set(self.lengths)) <= 1 else self._held.unsqueeze(1) + new
 
     def begin_forward(self, counts: Optional[Sequence[int]] = None):
         self._layer, self._counts = 0, None if counts is None else [int(c) for c in counts]

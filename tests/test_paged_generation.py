@@ -232,6 +232,34 @@ def test_server_takes_the_settings():
         assert r.status_code == 200 and r.json()["output_ids"] == [[1, 2, 3, 9, 9, 9, 9], [4, 5, 9, 9, 9, 9]]
 
 
+def _parallel_worker(rank, world, kind, two_d):
+    import oslo_b200
+    from oslo_b200 import ParallelContext, ParallelMode
+    from oslo_b200.parallel import TensorParallel
+
+    pc = ParallelContext.from_torch(tensor_parallel_size=world, backend="gloo", seed=0,
+                                    tensor_parallel_mode=ParallelMode.TENSOR_2D if two_d else ParallelMode.TENSOR_1D)
+    ref, wrapped = _model(kind), TensorParallel(_model(kind), pc)
+    oslo_b200.ready(wrapped, pc)
+    prompt = torch.randint(1, 67, (2, 9), generator=torch.Generator().manual_seed(1))
+    kw = dict(max_new_tokens=10, paged_cache=True, page_size=16, repetition_penalty=1.3)
+    assert torch.equal(generate(wrapped, prompt, **kw), generate(ref, prompt, **kw))
+    if two_d:
+        with pytest.raises(ValueError, match="split the batch"):
+            generate(wrapped, prompt, prompt_lengths=[4, 9], **kw)
+    else:
+        assert torch.equal(generate(wrapped, prompt, prompt_lengths=[4, 9], **kw), generate(ref, prompt, prompt_lengths=[4, 9], **kw))
+    pc.destroy()
+
+
+@pytest.mark.parametrize("kind,world,two_d", [("gpt2", 2, False), ("neox", 2, False), ("llama", 2, False), ("neox", 4, True),
+                                              ("gpt2", 4, True)])
+def test_paged_generation_through_tensor_parallel_models(kind, world, two_d):
+    from dist_utils import run_dist
+
+    run_dist(_parallel_worker, world, kind, two_d)
+
+
 # ------------------------------------------------------------------------------------------------ the operators on the GPU
 def _step(q, k, v, kp, vp, table, held, rope, logits, tokens, lens):
     """One decoding step's calls."""
