@@ -1135,7 +1135,10 @@ int paged_attention_mask(PagedAttnParams& p, int block_rows, PagedAttnPlan& plan
   if constexpr (sizeof(T) == 2) {
     if (block_rows == kRows64) return paged_attention_do<PagedAttnLaunch<T, DP, true, MASK, true>>(p, plan, run, ws, st);
   }
-  return paged_attention_do<PagedAttnLaunch<T, DP, true, MASK, false>>(p, plan, run, ws, st);
+  if constexpr (sizeof(T) == 2 || DP < 256) {
+    if (block_rows == kRows16) return paged_attention_do<PagedAttnLaunch<T, DP, true, MASK, false>>(p, plan, run, ws, st);
+  }
+  return -1;
 }
 template <typename T, int DP>
 int paged_attention_dp(PagedAttnParams& p, int block_rows, PagedAttnPlan& plan, bool run, void* ws, cudaStream_t st) {
