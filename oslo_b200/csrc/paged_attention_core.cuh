@@ -173,7 +173,7 @@ struct AttnWarp {
   uint4 q0[KC], q1[WIDE ? KC : 1];
   float o[VC][E][4];  // rows r and r + 8; with up to 8 rows the second pair holds what the remainders of the weights add
   float m0, m1, l0, l1;
-  int end0, end1, least, most;  // tokens that rows r and r + 8 see; of all rows, the least and the most
+  int end0, end1, least, most;  // tokens that rows r and r + 8 see; of the warp's rows, the least and the most
 
   OSLO_DEVINL void load_q(const PagedAttnParams& p, const Segment& seg, float*) {
     const int r = (threadIdx.x & 31) >> 2, quad = threadIdx.x & 3;
@@ -304,9 +304,10 @@ struct AttnWarp {
         lo[2 * n + x] = Mma16<T>::pack(a - Mma16<T>::low(h), b - Mma16<T>::high(h));
       }
     if constexpr (!WIDE) hi[1] = lo[0], hi[3] = lo[2];  // the remainders take the empty rows
-    // Some tokens of a group's last tiles are seen by some rows only.  Their weights are zero for the others, which is enough where
-    // the values are finite; where one is not, each query token gets a product of its own, over the tokens that it sees.
-    if (least == most || token + TT <= least || !wild(ring)) {
+    // Some tokens of a group's last tiles are seen by some rows only, or by rows of another warp or block only.  Their weights are
+    // zero for the others, which is enough where the values are finite; where one is not, each query token gets a product of its
+    // own, over the tokens that it sees.
+    if (min(token + TT, limit) <= least || !wild(ring)) {
 #pragma unroll
       for (int j = 0; j < VC; ++j) {
         uint4 vr[VT];
@@ -435,7 +436,7 @@ struct AttnWarp<float, DP, WIDE, MASK> {
   float4 o[RT][VC];
   float m[OWN], l[OWN];
   int end[OWN];  // tokens that the lane's rows see
-  int rows, first, group, least, most;  // row g sees least + (first + g) / group tokens
+  int rows, first, group, least;  // row g sees least + (first + g) / group tokens
 
   static OSLO_DEVINL int own_row(int i) {
     const int quad = threadIdx.x & 3;
@@ -449,8 +450,7 @@ struct AttnWarp<float, DP, WIDE, MASK> {
     }
 #pragma unroll
     for (int i = 0; i < OWN; ++i) end[i] = seg.length + seg.token(p, min(own_row(i), rows - 1));
-    first = seg.row0 % p.group, group = p.group;
-    least = seg.length + seg.token(p, 0), most = seg.length + seg.token(p, rows - 1);
+    first = seg.row0 % p.group, group = p.group, least = seg.length + seg.token(p, 0);
     __syncthreads();
   }
   OSLO_DEVINL void clear() {
@@ -542,7 +542,7 @@ struct AttnWarp<float, DP, WIDE, MASK> {
     }
     constexpr int N = TT / HALVES;  // tokens of a lane
     const int half = HALVES == 2 ? lane >> 4 : 0, column = (HALVES == 2 ? lane & 15 : lane) * 4;
-    const bool mixed = least != most && token + TT > least;
+    const bool mixed = min(token + TT, limit) > least;
 #pragma unroll
     for (int j = 0; j < VC; ++j)
 #pragma unroll
@@ -556,7 +556,7 @@ struct AttnWarp<float, DP, WIDE, MASK> {
             if (!((visible >> (4 * at)) & 1)) v[t] = make_float4(0.f, 0.f, 0.f, 0.f);
           }
         }
-        if (mixed) {  // tokens that only some rows see have weight zero for the others, which is enough where the values are finite
+        if (mixed) {  // tokens that some rows do not see have weight zero for them, which is enough where the values are finite
           bool wild = false;
 #pragma unroll
           for (int t = 0; t < 4; ++t) {

@@ -1,0 +1,69 @@
+"""Edges of the paged cache's and the logits' operators: values, layouts and arguments at which they could go wrong.
+
+Tolerances count roundings, as in test_paged_ops.py: u = 2**-24 is the unit rounding of 32 bits, a result rounded to type t is off by
+``eps(t) / 2`` of its value.
+"""
+import math
+
+import pytest
+import torch
+
+from oslo_b200.nn import functional as OF
+from test_paged_ops import DEVICES, TYPES, U, _attend_exact, _half_step, _pool, _seq, _sync_status
+
+gpu = pytest.mark.gpu
+I32 = dict(dtype=torch.int32)
+
+# s, query heads, key heads, head dim, page, lengths, width of the table in tokens: calls that the kernels' forms take
+FORMS = [
+    (1, 6, 2, 64, 16, [70, 33], 0),                     # 8 rows, one launch
+    (1, 4, 2, 128, 32, [500, 70], 9000),                # 8 rows, two launches
+    (1, 12, 1, 256, 16, [70, 41], 0),                   # 16 rows, one launch
+    (1, 24, 2, 128, 16, [300, 77], 9000),               # 16 rows, two launches
+    (3, 6, 2, 64, 16, [70, 33], 0),                     # several new tokens
+    (5, 40, 2, 128, 16, [90, 65] + [40] * 38, 0),       # 64 rows, one launch
+    (5, 40, 2, 64, 16, [90, 65] + [200] * 38, 9000),    # 64 rows, two launches
+    (3, 70, 1, 256, 16, [60, 41] + [30] * 30, 9000),
+]
+
+
+def _wide(table, tokens, page):
+    """The same table with room for sequences of ``tokens`` tokens."""
+    wide = torch.zeros(table.shape[0], max(table.shape[1], tokens // page), **I32)
+    wide[:, : table.shape[1]] = table.cpu()
+    return wide.to(table.device)
+
+
+def _form(dev, dtype, form, seed=0):
+    torch.manual_seed(seed)
+    s, hq, hkv, d, page, lens, width = form
+    kp, vp, table = _pool(lens, page, hkv, d, dtype, dev)
+    q = torch.randn(len(lens), s, hq, d).to(dtype).to(dev)
+    return q, kp, vp, _wide(table, width, page), torch.tensor(lens, **I32).to(dev)
+
+
+# ------------------------------------------------------------------------------------------------ attention: values
+LATER = [  # the query tokens of a sequence fill several blocks, or several warps of one
+    (4, 24, 1, 64, 32, [61, 40], 0), (4, 24, 1, 64, 32, [601, 40], 9000),      # 16 rows a block, of one or two tokens
+    (3, 16, 1, 256, 16, [33, 20], 0),                                         # 8 or 16 rows a block
+    (2, 40, 1, 128, 16, [33, 50], 0), (9, 8, 2, 80, 16, [70, 9], 0),
+    (5, 40, 2, 64, 16, [40, 5, 0, 17, 3, 90, 64, 65] * 5, 0),                 # 64 rows a block, 16 a warp
+    (5, 40, 2, 128, 16, [40, 5, 0, 17, 3, 90, 64, 65] * 5, 9000),
+    (7, 12, 1, 96, 16, [70, 8, 0, 33] * 20, 0),
+]
+
+
+@pytest.mark.parametrize("dev,form", [("cpu", LATER[4])] + [pytest.param("cuda", f, marks=gpu) for f in LATER])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_later_tokens_do_not_show_in_any_block(dev, dtype, form):
+    """The newest token's key is NaN and its value infinite; the results of the tokens before it do not change."""
+    q, kp, vp, table, lens = _form(dev, dtype, form)
+    s, _, _, _, page, n, _ = form
+    want = OF.paged_attention(q, kp, vp, table, lens)
+    rows = [r for r in range(len(n)) if n[r]]
+    for r in rows:
+        t = n[r] - 1
+        kp[int(table[r, t // page]), :, t % page], vp[int(table[r, t // page]), :, t % page] = math.nan, math.inf
+    got = OF.paged_attention(q, kp, vp, table, lens)
+    assert torch.equal(got[:, : s - 1], want[:, : s - 1])
+    assert got[rows, s - 1].isnan().all()
