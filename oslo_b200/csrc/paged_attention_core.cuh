@@ -31,6 +31,7 @@
 #include "common.cuh"
 
 #include <atomic>
+#include <type_traits>
 
 namespace oslo {
 
@@ -103,8 +104,8 @@ struct Mma16<__nv_bfloat16> {
     const __nv_bfloat162 r = __floats2bfloat162_rn(lo, hi);
     return reinterpret_cast<const uint32_t&>(r);
   }
-  // one of the two has all exponent bits set
-  static OSLO_DEVINL bool wild(uint32_t r) { return (r & 0x7f80u) == 0x7f80u || (r & 0x7f800000u) == 0x7f800000u; }
+  // all bits of those of the two that are infinite or not a number
+  static OSLO_DEVINL uint32_t wild(uint32_t r) { return ((r & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((r & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u); }
   static OSLO_DEVINL float low(uint32_t r) { return __uint_as_float(r << 16); }
   static OSLO_DEVINL float high(uint32_t r) { return __uint_as_float(r & 0xffff0000u); }
 };
@@ -118,7 +119,7 @@ struct Mma16<__half> {
     const __half2 r = __floats2half2_rn(lo, hi);
     return reinterpret_cast<const uint32_t&>(r);
   }
-  static OSLO_DEVINL bool wild(uint32_t r) { return (r & 0x7c00u) == 0x7c00u || (r & 0x7c000000u) == 0x7c000000u; }
+  static OSLO_DEVINL uint32_t wild(uint32_t r) { return ((r & 0x7c00u) == 0x7c00u ? 0xffffu : 0u) | ((r & 0x7c000000u) == 0x7c000000u ? 0xffff0000u : 0u); }
   static OSLO_DEVINL float low(uint32_t r) { return __low2float(reinterpret_cast<const __half2&>(r)); }
   static OSLO_DEVINL float high(uint32_t r) { return __high2float(reinterpret_cast<const __half2&>(r)); }
 };
@@ -219,6 +220,8 @@ struct AttnWarp {
   }
 
   // One tile of the ring: its TT tokens start at `token`; tokens at or past `limit` are not seen.
+  // CAREFUL: values may be infinite or not a number, see below.
+  template <bool CAREFUL>
   OSLO_DEVINL void tile(const PagedAttnParams& p, const T* ring, int token, int limit, const float* mask, float*) {
     const int lane = threadIdx.x & 31, r = lane >> 2, quad = lane & 3;
     float add[NT][2];
@@ -304,10 +307,7 @@ struct AttnWarp {
         lo[2 * n + x] = Mma16<T>::pack(a - Mma16<T>::low(h), b - Mma16<T>::high(h));
       }
     if constexpr (!WIDE) hi[1] = lo[0], hi[3] = lo[2];  // the remainders take the empty rows
-    // Some tokens of a group's last tiles are seen by some rows only, or by rows of another warp or block only.  Their weights are
-    // zero for the others, which is enough where the values are finite; where one is not, each query token gets a product of its
-    // own, over the tokens that it sees.
-    if (min(token + TT, limit) <= least || !wild(ring)) {
+    if constexpr (!CAREFUL) {
 #pragma unroll
       for (int j = 0; j < VC; ++j) {
         uint4 vr[VT];
@@ -322,36 +322,44 @@ struct AttnWarp {
             Mma16<T>::run(o[j][e], a[0], a[1], a[2], a[3], b0, b1);
           }
       }
-      return;
-    }
+    } else {
+      // An infinite value (or one that is not a number) times a weight in two parts, or times the weight zero of a row that does not
+      // see it, would be NaN.  So each query token gets a product of its own, over the tokens that it sees, and in it such values
+      // are left out of the parts' product and get another one, with 1 for every weight above zero.
+      uint32_t one[4];
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          one[2 * n + x] = x == 0 || WIDE ? Mma16<T>::pack(sc[n][2 * x] > 0.f ? 1.f : 0.f, sc[n][2 * x + 1] > 0.f ? 1.f : 0.f) : 0u;
 #pragma unroll 1
-    for (int end = least; end <= most; ++end)
+      for (int end = min(token + TT, limit) <= least ? most : least; end <= most; ++end) {
+        const bool mine0 = min(token + TT, limit) <= least || end0 == end, mine1 = min(token + TT, limit) <= least || end1 == end;
 #pragma unroll
-      for (int j = 0; j < VC; ++j) {
-        uint4 vr[VT];
-        load_v<true>(vr, ring, j, seen, end - token);
+        for (int j = 0; j < VC; ++j) {
+          uint4 vr[VT], inf[VT];
+          load_v<true>(vr, ring, j, seen, end - token);
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          uint32_t b0, b1;
-          columns(vr, e, b0, b1);
-          float c[4] = {o[j][e][0], o[j][e][1], o[j][e][2], o[j][e][3]};
-          Mma16<T>::run(c, hi[0], hi[1], hi[2], hi[3], b0, b1);
-          if constexpr (WIDE) Mma16<T>::run(c, lo[0], lo[1], lo[2], lo[3], b0, b1);
-          if (end0 == end) o[j][e][0] = c[0], o[j][e][1] = c[1];
-          if ((WIDE ? end1 : end0) == end) o[j][e][2] = c[2], o[j][e][3] = c[3];
+          for (int t = 0; t < VT; ++t) {
+            inf[t].x = vr[t].x & Mma16<T>::wild(vr[t].x), inf[t].y = vr[t].y & Mma16<T>::wild(vr[t].y);
+            inf[t].z = vr[t].z & Mma16<T>::wild(vr[t].z), inf[t].w = vr[t].w & Mma16<T>::wild(vr[t].w);
+            vr[t].x ^= inf[t].x, vr[t].y ^= inf[t].y, vr[t].z ^= inf[t].z, vr[t].w ^= inf[t].w;
+          }
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            uint32_t b0, b1;
+            columns(vr, e, b0, b1);
+            float c[4] = {o[j][e][0], o[j][e][1], o[j][e][2], o[j][e][3]}, w[4] = {0.f, 0.f, 0.f, 0.f};
+            Mma16<T>::run(c, hi[0], hi[1], hi[2], hi[3], b0, b1);
+            if constexpr (WIDE) Mma16<T>::run(c, lo[0], lo[1], lo[2], lo[3], b0, b1);
+            columns(inf, e, b0, b1);
+            Mma16<T>::run(w, one[0], one[1], one[2], one[3], b0, b1);
+            if (mine0) o[j][e][0] = c[0] + w[0], o[j][e][1] = c[1] + w[1];
+            if (WIDE ? mine1 : mine0) o[j][e][2] = WIDE ? c[2] + w[2] : c[2], o[j][e][3] = WIDE ? c[3] + w[3] : c[3];
+          }
         }
       }
-  }
-
-  // Whether a value of the tile is infinite or not a number.
-  static OSLO_DEVINL bool wild(const T* ring) {
-    const int lane = threadIdx.x & 31;
-    bool any = false;
-    for (int x = lane; x < TT * (DP / E); x += 32) {
-      const uint4 v = *reinterpret_cast<const uint4*>(ring + TT * PITCH + x / (DP / E) * PITCH + x % (DP / E) * E);
-      any = any || Mma16<T>::wild(v.x) || Mma16<T>::wild(v.y) || Mma16<T>::wild(v.z) || Mma16<T>::wild(v.w);
     }
-    return __any_sync(0xffffffffu, any);
   }
 
   OSLO_DEVINL void join(T* ring, float* ml) {
@@ -462,6 +470,7 @@ struct AttnWarp<float, DP, WIDE, MASK> {
       for (int j = 0; j < VC; ++j) o[g][j] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
 
+  template <bool CAREFUL>
   OSLO_DEVINL void tile(const PagedAttnParams& p, const float* ring, int token, int limit, const float* mask, float* scratch) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, quad = lane & 3;
     float* const weights = scratch + RT * DP + warp * WEIGHTS;
@@ -674,12 +683,12 @@ struct PagedAttn : AttnWarp<T, DP, WIDE, MASK> {
   // Row maxima of the four warps, then their row sums.
   static OSLO_DEVINL float* ml_of(char* smem) { return reinterpret_cast<float*>(smem + kRing * WARPS); }
 
-  // Attends over tokens [begin, end) of a segment with all warps of the block and joins them.
-  OSLO_DEVINL void walk(const PagedAttnParams& p, char* smem, Segment& seg, int limit, int begin, int end) {
+  // The warps' sums over tokens [begin, end) of a segment.
+  template <bool CAREFUL>
+  OSLO_DEVINL void pass(const PagedAttnParams& p, char* smem, const Segment& seg, int limit, int begin, int end) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h = seg.h;
     const float* mask = MASK ? p.mask + seg.b * p.m_sb + seg.first * p.m_ss : nullptr;
     const int* table = p.table + seg.b * p.table_stride;
-    seg.length = p.lens[seg.b] - p.s + 1;
     T* ring = reinterpret_cast<T*>(smem + kRing * warp);
     const T* k = static_cast<const T*>(p.k) + h * p.k_head;
     const T* v = static_cast<const T*>(p.v) + h * p.v_head;
@@ -719,33 +728,41 @@ struct PagedAttn : AttnWarp<T, DP, WIDE, MASK> {
 #pragma unroll 1
           for (int w = 0; w < WARPS; ++w)
             if (t + w * TT < end)
-              this->tile(p, reinterpret_cast<const T*>(smem + kRing * w) + slot * TILE, t + w * TT, (all_missing[w] >> slot) & 1 ? 0 : limit, mask, scratch);
+              this->template tile<CAREFUL>(p, reinterpret_cast<const T*>(smem + kRing * w) + slot * TILE, t + w * TT,
+                                           (all_missing[w] >> slot) & 1 ? 0 : limit, mask, scratch);
         }
         __syncthreads();
         advance(slot);
         slot = slot + 1 == STAGES ? 0 : slot + 1;
       }
-      copy_wait<0>();
-      __syncwarp();
-      this->leave(reinterpret_cast<float*>(ring), ml_of(smem));
-      __syncthreads();
-      return;
-    }
-    this->load_q(p, seg, scratch);
-    this->clear();
-    for (int slot = 0; t < end; t += STEP) {
-      copy_wait<STAGES - 1>();
-      __syncwarp();
-      this->tile(p, ring + slot * TILE, t, (missing >> slot) & 1 ? 0 : limit, mask, scratch);
-      __syncwarp();
-      advance(slot);
-      slot = slot + 1 == STAGES ? 0 : slot + 1;
+    } else {
+      this->load_q(p, seg, scratch);
+      this->clear();
+      for (int slot = 0; t < end; t += STEP) {
+        copy_wait<STAGES - 1>();
+        __syncwarp();
+        this->template tile<CAREFUL>(p, ring + slot * TILE, t, (missing >> slot) & 1 ? 0 : limit, mask, scratch);
+        __syncwarp();
+        advance(slot);
+        slot = slot + 1 == STAGES ? 0 : slot + 1;
+      }
     }
     copy_wait<0>();
     __syncwarp();
-    this->join(ring, ml_of(smem));  // then every thread may read row sums, maxima and the warps' outputs, scaled to one maximum
   }
-
+  // Attends over tokens [begin, end) of a segment with all warps of the block; every thread may then read row sums, maxima and outputs.
+  template <bool CAREFUL>
+  OSLO_DEVINL void walk(const PagedAttnParams& p, char* smem, Segment& seg, int limit, int begin, int end) {
+    T* ring = reinterpret_cast<T*>(smem + kRing * (threadIdx.x >> 5));
+    seg.length = p.lens[seg.b] - p.s + 1;
+    this->template pass<CAREFUL>(p, smem, seg, limit, begin, end);
+    if constexpr (SPLIT) {
+      this->leave(reinterpret_cast<float*>(ring), ml_of(smem));
+      __syncthreads();
+    } else {
+      this->join(ring, ml_of(smem));  // the warps' outputs, scaled to one maximum
+    }
+  }
 };
 
 // The tokens that a group's last query token sees, as far as the table (and the mask) reach.
@@ -779,6 +796,35 @@ OSLO_DEVINL float4 block_sum(const char* smem, int row, int dim, float& l, float
   return s;
 }
 
+// Where a block's sums of a segment go.
+struct Finish {
+  float2* total;   // with it: to shared memory for the cluster, maxima and sums to total[row]
+  long long slot;  // else, where not negative: to this slot of the parts
+};
+
+// Puts the block's sums where they go; whether one of this thread's is infinite or not a number.
+template <typename A, typename T, int DP>
+OSLO_DEVINL bool finish(const PagedAttnParams& p, char* smem, const Segment& seg, const Finish& to) {
+  const int quads = p.d / 4;
+  float wild = 0.f;  // 0, or NaN
+  for (int x = threadIdx.x; x < seg.rows * quads; x += 128) {
+    const int row = x / quads, dim = (x - row * quads) * 4;
+    float l, m;
+    const float4 s = block_sum<A>(smem, row, dim, l, m);
+    wild = fmaf(s.x, 0.f, fmaf(s.y, 0.f, fmaf(s.z, 0.f, fmaf(s.w, 0.f, wild))));
+    if (to.total != nullptr) {  // in place of the first warp's output, or where its warp left it
+      *reinterpret_cast<float4*>(smem + A::place(row, dim)) = s;
+      if (dim == 0) to.total[row] = make_float2(m, l);
+    } else if (to.slot >= 0) {
+      *reinterpret_cast<float4*>(p.part_o + (to.slot * A::ROWS + row) * DP + dim) = s;
+      if (dim == 0) p.part_ml[to.slot * A::ROWS + row] = make_float2(m, l);
+    } else {
+      pa_store(static_cast<T*>(p.out) + seg.out_at(p, row) + dim, s, l);
+    }
+  }
+  return wild != 0.f;
+}
+
 // Units of a segment: those that starting it costs, then its tokens.
 template <typename A>
 OSLO_DEVINL int segment_units(int limit) {
@@ -786,8 +832,64 @@ OSLO_DEVINL int segment_units(int limit) {
   return A::SEGMENT_UNITS + max(1, (limit + UNIT - 1) / UNIT);
 }
 
+// A block's range of units.
+struct Range {
+  long long u, u_end, base, units, blocks;  // base: first unit of the query that u is in; units: of the whole grid
+  int query;
+};
+
+// Attends over the segments of a range; whether one of the thread's sums is infinite or not a number.
+template <typename A, typename T, int DP, bool MASK, bool CAREFUL>
+OSLO_DEVINL bool attend_range(const PagedAttnParams& p, char* smem, const Range& range) {
+  constexpr int UNIT = A::WARPS * A::TT;
+  const int heads = p.hkv * p.row_tiles;
+  long long u = range.u, base = range.base;
+  int query = range.query;
+  int limit = query_limit<MASK>(p, query, threadIdx.x == 0);
+  int n_units = segment_units<A>(limit);
+  bool wild = false;
+
+  while (u < range.u_end) {
+    if (u >= base + static_cast<long long>(n_units) * heads) {
+      base += static_cast<long long>(n_units) * heads;
+      ++query;
+      limit = query_limit<MASK>(p, query, threadIdx.x == 0);
+      n_units = segment_units<A>(limit);
+    }
+    const int seg = static_cast<int>((u - base) / n_units);
+    // [a, e) of the segment's units; a range that begins in the units without tokens begins with the segment, and one that ends
+    // there leaves the segment to the next block
+    const int a0 = static_cast<int>((u - base) - static_cast<long long>(seg) * n_units), a = a0 <= A::SEGMENT_UNITS ? 0 : a0;
+    const int e = static_cast<int>(min(static_cast<long long>(n_units), a0 + (range.u_end - u)));
+    if (e <= A::SEGMENT_UNITS) break;
+    const int h = seg / p.row_tiles, row0 = (seg - h * p.row_tiles) * A::ROWS;
+
+    Segment rows(p, query, h, row0, A::ROWS);
+    {
+      A acc;
+      acc.template walk<CAREFUL>(p, smem, rows, limit, max(0, a - A::SEGMENT_UNITS) * UNIT, min(limit, (e - A::SEGMENT_UNITS) * UNIT));
+    }
+    const bool whole = a == 0 && e == n_units;
+    wild |= finish<A, T, DP>(p, smem, rows, Finish{nullptr, whole ? -1 : static_cast<long long>(blockIdx.x) * 2 + (a == 0 ? 1 : 0)});
+    if (threadIdx.x == 0 && a > 0 && e == n_units) {
+      const long long start = base + static_cast<long long>(seg) * n_units;
+      p.shared_seg[blockIdx.x] = make_int4(static_cast<int>(((start + A::SEGMENT_UNITS + 1) * range.blocks - 1) / range.units), query, h, row0);
+    }
+    u += e - a0;
+    __syncthreads();  // the rings are free for the next segment
+  }
+  return wild;
+}
+// The range once more, with care for infinite values.  A function of its own at the kernel's end, so that the ordinary walk gets its
+// registers as if this one were not there: in one loop with it 64 bytes and more went to memory, and a ragged batch of 32 took 33 us
+// instead of 30.
+template <typename A, typename T, int DP, bool MASK>
+__device__ __noinline__ void attend_range_again(const PagedAttnParams& p, char* smem, Range range) {
+  attend_range<A, T, DP, MASK, true>(p, smem, range);
+}
+
 template <typename T, int DP, bool WIDE, bool MASK, bool SPLIT>
-__global__ void __launch_bounds__(128, PagedAttn<T, DP, WIDE, MASK, SPLIT>::BLOCKS) paged_attention_kernel(const PagedAttnParams p) {
+__global__ void __launch_bounds__(128, PagedAttn<T, DP, WIDE, MASK, SPLIT>::BLOCKS) paged_attention_kernel(const __grid_constant__ PagedAttnParams p) {
   using A = PagedAttn<T, DP, WIDE, MASK, SPLIT>;
   constexpr int UNIT = A::WARPS * A::TT;
   extern __shared__ float4 smem4[];
@@ -832,50 +934,11 @@ __global__ void __launch_bounds__(128, PagedAttn<T, DP, WIDE, MASK, SPLIT>::BLOC
     scan[1] = before;
   }
   __syncthreads();
-  int query = static_cast<int>(scan[0]);
-  long long base = scan[1] * heads;  // first unit of the query
-  int limit = query_limit<MASK>(p, query, threadIdx.x == 0);
-  int n_units = segment_units<A>(limit);
-
-  while (u < u_end) {
-    if (u >= base + static_cast<long long>(n_units) * heads) {
-      base += static_cast<long long>(n_units) * heads;
-      ++query;
-      limit = query_limit<MASK>(p, query, threadIdx.x == 0);
-      n_units = segment_units<A>(limit);
-    }
-    const int seg = static_cast<int>((u - base) / n_units);
-    // [a, e) of the segment's units; a range that begins in the units without tokens begins with the segment, and one that ends
-    // there leaves the segment to the next block
-    const int a0 = static_cast<int>((u - base) - static_cast<long long>(seg) * n_units), a = a0 <= A::SEGMENT_UNITS ? 0 : a0;
-    const int e = static_cast<int>(min(static_cast<long long>(n_units), a0 + (u_end - u)));
-    if (e <= A::SEGMENT_UNITS) break;
-    const int h = seg / p.row_tiles, row0 = (seg - h * p.row_tiles) * A::ROWS;
-
-    A acc;
-    Segment rows(p, query, h, row0, A::ROWS);
-    acc.walk(p, reinterpret_cast<char*>(smem4), rows, limit, max(0, a - A::SEGMENT_UNITS) * UNIT, min(limit, (e - A::SEGMENT_UNITS) * UNIT));
-
-    const bool whole = a == 0 && e == n_units;
-    const long long slot = static_cast<long long>(blockIdx.x) * 2 + (a == 0 ? 1 : 0);
-    for (int x = threadIdx.x; x < A::ROWS * (DP / 4); x += blockDim.x) {
-      const int row = x / (DP / 4), dim = x % (DP / 4) * 4;
-      if (row >= rows.rows || dim >= p.d) continue;
-      float l, m;
-      const float4 s = block_sum<A>(reinterpret_cast<const char*>(smem4), row, dim, l, m);
-      if (whole) {
-        pa_store(static_cast<T*>(p.out) + rows.out_at(p, row) + dim, s, l);
-      } else {
-        *reinterpret_cast<float4*>(p.part_o + (slot * A::ROWS + row) * DP + dim) = s;
-        if (dim == 0) p.part_ml[slot * A::ROWS + row] = make_float2(m, l);
-      }
-    }
-    if (threadIdx.x == 0 && a > 0 && e == n_units) {
-      const long long start = base + static_cast<long long>(seg) * n_units;
-      p.shared_seg[blockIdx.x] = make_int4(static_cast<int>(((start + A::SEGMENT_UNITS + 1) * blocks - 1) / units), query, h, row0);
-    }
-    u += e - a0;
-    __syncthreads();  // the rings are free for the next segment
+  const Range range{u, u_end, scan[1] * heads, units, blocks, static_cast<int>(scan[0])};
+  char* smem = reinterpret_cast<char*>(smem4);
+  const bool wild = attend_range<A, T, DP, MASK, false>(p, smem, range);
+  if constexpr (sizeof(T) == 2) {
+    if (__syncthreads_or(wild)) attend_range_again<A, T, DP, MASK>(p, smem, range);
   }
 }
 
@@ -898,43 +961,32 @@ OSLO_DEVINL float2 peer_load2(uint32_t addr) {
   return r;
 }
 
-// The same attention in one launch, for sequences that cannot be long: a cluster of up to eight blocks takes one segment, each an
-// equal part of its tokens, and joins the parts through distributed shared memory.
-template <typename T, int DP, bool WIDE, bool MASK, bool SPLIT>
-__global__ void __launch_bounds__(128, PagedAttn<T, DP, WIDE, MASK, SPLIT>::BLOCKS) paged_attention_cluster_kernel(const PagedAttnParams p, int cluster) {
-  using A = PagedAttn<T, DP, WIDE, MASK, SPLIT>;
+OSLO_DEVINL void peer_store(uint32_t addr, int x) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(x) : "memory"); }
+
+// A cluster's segment: each block takes an equal part of its tokens, and the parts are joined through distributed shared memory.
+// Sets `wild` of all its blocks where a sum is infinite or not a number.
+template <typename A, typename T, int DP, bool MASK, bool CAREFUL>
+OSLO_DEVINL void attend_cluster(const PagedAttnParams& p, int cluster, char* smem, float2* total, int* wild) {
   constexpr int UNIT = A::WARPS * A::TT;
-  extern __shared__ float4 smem4[];
-  __shared__ float2 total[A::ROWS];
-  char* smem = reinterpret_cast<char*>(smem4);
   const int rank = blockIdx.x % cluster, seg = blockIdx.x / cluster;
   const int heads = p.hkv * p.row_tiles, query = seg / heads, rest = seg - query * heads;
   const int h = rest / p.row_tiles, row0 = (rest - h * p.row_tiles) * A::ROWS;
   const int limit = query_limit<MASK>(p, query, threadIdx.x == 0);
   const int units = (limit + UNIT - 1) / UNIT;
-  A acc;
   Segment part(p, query, h, row0, A::ROWS);
-  acc.walk(p, smem, part, limit, units * rank / cluster * UNIT, min(limit, units * (rank + 1) / cluster * UNIT));
-  T* out = static_cast<T*>(p.out);
-  const int rows = part.rows, quads = p.d / 4;
+  {
+    A acc;
+    acc.template walk<CAREFUL>(p, smem, part, limit, units * rank / cluster * UNIT, min(limit, units * (rank + 1) / cluster * UNIT));
+  }
+  const bool mine = finish<A, T, DP>(p, smem, part, Finish{cluster == 1 ? nullptr : total, -1});
   if (cluster == 1) {
-    for (int x = threadIdx.x; x < rows * quads; x += 128) {
-      const int row = x / quads, dim = (x - row * quads) * 4;
-      float l, m;
-      const float4 s = block_sum<A>(smem, row, dim, l, m);
-      pa_store(out + part.out_at(p, row) + dim, s, l);
-    }
+    if (!CAREFUL && mine) *wild = 1;
     return;
   }
-  // the block's sum replaces its first warp's output, or stays where its warp left it
-  for (int x = threadIdx.x; x < rows * quads; x += 128) {
-    const int row = x / quads, dim = (x - row * quads) * 4;
-    float l, m;
-    const float4 s = block_sum<A>(smem, row, dim, l, m);
-    *reinterpret_cast<float4*>(smem + A::place(row, dim)) = s;
-    if (dim == 0) total[row] = make_float2(m, l);
-  }
   cluster_barrier();
+  T* out = static_cast<T*>(p.out);
+  const int rows = part.rows, quads = p.d / 4;
+  float sums = 0.f;  // 0, or NaN
   for (int x = rank * 128 + threadIdx.x; x < rows * quads; x += cluster * 128) {
     const int row = x / quads, dim = (x - row * quads) * 4;
     const uint32_t at = smem_u32(smem) + static_cast<uint32_t>(A::place(row, dim)), at_total = smem_u32(total + row);
@@ -956,8 +1008,30 @@ __global__ void __launch_bounds__(128, PagedAttn<T, DP, WIDE, MASK, SPLIT>::BLOC
         s.x += y[i].x * w, s.y += y[i].y * w, s.z += y[i].z * w, s.w += y[i].w * w;
       }
     pa_store(out + part.out_at(p, row) + dim, s, l);
+    sums = fmaf(s.x, 0.f, fmaf(s.y, 0.f, fmaf(s.z, 0.f, fmaf(s.w, 0.f, sums))));
   }
+  if (!CAREFUL && sizeof(T) == 2 && sums != 0.f)
+    for (int i = 0; i < cluster; ++i) peer_store(peer_smem(smem_u32(wild), i), 1);
   cluster_barrier();  // a block's shared memory stays until all have read it
+}
+template <typename A, typename T, int DP, bool MASK>
+__device__ __noinline__ void attend_cluster_again(const PagedAttnParams& p, int cluster, char* smem, float2* total) {
+  attend_cluster<A, T, DP, MASK, true>(p, cluster, smem, total, nullptr);
+}
+
+// The same attention in one launch, for sequences that cannot be long: a cluster of up to eight blocks takes one segment.
+template <typename T, int DP, bool WIDE, bool MASK, bool SPLIT>
+__global__ void __launch_bounds__(128, PagedAttn<T, DP, WIDE, MASK, SPLIT>::BLOCKS) paged_attention_cluster_kernel(const __grid_constant__ PagedAttnParams p, int cluster) {
+  using A = PagedAttn<T, DP, WIDE, MASK, SPLIT>;
+  extern __shared__ float4 smem4[];
+  __shared__ float2 total[A::ROWS];
+  __shared__ int wild;
+  if (threadIdx.x == 0) wild = 0;  // every walk has a barrier before its sums are there
+  attend_cluster<A, T, DP, MASK, false>(p, cluster, reinterpret_cast<char*>(smem4), total, &wild);
+  if constexpr (sizeof(T) == 2) {
+    if (cluster == 1) __syncthreads();
+    if (*static_cast<volatile int*>(&wild)) attend_cluster_again<A, T, DP, MASK>(p, cluster, reinterpret_cast<char*>(smem4), total);
+  }
 }
 
 // Joins a segment that several blocks of the first kernel share.  Block (a few rows, last block of the segment); of a row's W warps

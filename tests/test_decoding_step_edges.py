@@ -67,3 +67,45 @@ def test_later_tokens_do_not_show_in_any_block(dev, dtype, form):
     got = OF.paged_attention(q, kp, vp, table, lens)
     assert torch.equal(got[:, : s - 1], want[:, : s - 1])
     assert got[rows, s - 1].isnan().all()
+
+
+@pytest.mark.parametrize("dev,form", [("cpu", FORMS[0]), ("cpu", FORMS[4])] + [pytest.param("cuda", f, marks=gpu) for f in FORMS])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("masked", [False, True])
+def test_a_seen_infinite_value_stays_infinite(dev, dtype, masked, form):
+    """Keys are finite, so every weight is positive: a column with one infinity among the seen values is that infinity, one with both
+    signs or a NaN is NaN, and every other column is what it is without them."""
+    q, kp, vp, table, lens = _form(dev, dtype, form)
+    s, _, hkv, d, page, n, _ = form
+    b = len(n)
+    mask = torch.randn(b, 1, 1, max(n)).to(dev) if masked else None
+    column = torch.zeros(b, s, hkv, d, device=dev)  # what the infinities leave of a column
+    clean = vp.clone()
+    for r in range(b):
+        for t, j, x in ((0, 0, math.inf), (n[r] // 2, 1, -math.inf), (n[r] - 1, 2, math.inf), (2, 3, math.inf), (n[r] - s, 3, -math.inf),
+                        (5, 4, math.nan), (n[r] - 1, 5, -math.inf)):
+            at = int(table[r, t // page]), slice(None), t % page, j
+            vp[at], clean[at] = x, 0.0
+            for i in range(s):
+                if t < n[r] - s + 1 + i:
+                    column[r, i, :, j] += x
+    want = OF.paged_attention(q, kp, clean, table, lens, mask=mask).view(b, s, hkv, -1, d)
+    got = OF.paged_attention(q, kp, vp, table, lens, mask=mask).view(b, s, hkv, -1, d)
+    _sync_status(dev)
+    column = column.unsqueeze(3).expand_as(got)
+    wild = column != 0
+    assert torch.equal(got[wild].float().nan_to_num(nan=7.0, posinf=8.0, neginf=9.0), column[wild].nan_to_num(nan=7.0, posinf=8.0, neginf=9.0))
+    # the same sums in 32 bits, rounded once on either side
+    tol = 2 * (max(n) + 16) * U * vp[vp.isfinite()].abs().max() + 2 * _half_step(dtype) * want.abs().float()
+    assert ((got.float() - want.float()).abs() <= tol)[~wild].all()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_one_token_of_infinities(dev, dtype):
+    q, kp, vp, table, lens = _form(dev, dtype, (1, 4, 2, 64, 16, [1, 1], 0))
+    vp[int(table[0, 0]), :, 0] = math.inf
+    vp[int(table[1, 0]), :, 0, ::2] = -math.inf
+    got = OF.paged_attention(q, kp, vp, table, lens).view(2, 4, 64)
+    assert (got[0] == math.inf).all() and (got[1, :, ::2] == -math.inf).all()
+    assert torch.equal(got[1, :2, 1::2], vp[int(table[1, 0]), 0, 0, 1::2].expand(2, -1))
