@@ -25,8 +25,9 @@
 //            the values of exactly those tokens, 16 bytes at head dim r * E of each 8 E wide block.
 // (Rows of the ring are 16 bytes longer than a head, which keeps the value loads free of bank conflicts.)  tcgen05 would
 // multiply 128 rows where there are 1 to 16: the tensor cores are not what bounds this.
-// The probabilities enter the second product as the sum of two 16-bit numbers (high part and remainder), which keeps 16 bits
-// and more of each.
+// The weights enter the second product as the sum of two 16-bit numbers (high part and remainder): 16 bits of a weight in bf16, 22
+// in fp16.  fp16 ends at 2^-24, so its weights and their sum carry a factor of 2^15, which the last division takes out: a token
+// that weighs 2^-25 of the heaviest keeps 14 bits, and no weight loses more than 2^-22 of itself or 2^-40 of the heaviest.
 #pragma once
 #include "common.cuh"
 
@@ -96,6 +97,7 @@ template <typename T>
 struct Mma16;  // D[16 x 8] += A[16 x 16] B[16 x 8], 16-bit operands
 template <>
 struct Mma16<__nv_bfloat16> {
+  static constexpr float WEIGHT = 1.f;  // of the heaviest token
   static OSLO_DEVINL void run(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -111,6 +113,7 @@ struct Mma16<__nv_bfloat16> {
 };
 template <>
 struct Mma16<__half> {
+  static constexpr float WEIGHT = 32768.f;
   static OSLO_DEVINL void run(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -289,10 +292,10 @@ struct AttnWarp {
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        sc[n][x] = Math::weight(sc[n][x], m0);
+        sc[n][x] = Math::weight(sc[n][x], m0) * Mma16<T>::WEIGHT;
         l0 += sc[n][x];
         if constexpr (WIDE) {
-          sc[n][2 + x] = Math::weight(sc[n][2 + x], m1);
+          sc[n][2 + x] = Math::weight(sc[n][2 + x], m1) * Mma16<T>::WEIGHT;
           l1 += sc[n][2 + x];
         }
       }

@@ -109,3 +109,43 @@ def test_one_token_of_infinities(dev, dtype):
     got = OF.paged_attention(q, kp, vp, table, lens).view(2, 4, 64)
     assert (got[0] == math.inf).all() and (got[1, :, ::2] == -math.inf).all()
     assert torch.equal(got[1, :2, 1::2], vp[int(table[1, 0]), 0, 0, 1::2].expand(2, -1))
+
+
+def _tail_bound(q, k, x, p, v, o, scale, dtype):
+    """As in test_paged_ops.py: sums of d products (2 d u of their magnitudes) and 4 u of a score change a weight by exp(2 e); the
+    exponential 2**-21; two 16-bit parts of a weight 2**-16 (32-bit inputs: none); n weights summed in 32 bits.  Parts of 16-bit
+    floats have steps of 2**-24 of a weight that was scaled by 2**15: a token's weight is off by at most 2**-40, whatever it is."""
+    d, n = q.shape[-1], x.shape[-1]
+    e = (2 * d * U * (q.abs() @ k.abs().T * abs(scale)) + 4 * U * x.abs()).amax(-1, keepdim=True)
+    part = 0.0 if dtype == torch.float32 else 2.0 ** -16
+    pre = (torch.expm1(2 * e) + 2.0 ** -21 + part + 2 * (n + 16) * U) * (p @ v.abs())
+    small = 2.0 ** -39 * v.abs().sum(0) if dtype == torch.float16 else 0.0
+    return _half_step(dtype) * (o.abs() + pre) + pre + small + 2.0 ** -25
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hq,n,batch", [(1, 4001, 1), (4, 131071, 1), (12, 4001, 1), (12, 60000, 1), (40, 4001, 64), (5, 300, 1)])
+@pytest.mark.parametrize("gap", [12.0, 17.0, 20.0])
+@pytest.mark.parametrize("masked", [False, True])
+def test_many_light_tokens_behind_a_heavy_one(dtype, hq, n, batch, gap, masked):
+    """One token's score is `gap` above the others', and its value is zero: the result is what the light tokens give, each of them
+    exp(-gap) of the heavy one."""
+    torch.manual_seed(hq + n)
+    d, page = 64, 64
+    kp, vp, table = _pool([n], page, 1, d, dtype, "cuda")
+    q = torch.randn(1, 1, 1, d).sign().expand(batch, 1, hq, d).to(dtype).cuda()
+    kp.mul_(0.0)
+    vp.abs_().mul_(1000.0 if n < 10000 else 100.0)
+    heavy = int(table[0, 0]), 0, 3
+    kp[heavy], vp[heavy] = (q[0, 0, 0].float() * gap / 8).to(dtype), 0.0  # q k = 64 gap / 8, scaled by 1 / 8
+    mask = torch.zeros(1, 1, 1, n, device="cuda") if masked else None
+    got = OF.paged_attention(q, kp, vp, table.expand(batch, -1).contiguous(), torch.full((batch,), n, device="cuda", **I32), mask=mask)
+    _sync_status("cuda")
+    k, v = _seq(kp, table, 0, n)[:, 0].double(), _seq(vp, table, 0, n)[:, 0].double()
+    x = q[0, 0].double() @ k.T / 8
+    p = torch.softmax(x, -1)
+    want = p @ v
+    off = (got.view(batch, hq, d).double() - want).abs()
+    tol = _tail_bound(q[0, 0].double(), k, x, p, v, want, 1 / 8, dtype)
+    assert (off <= tol).all(), (off / tol).max().item()
