@@ -40,7 +40,7 @@ struct PagedAttnParams {
   const void* q;
   const void* k;
   const void* v;
-  const float* mask;  // additive, [b, s, mask_len] by strides; null: none
+  const float* mask;  // additive, [b, s, mask_len] by strides; mask_len < 0: none
   void* out;          // [b, s, hq, d] contiguous
   const int* table;
   const int* lens;
@@ -1219,7 +1219,7 @@ int paged_attention_mask(PagedAttnParams& p, int block_rows, PagedAttnPlan& plan
 }
 template <typename T, int DP>
 int paged_attention_dp(PagedAttnParams& p, int block_rows, PagedAttnPlan& plan, bool run, void* ws, cudaStream_t st) {
-  return p.mask ? paged_attention_mask<T, DP, true>(p, block_rows, plan, run, ws, st) : paged_attention_mask<T, DP, false>(p, block_rows, plan, run, ws, st);
+  return p.mask_len >= 0 ? paged_attention_mask<T, DP, true>(p, block_rows, plan, run, ws, st) : paged_attention_mask<T, DP, false>(p, block_rows, plan, run, ws, st);
 }
 template <typename T>
 int paged_attention_type(PagedAttnParams& p, int block_rows, PagedAttnPlan& plan, bool run, void* ws, cudaStream_t st) {

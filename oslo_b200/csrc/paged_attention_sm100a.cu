@@ -15,7 +15,7 @@ static bool paged_attention_params(const OsloPagedAttentionArgs* a, oslo::PagedA
   if (a->hkv <= 0 || a->group <= 0 || a->d <= 0 || a->d > 256 || a->d % 8 || a->page_size <= 0 || a->page_size % 16) return false;
   if (a->b > 0x3fffffff || a->s > 0x3fffffff || a->group > 0x3fffffff || a->s * a->group > 0x3fffffff) return false;
   if (a->hkv > 0x3fffffff || a->b * a->hkv > 0x3fffffff) return false;
-  const bool together = a->mask == 0 || a->mask_s == 0;  // the query tokens of a sequence share what they see but for the last ones
+  const bool together = a->mask_len < 0 || a->mask_s == 0;  // the query tokens of a sequence share what they see but for the last ones
   const long long rows = together ? a->s * a->group : a->group, groups = a->b * a->hkv * (together ? 1 : a->s);
   const long long most = oslo::paged_attention_rows(a->dtype, a->d, rows, groups),
                   tiles = (rows + most - 1) / most;

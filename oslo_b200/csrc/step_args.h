@@ -11,9 +11,9 @@ struct OsloPagedAppendArgs {
 };
 
 struct OsloPagedAttentionArgs {
-  long long q, k_pages, v_pages, table, lens, mask, out, workspace, status, stream;  // mask may be 0
+  long long q, k_pages, v_pages, table, lens, mask, out, workspace, status, stream;
   long long q_b, q_s, q_h, k_page, k_head, v_page, v_head, table_row, mask_b, mask_s;
-  long long b, s, hkv, group, d, page_size, max_pages, num_pages, mask_len, dtype;
+  long long b, s, hkv, group, d, page_size, max_pages, num_pages, mask_len, dtype;  // mask_len < 0: no mask (an empty one has no address)
   double scale;
 };
 

@@ -147,6 +147,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (hq == 0 || hq % hkv || !plain(*q, recording) || !plain(*kp, recording) || !plain(*vp, recording) || !aligned(*q, 16 / q->element_size()))
     return other();
   OsloPagedAttentionArgs x{};
+  x.mask_len = -1;
   x.scale = 1.0 / std::sqrt(static_cast<double>(d));
   if (a.has(5)) {
     if (!PyFloat_Check(args[5])) return other();
@@ -156,7 +157,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (a.has(6)) {
     const Tensor* m = a.tensor(6);
     if (!m || m->scalar_type() != at::kFloat || m->dim() != 4 || (m->size(0) != b && m->size(0) != 1) || m->size(1) != 1 ||
-        (m->size(2) != s && m->size(2) != 1) || m->size(3) == 0 || m->stride(3) != 1 || !on(*m, device) || !plain(*m, recording))
+        (m->size(2) != s && m->size(2) != 1) || m->stride(3) != 1 || !on(*m, device) || !plain(*m, recording))
       return other();
     x.mask = address(*m), x.mask_b = m->size(0) == 1 ? 0 : m->stride(0), x.mask_s = m->size(2) == 1 ? 0 : m->stride(2), x.mask_len = m->size(3);
   }

@@ -196,7 +196,8 @@ def paged_attention(q, k_pages, v_pages, block_table, lengths, scale: Optional[f
             return paged_attention(q, k_pages, v_pages, block_table, lengths, scale, mask)
     q, qs, qp = _aligned(q)
     out = q.new_empty((b, s, hq * hd))
-    mptr = mb = mt = mlen = 0
+    mptr = mb = mt = 0
+    mlen = -1
     if mask is not None:
         mlen = mask.shape[3]
         mask = mask.expand(b, 1, s, mlen)

@@ -149,3 +149,25 @@ def test_many_light_tokens_behind_a_heavy_one(dtype, hq, n, batch, gap, masked):
     off = (got.view(batch, hq, d).double() - want).abs()
     tol = _tail_bound(q[0, 0].double(), k, x, p, v, want, 1 / 8, dtype)
     assert (off <= tol).all(), (off / tol).max().item()
+
+
+# ------------------------------------------------------------------------------------------------ arguments without elements
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_mask_without_tokens_is_a_short_mask(dev, dtype):
+    q, kp, vp, table, lens = _form(dev, dtype, (1, 6, 2, 64, 16, [20, 3], 0))
+    for rows in (1, 2):
+        m = torch.zeros(rows, 1, 1, 0, device=dev)
+        if dev == "cpu":
+            with pytest.raises(ValueError, match="mask"):
+                OF.paged_attention(q, kp, vp, table, lens, mask=m)
+        else:
+            from oslo_b200.ops import _lib
+
+            got = OF.paged_attention(q, kp, vp, table, lens, mask=m)
+            torch.cuda.synchronize()
+            with pytest.raises(RuntimeError, match="paged cache"):
+                _lib.check_status()
+            assert (got == 0).all()
+        assert (OF.paged_attention(q, kp, vp, table, torch.zeros_like(lens), mask=m) == 0).all()  # nothing to cover
+        _sync_status(dev)
