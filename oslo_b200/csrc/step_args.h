@@ -5,9 +5,9 @@
 extern "C" {
 
 struct OsloPagedAppendArgs {
-  long long q, k, v, q_out, k_pages, v_pages, table, start, count, cosb, sinb, status, stream;  // q, count, cosb and sinb may be 0
+  long long q, k, v, q_out, k_pages, v_pages, table, start, count, cosb, sinb, status, stream;  // q and count may be 0
   long long q_b, q_s, q_h, k_b, k_s, k_h, v_b, v_s, v_h, k_page, k_head, v_page, v_head, table_row;
-  long long b, s, hq, hkv, d, rot, neox, positions, page_size, max_pages, num_pages, dtype;
+  long long b, s, hq, hkv, d, rot, neox, positions, page_size, max_pages, num_pages, dtype;  // rot = 0: no rotation
 };
 
 struct OsloPagedAttentionArgs {

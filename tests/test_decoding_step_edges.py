@@ -171,3 +171,25 @@ def test_a_mask_without_tokens_is_a_short_mask(dev, dtype):
             assert (got == 0).all()
         assert (OF.paged_attention(q, kp, vp, table, torch.zeros_like(lens), mask=m) == 0).all()  # nothing to cover
         _sync_status(dev)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("neox", [False, True])
+def test_rotation_tables_without_positions_are_short_tables(dev, neox):
+    q, kp, vp, table, lens = _form(dev, torch.bfloat16, (1, 6, 2, 64, 16, [20, 3], 0))
+    k, v = (torch.randn(2, 1, 2, 64).bfloat16().to(dev) for _ in range(2))
+    none = torch.zeros(0, 32, device=dev)
+    before = kp.clone(), vp.clone()
+    call = lambda: OF.paged_kv_append(k, v, kp, vp, table, torch.zeros_like(lens), q=q, rope=(none, none, 64, neox))
+    if dev == "cpu":
+        with pytest.raises(ValueError, match="rotation"):
+            call()
+    else:
+        from oslo_b200.ops import _lib
+
+        out = call()
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="paged cache"):
+            _lib.check_status()
+        assert (out == 0).all()
+    assert torch.equal(kp, before[0]) and torch.equal(vp, before[1])
