@@ -152,7 +152,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (a.has(5)) {
     if (!PyFloat_Check(args[5])) return other();
     x.scale = PyFloat_AS_DOUBLE(args[5]);
-    if (!std::isfinite(x.scale)) return other();
+    if (!(std::abs(x.scale) <= 0x1p127)) return other();
   }
   if (a.has(6)) {
     const Tensor* m = a.tensor(6);

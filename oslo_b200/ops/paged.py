@@ -27,6 +27,7 @@ _DT = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # of a device's current stream
 _device = getattr(torch._C, "_cuda_getDevice", None)
 MAX_HEAD_DIM = 256
+MAX_SCALE = 2.0 ** 127  # times log2(e) it still is a 32-bit number
 _INFERENCE = "the paged cache is for inference: call it under torch.no_grad() or detach its inputs"
 
 
@@ -162,6 +163,7 @@ def paged_attention(q, k_pages, v_pages, block_table, lengths, scale: Optional[f
     ``lengths[b] - s + 1 + i``.  ``heads`` is a multiple of the pages' ``kv_heads``; consecutive heads share one.
     ``mask``: additive, ``[b or 1, 1, s or 1, tokens]``, any floating type; tokens at ``-inf`` take no part, whatever they hold,
     nor does what lies behind a sequence's last token.  It covers the longest sequence.  A query that sees nothing gives zeros.
+    ``scale``: up to ``2**127`` (default ``head_dim ** -0.5``).
 
     Returns ``[b, s, heads * head_dim]``, like :func:`oslo_b200.ops.attention.attention`.
     """
@@ -181,8 +183,8 @@ def paged_attention(q, k_pages, v_pages, block_table, lengths, scale: Optional[f
     if hq == 0 or group * hkv != hq:
         raise ValueError(f"{hq} query heads do not share {hkv} key heads evenly")
     scale = hd ** -0.5 if scale is None else float(scale)
-    if not math.isfinite(scale):
-        raise ValueError(f"scale is a finite number: got {scale}")
+    if not abs(scale) <= MAX_SCALE:
+        raise ValueError(f"scale is a number up to {MAX_SCALE:g}: got {scale}")
     if mask is not None:
         if mask.dim() != 4 or mask.shape[0] not in (1, b) or mask.shape[1] != 1 or mask.shape[2] not in (1, s) \
                 or mask.get_device() != dev or not mask.is_floating_point():

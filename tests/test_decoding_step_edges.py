@@ -193,3 +193,12 @@ def test_rotation_tables_without_positions_are_short_tables(dev, neox):
             _lib.check_status()
         assert (out == 0).all()
     assert torch.equal(kp, before[0]) and torch.equal(vp, before[1])
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_a_scale_that_32_bits_do_not_hold_is_refused(dev):
+    q, kp, vp, table, lens = _form(dev, torch.float32, (1, 6, 2, 64, 16, [20, 3], 0))
+    OF.paged_attention(q, kp, vp, table, lens)
+    for scale in (1e39, -1e300, 3e38, math.inf, math.nan):
+        with pytest.raises(ValueError, match="scale"):
+            OF.paged_attention(q, kp, vp, table, lens, scale=scale)
