@@ -87,6 +87,14 @@ def _grad(*tensors):
     return False
 
 
+def _mask32(mask):
+    """``mask`` in 32 bits; finite numbers stay finite: the lowest one of 64 bits hides nothing, as that of 32 bits does not."""
+    if mask.dtype == torch.float64:
+        most = torch.finfo(torch.float32).max
+        mask = torch.where(mask.isfinite(), mask.clamp(-most, most), mask)
+    return mask.float()
+
+
 def _aligned(t):
     """``t`` with unit inner stride and 16-byte aligned heads (a copy where it has not), its strides and its address."""
     st, at = t.stride(), t.data_ptr()
@@ -190,7 +198,7 @@ def paged_attention(q, k_pages, v_pages, block_table, lengths, scale: Optional[f
                 or mask.get_device() != dev or not mask.is_floating_point():
             raise ValueError(f"mask is an additive floating tensor [{b} or 1, 1, {s} or 1, tokens] beside q: got {mask.dtype} "
                              f"{tuple(mask.shape)} on {mask.device}")
-        mask = mask.float()
+        mask = _mask32(mask)
     if not q.is_cuda:
         return _attention_reference(q, k_pages, v_pages, block_table, lengths, scale, mask)
     if dev != _device():

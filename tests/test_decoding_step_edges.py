@@ -202,3 +202,19 @@ def test_a_scale_that_32_bits_do_not_hold_is_refused(dev):
     for scale in (1e39, -1e300, 3e38, math.inf, math.nan):
         with pytest.raises(ValueError, match="scale"):
             OF.paged_attention(q, kp, vp, table, lens, scale=scale)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_the_lowest_value_of_64_bits_is_not_minus_infinity(dev):
+    """A mask of 64 bits at its type's lowest value: every token is there and weighs the same.  At -inf none is."""
+    q, kp, vp, table, lens = _form(dev, torch.float32, (1, 6, 2, 64, 16, [20, 3], 0))
+    for low in (torch.finfo(torch.float64).min, -1e39):
+        m = torch.full((2, 1, 1, 20), low, dtype=torch.float64, device=dev)
+        m[1, ..., 1] = -math.inf
+        got = OF.paged_attention(q, kp, vp, table, lens, mask=m).view(2, 2, 3, 64)
+        a, b = _seq(vp, table, 0, 20), _seq(vp, table, 1, 3)[[0, 2]]
+        for r, v in ((0, a), (1, b)):  # a mean of n values: n sums and a division, n + 2 roundings
+            tol = (v.shape[0] + 2) * U * v.abs().mean(0)[:, None] + 2.0 ** -21 * v.abs().mean(0)[:, None]
+            assert ((got[r] - v.mean(0)[:, None]).abs() <= tol).all()
+        m[:] = -math.inf
+        assert (OF.paged_attention(q, kp, vp, table, lens, mask=m) == 0).all()
