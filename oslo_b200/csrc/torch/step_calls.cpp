@@ -36,8 +36,10 @@ PyObject* other() { Py_RETURN_NOTIMPLEMENTED; }
 int type_code(at::ScalarType t) { return t == at::kFloat ? 0 : t == at::kHalf ? 1 : t == at::kBFloat16 ? 2 : -1; }
 int64_t address(const Tensor& t) { return reinterpret_cast<int64_t>(t.data_ptr()); }
 bool on(const Tensor& t, int device) { return t.is_cuda() && t.get_device() == device; }
-// strided storage that records no gradient
-bool plain(const Tensor& t, bool recording) { return t.layout() == at::kStrided && !(recording && t.requires_grad()) && !t.is_neg(); }
+// strided storage without a gradient that would be recorded or a forward derivative
+bool plain(const Tensor& t, bool recording) {
+  return t.layout() == at::kStrided && !(recording && t.requires_grad()) && !t._fw_grad(0).defined() && !t.is_neg();
+}
 
 struct Args {
   PyObject* const* args;
@@ -114,7 +116,7 @@ PyObject* paged_kv_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
     }
     if (rot <= 0 || rot % 2 || rot > d || cosb.dim() != 2 || cosb.size(1) != rot / 2 || sinb.sizes() != cosb.sizes()) return other();
     for (const Tensor* t : {&cosb, &sinb})
-      if (t->scalar_type() != at::kFloat || !t->is_contiguous() || !on(*t, device)) return other();
+      if (t->scalar_type() != at::kFloat || !t->is_contiguous() || !on(*t, device) || !plain(*t, recording)) return other();
     x.cosb = address(cosb), x.sinb = address(sinb), x.rot = rot, x.neox = neox, x.positions = cosb.size(0);
   }
   Tensor out;
@@ -178,13 +180,13 @@ PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 // one number a row, or a number for all of them
-bool penalty(const Args& a, int i, int64_t rows, int device, long long& where, double& number) {
+bool penalty(const Args& a, int i, int64_t rows, int device, bool recording, long long& where, double& number) {
   if (PyFloat_Check(a.args[i])) {
     number = PyFloat_AS_DOUBLE(a.args[i]);
     return true;
   }
   const Tensor* t = a.tensor(i);
-  if (!t || t->scalar_type() != at::kFloat || t->dim() != 1 || t->size(0) != rows || !t->is_contiguous() || !on(*t, device)) return false;
+  if (!t || t->scalar_type() != at::kFloat || t->dim() != 1 || t->size(0) != rows || !t->is_contiguous() || !on(*t, device) || !plain(*t, recording)) return false;
   where = address(*t);
   return true;
 }
@@ -203,8 +205,8 @@ PyObject* process_logits(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const int64_t rows = x->size(0), vocab = x->size(1);
   if (code < 0 || !plain(*x, recording) || x->stride(1) != 1) return other();
   OsloProcessLogitsArgs y{};
-  if (!penalty(a, 4, rows, device, y.rep, y.rep_s) || !penalty(a, 5, rows, device, y.pres, y.pres_s) ||
-      !penalty(a, 6, rows, device, y.freq, y.freq_s) || (!y.rep && !(y.rep_s > 0)))
+  if (!penalty(a, 4, rows, device, recording, y.rep, y.rep_s) || !penalty(a, 5, rows, device, recording, y.pres, y.pres_s) ||
+      !penalty(a, 6, rows, device, recording, y.freq, y.freq_s) || (!y.rep && !(y.rep_s > 0)))
     return other();
   if (a.has(1)) {
     const Tensor* t = a.tensor(1);

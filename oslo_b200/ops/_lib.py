@@ -112,6 +112,15 @@ def has_cuda_kernels() -> bool:
     return torch.cuda.is_available()
 
 
+def carries_gradient(*tensors) -> bool:
+    """Whether autograd would record a use of any of the tensors (``None`` among them is skipped), or one has a forward derivative."""
+    recording, level = torch.is_grad_enabled(), torch.autograd.forward_ad._current_level
+    for t in tensors:
+        if t is not None and ((recording and t.requires_grad) or (level >= 0 and torch.autograd.forward_ad.unpack_dual(t).tangent is not None)):
+            return True
+    return False
+
+
 def ptr(t) -> ctypes.c_void_p:
     return ctypes.c_void_p(0 if t is None else t.data_ptr())
 

@@ -55,7 +55,8 @@ def process_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     ``[rows]``, how many of them count (``None``: all).  ``prompt_lengths``: int32 ``[rows]``, how many of those are the prompt, not
     generated (``None``: none).  The penalties are numbers or floating tensors ``[rows]``.  ``bias``: ``[vocab]`` or ``[rows, vocab]``.
     ``allowed``: int32 ``[rows or 1, ceil(vocab / 32)]`` from :func:`pack_token_mask`; a row that allows nothing is all ``-inf``.
-    The result is a new tensor, or ``out`` (which may be ``logits``).  For inference: no gradient.
+    The result is a new tensor, or ``out`` (which may be ``logits``).  For inference: tensors that require a gradient or carry a
+    forward derivative are refused.
     """
     if logits.is_cuda and out is None:
         y = _step(logits, tokens, token_lengths, prompt_lengths, repetition_penalty, presence_penalty, frequency_penalty, bias, allowed)
@@ -64,7 +65,8 @@ def process_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     dtype, dev = logits.dtype, logits.device
     if logits.dim() != 2 or dtype not in _DT:
         raise ValueError(f"logits are float32, float16 or bfloat16 [rows, vocab]: got {dtype} {tuple(logits.shape)}")
-    if torch.is_grad_enabled() and (logits.requires_grad or (bias is not None and bias.requires_grad)):
+    if _lib.carries_gradient(*(t for t in (logits, bias, repetition_penalty, presence_penalty, frequency_penalty, out)
+                               if isinstance(t, torch.Tensor))):
         raise RuntimeError("process_logits is for inference: call it under torch.no_grad() or detach its inputs")
     rows, v = logits.shape
     rep, rep_s = _per_row("repetition_penalty", repetition_penalty, rows, dev)

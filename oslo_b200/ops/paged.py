@@ -8,7 +8,7 @@ Keys and values live in pools ``[pages, kv_heads, page_size, head_dim]``; ``bloc
 ``PagedDecodeCache``  the paged counterpart of :class:`oslo_b200.ops.attention.DecodeCache`: pages are taken from a free list as
                       sequences grow, and the sequences of a batch may have different lengths
 
-The functions are for inference: inputs that require a gradient are refused.  On the GPU a page, position or length outside
+The functions are for inference: inputs that require a gradient or carry a forward derivative are refused.  On the GPU a page, position or length outside
 its pool or table is skipped by the kernel and reported by ``oslo_b200.ops._lib.check_status()``; on the CPU it raises.
 """
 from __future__ import annotations
@@ -80,13 +80,6 @@ def _check_rope(rope, hd: int, device: int):
     return cos, sin, rot, 1 if neox else 0, shape[0]
 
 
-def _grad(*tensors):
-    for t in tensors:
-        if t is not None and t.requires_grad:
-            return True
-    return False
-
-
 def _mask32(mask):
     """``mask`` in 32 bits; finite numbers stay finite: the lowest one of 64 bits hides nothing, as that of 32 bits does not."""
     if mask.dtype == torch.float64:
@@ -125,8 +118,6 @@ def paged_kv_append(k, v, k_pages, v_pages, block_table, start, count=None, q=No
         raise ValueError(f"k and v are [b, s, kv_heads, head_dim], both alike: got {tuple(shape)} {dtype} and {tuple(v.shape)} "
                          f"{v.dtype}")
     b, s, hkv, hd = shape
-    if torch.is_grad_enabled() and _grad(k, v, q, k_pages, v_pages):
-        raise RuntimeError(_INFERENCE)
     pages, heads, page, width, row, kps, vps, kp, vp = _check_pages(k_pages, v_pages, block_table, b, hd, dtype, dev)
     if heads != hkv:
         raise ValueError(f"the pages hold {heads} key heads, the tokens {hkv}")
@@ -140,6 +131,8 @@ def paged_kv_append(k, v, k_pages, v_pages, block_table, start, count=None, q=No
             raise ValueError(f"q is [{b}, {s}, heads, {hd}] {dtype} beside k: got {tuple(qshape)} {q.dtype} on {q.device}")
         hq = qshape[2]
     cos, sin, rot, neox, positions = _check_rope(rope, hd, dev) if rope is not None else (None, None, 0, 1, 0)
+    if _lib.carries_gradient(k, v, q, k_pages, v_pages, cos, sin):
+        raise RuntimeError(_INFERENCE)
     if not k.is_cuda:
         return _append_reference(k, v, k_pages, v_pages, block_table, start, count, q, rope if rot else None)
     if dev != _device():
@@ -183,7 +176,7 @@ def paged_attention(q, k_pages, v_pages, block_table, lengths, scale: Optional[f
     if len(shape) != 4:
         raise ValueError(f"q is [b, s, heads, head_dim]: got {tuple(shape)}")
     b, s, hq, hd = shape
-    if torch.is_grad_enabled() and _grad(q, k_pages, v_pages, mask):
+    if _lib.carries_gradient(q, k_pages, v_pages, mask):
         raise RuntimeError(_INFERENCE)
     pages, hkv, page, width, row, ks, vs, kp, vp = _check_pages(k_pages, v_pages, block_table, b, hd, dtype, dev)
     _check_ints("lengths", lengths, b, dev)

@@ -218,3 +218,48 @@ def test_the_lowest_value_of_64_bits_is_not_minus_infinity(dev):
             assert ((got[r] - v.mean(0)[:, None]).abs() <= tol).all()
         m[:] = -math.inf
         assert (OF.paged_attention(q, kp, vp, table, lens, mask=m) == 0).all()
+
+
+# ------------------------------------------------------------------------------------------------ no gradient is lost silently
+@pytest.mark.parametrize("dev", DEVICES)
+def test_inputs_that_carry_a_gradient_are_refused(dev):
+    from torch.autograd import forward_ad as fwd
+
+    q, kp, vp, table, lens = _form(dev, torch.float32, (1, 6, 2, 64, 16, [20, 3], 0))
+    k, v = (torch.randn(2, 1, 2, 64, device=dev) for _ in range(2))
+    cos, sin = OF.rope_tables(64, 64, device=dev)
+    m = torch.zeros(2, 1, 1, 20, device=dev)
+    x, tokens = torch.randn(2, 50, device=dev), torch.zeros(2, 4, dtype=torch.int64, device=dev)
+    one = torch.ones(2, device=dev)
+    append = dict(k=k, v=v, k_pages=kp, v_pages=vp, block_table=table, start=lens - 1, q=q)
+    attend = dict(q=q, k_pages=kp, v_pages=vp, block_table=table, lengths=lens, mask=m)
+    logits = dict(logits=x, tokens=tokens, repetition_penalty=one, presence_penalty=one, frequency_penalty=one, bias=torch.zeros(50, device=dev))
+    OF.paged_kv_append(**append, rope=(cos, sin, 64, True))
+    OF.paged_attention(**attend)
+    OF.process_logits(**logits)
+    calls = [(OF.paged_kv_append, append, n) for n in ("k", "v", "q", "k_pages", "v_pages")]
+    calls += [(OF.paged_attention, attend, n) for n in ("q", "k_pages", "v_pages", "mask")]
+    calls += [(OF.process_logits, logits, n) for n in ("logits", "bias", "repetition_penalty", "presence_penalty", "frequency_penalty")]
+    for f, good, name in calls:
+        with pytest.raises(RuntimeError, match="inference"):
+            f(**{**good, name: good[name].clone().requires_grad_()})
+        with torch.no_grad():  # nothing is recorded
+            f(**{**good, name: good[name].clone().requires_grad_()})
+        with fwd.dual_level():
+            dual = fwd.make_dual(good[name].clone(), torch.ones_like(good[name]))
+            for grad in (True, False):  # forward derivatives do not hang on the recording of backward ones
+                with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="inference"):
+                    f(**{**good, name: dual})
+    for i in range(2):
+        tables = [cos, sin]
+        tables[i] = tables[i].clone().requires_grad_()
+        with pytest.raises(RuntimeError, match="inference"):
+            OF.paged_kv_append(**append, rope=(*tables, 64, True))
+        with fwd.dual_level():
+            tables[i] = fwd.make_dual(tables[i].detach(), torch.ones_like(cos))
+            with pytest.raises(RuntimeError, match="inference"):
+                OF.paged_kv_append(**append, rope=(*tables, 64, True))
+    out = torch.empty_like(x).requires_grad_()
+    with pytest.raises(RuntimeError, match="inference"):
+        OF.process_logits(x, out=out)
+    _sync_status(dev)
