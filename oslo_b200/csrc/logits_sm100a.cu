@@ -57,7 +57,10 @@ OSLO_DEVINL void lg_st(__nv_bfloat16& p, float x) { p = __float2bfloat16_rn(x); 
 template <typename C>
 struct LogitsRow {
   float rep, inv, pres, freq;
-  OSLO_DEVINL float operator()(float f, unsigned seen) const {  // without branches: some lane of a warp has a seen token nearly always
+  // x / r is x times the reciprocal, both rounded to 32 bits: off by 2^-23 of the quotient at most, where a division is by 2^-24
+  // (192 x 250112 bf16 with every option: 58 us, with a division 70 us under a branch and 74 us
+  // without).  No branches here: some lane of a warp has a seen token nearly always.
+  OSLO_DEVINL float operator()(float f, unsigned seen) const {
     const unsigned c = seen & ~Counter<C>::kPrompt;
     const float r = f * (f > 0.f ? inv : rep);
     f = seen ? r : f;

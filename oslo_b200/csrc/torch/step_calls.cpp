@@ -206,7 +206,7 @@ PyObject* process_logits(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (code < 0 || !plain(*x, recording) || x->stride(1) != 1) return other();
   OsloProcessLogitsArgs y{};
   if (!penalty(a, 4, rows, device, recording, y.rep, y.rep_s) || !penalty(a, 5, rows, device, recording, y.pres, y.pres_s) ||
-      !penalty(a, 6, rows, device, recording, y.freq, y.freq_s) || (!y.rep && !(y.rep_s > 0)))
+      !penalty(a, 6, rows, device, recording, y.freq, y.freq_s) || (!y.rep && !(y.rep_s >= 0x1p-126 && y.rep_s <= 0x1p126)))
     return other();
   if (a.has(1)) {
     const Tensor* t = a.tensor(1);

@@ -14,6 +14,7 @@ import torch
 from . import _lib
 
 _DT = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+MAX_REPETITION = 2.0 ** 126  # its reciprocal still is a normal 32-bit number, and the other way round
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # of a device's current stream
 _device = getattr(torch._C, "_cuda_getDevice", None)
 
@@ -53,7 +54,8 @@ def process_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
 
     ``tokens``: int64 or int32 ``[rows, length]``, the history; ids outside the vocabulary are ignored.  ``token_lengths``: int32
     ``[rows]``, how many of them count (``None``: all).  ``prompt_lengths``: int32 ``[rows]``, how many of those are the prompt, not
-    generated (``None``: none).  The penalties are numbers or floating tensors ``[rows]``.  ``bias``: ``[vocab]`` or ``[rows, vocab]``.
+    generated (``None``: none).  The penalties are numbers or floating tensors ``[rows]``, ``repetition_penalty`` from ``2**-126`` to
+    ``2**126``.  ``bias``: ``[vocab]`` or ``[rows, vocab]``.
     ``allowed``: int32 ``[rows or 1, ceil(vocab / 32)]`` from :func:`pack_token_mask`; a row that allows nothing is all ``-inf``.
     The result is a new tensor, or ``out`` (which may be ``logits``).  For inference: tensors that require a gradient or carry a
     forward derivative are refused.
@@ -72,8 +74,8 @@ def process_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
     rep, rep_s = _per_row("repetition_penalty", repetition_penalty, rows, dev)
     pres, pres_s = _per_row("presence_penalty", presence_penalty, rows, dev)
     freq, freq_s = _per_row("frequency_penalty", frequency_penalty, rows, dev)
-    if rep is None and not rep_s > 0:
-        raise ValueError(f"repetition_penalty is positive: got {rep_s}")
+    if rep is None and not 1 / MAX_REPETITION <= rep_s <= MAX_REPETITION:
+        raise ValueError(f"repetition_penalty is positive, from 1 / {MAX_REPETITION:g} to {MAX_REPETITION:g}: got {rep_s}")
     if tokens is None:
         if token_lengths is not None or prompt_lengths is not None:
             raise ValueError("token_lengths and prompt_lengths describe tokens, which are missing")

@@ -263,3 +263,35 @@ def test_inputs_that_carry_a_gradient_are_refused(dev):
     with pytest.raises(RuntimeError, match="inference"):
         OF.process_logits(x, out=out)
     _sync_status(dev)
+
+
+# ------------------------------------------------------------------------------------------------ logits
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("v,t", [(1000, 3000), (1000, 40000), (70001, 9000)])
+def test_the_repetition_penalty_divides(dev, dtype, v, t):
+    """A quotient (a reciprocal and a product: two roundings to 32 bits) or a product (one), then one rounding to the logits' type."""
+    torch.manual_seed(v)
+    rep = torch.tensor([1.3, 1.1, 0.7, 3.0, 2.0 ** 126], device=dev)
+    x = (3 * torch.randn(5, v, device=dev)).to(dtype)
+    x[4] = (x[4].float() * (1e37 if dtype != torch.float16 else 1.0)).to(dtype)
+    tokens = torch.randint(0, v, (5, t), device=dev)
+    got = OF.process_logits(x, tokens, repetition_penalty=rep)
+    seen = torch.zeros(5, v, dtype=torch.bool, device=dev).scatter_(1, tokens, True)
+    x64, r64 = x.double(), rep.double()[:, None]
+    want = torch.where(x64 > 0, x64 / r64, x64 * r64)
+    normal = (want.abs() >= torch.finfo(dtype).tiny) & (want.abs() < torch.finfo(dtype).max)
+    pre = 2 * U * (1 + U) * want.abs()
+    tol = pre + _half_step(dtype) * (want.abs() + pre)
+    assert ((got.double() - want).abs() <= tol)[seen & normal].all()
+    assert torch.equal(got[~seen], x[~seen])
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_repetition_penalties_without_a_reciprocal_are_refused(dev):
+    x, tokens = torch.full((1, 8), 1e38, device=dev), torch.arange(8, device=dev)[None]
+    for rep in (2e38, 1e39, math.inf, 1e-38, 1e-45, 0.0):
+        with pytest.raises(ValueError, match="repetition_penalty"):
+            OF.process_logits(x, tokens, repetition_penalty=rep)
+    got = OF.process_logits(x, tokens, repetition_penalty=2.0 ** 126)  # a power of two: exact
+    assert torch.equal(got, (x.double() / 2.0 ** 126).float())
