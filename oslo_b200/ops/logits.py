@@ -39,6 +39,21 @@ def _per_row(name, p, rows: int, device):
     return None, float(p)
 
 
+def _partly_over(out, x) -> bool:
+    """Whether rows of ``out`` lie over rows of ``x`` without being the same rows (``x`` whose rows are not contiguous is copied)."""
+    rows, v = x.shape
+    a, b = out.data_ptr(), x.data_ptr()
+    if rows * v == 0 or (v > 1 and x.stride(1) != 1) or (a == b and (rows == 1 or out.stride(0) == x.stride(0))):
+        return False
+    size = x.element_size()
+    row, so, sx = v * size, out.stride(0) * size, x.stride(0) * size
+    if a + (rows - 1) * so + row <= b or b + (rows - 1) * sx + row <= a:
+        return False
+    mine, theirs = a + torch.arange(rows, device="cpu") * so, b + torch.arange(rows, device="cpu") * sx
+    near = torch.searchsorted(theirs, mine - row, right=True).clamp(max=rows - 1)  # the first that ends behind the row's beginning
+    return bool(((theirs[near] > mine - row) & (theirs[near] < mine + row)).any())
+
+
 def process_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, token_lengths: Optional[torch.Tensor] = None,
                    prompt_lengths: Optional[torch.Tensor] = None, repetition_penalty: Union[float, torch.Tensor] = 1.0,
                    presence_penalty: Union[float, torch.Tensor] = 0.0, frequency_penalty: Union[float, torch.Tensor] = 0.0,
@@ -99,6 +114,8 @@ def process_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None, 
                          f"{allowed.device}")
     if out is not None and (out.shape != logits.shape or out.dtype != logits.dtype or out.device != dev or out.stride(1) != 1):
         raise ValueError(f"out is like the logits, with contiguous rows: got {out.dtype} {tuple(out.shape)} on {out.device}")
+    if out is not None and ((rows > 1 and out.stride(0) < v) or _partly_over(out, logits)):
+        raise ValueError("out has rows of its own, and is the logits or apart from them")
     if not logits.is_cuda:
         y = _reference(logits, tokens, token_lengths, prompt_lengths, *(t if t is not None else s for t, s in
                        ((rep, rep_s), (pres, pres_s), (freq, freq_s))), bias, allowed)

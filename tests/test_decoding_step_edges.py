@@ -295,3 +295,32 @@ def test_repetition_penalties_without_a_reciprocal_are_refused(dev):
             OF.process_logits(x, tokens, repetition_penalty=rep)
     got = OF.process_logits(x, tokens, repetition_penalty=2.0 ** 126)  # a power of two: exact
     assert torch.equal(got, (x.double() / 2.0 ** 126).float())
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_logits_refuse_an_output_that_overlaps_them_or_itself(dev):
+    torch.manual_seed(2)
+    buf = torch.randn(4, 200, device=dev)
+    x = buf[:, :100]
+    for out in (buf[:, 1:101], buf[:, 99:199], buf.view(-1)[300:700].view(4, 100),
+                torch.empty(1, 100, device=dev).expand(4, 100), torch.empty(4 * 50 + 50, device=dev).as_strided((4, 100), (50, 1))):
+        with pytest.raises(ValueError, match="out"):
+            OF.process_logits(x, out=out)
+    want = x.clone() + 1.0
+    bias = torch.ones(100, device=dev)
+    assert torch.equal(OF.process_logits(x, bias=bias, out=buf[:, 100:]), want)  # side by side in one buffer
+    got = OF.process_logits(x, bias=bias, out=x)
+    assert got.data_ptr() == x.data_ptr() and torch.equal(x, want)
+    one = torch.randn(1, 100, device=dev)
+    want = one + 1.0
+    assert torch.equal(OF.process_logits(one, bias=bias, out=one), want)
+    rows = torch.randn(6, 40, device=dev)  # every second row, and the rows between
+    want = rows[::2] + 1.0
+    assert torch.equal(OF.process_logits(rows[::2], bias=bias[:40], out=rows[1::2]), want)
+    square = torch.randn(30, 30, device=dev)
+    want = square.t() + 1.0
+    assert torch.equal(OF.process_logits(square.t(), bias=bias[:30], out=square), want)  # columns are copied first
+    same = torch.randn(1, 40, device=dev).expand(3, 40)
+    assert torch.equal(OF.process_logits(same, bias=bias[:40], out=torch.empty(3, 40, device=dev)), same + 1.0)
+    with pytest.raises(ValueError, match="out"):
+        OF.process_logits(rows[:3], out=rows[1:4])
