@@ -186,7 +186,7 @@ def _reference(logits, tokens, token_lengths, prompt_lengths, rep, pres, freq, b
     x = logits.float()
     rows, v = x.shape
     col = lambda p: p[:, None] if isinstance(p, torch.Tensor) else p
-    if tokens is not None and tokens.shape[1]:
+    if tokens is not None and tokens.shape[1] and v:
         t = torch.arange(tokens.shape[1], device=x.device)
         known = (tokens >= 0) & (tokens < v)
         if token_lengths is not None:

@@ -324,3 +324,10 @@ def test_logits_refuse_an_output_that_overlaps_them_or_itself(dev):
     assert torch.equal(OF.process_logits(same, bias=bias[:40], out=torch.empty(3, 40, device=dev)), same + 1.0)
     with pytest.raises(ValueError, match="out"):
         OF.process_logits(rows[:3], out=rows[1:4])
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_logits_of_nothing(dev):
+    tokens = torch.tensor([[3, 5], [0, -1]], device=dev)
+    assert OF.process_logits(torch.empty(2, 0, device=dev), tokens, repetition_penalty=1.5).shape == (2, 0)
+    assert OF.process_logits(torch.empty(0, 9, device=dev), tokens[:0], repetition_penalty=1.5).shape == (0, 9)
