@@ -36,6 +36,13 @@ class _Request:
     t0: float = 0.0
 
 
+def _frozen(x):
+    """Settings as a key: lists, tuples and dicts by their contents."""
+    if isinstance(x, dict):
+        return tuple(sorted((str(k), _frozen(v)) for k, v in x.items()))
+    return tuple(map(_frozen, x)) if isinstance(x, (list, tuple)) else x
+
+
 class DynamicBatcher:
     """Groups queued requests into batches and runs them through ``generate_fn(ids [b, s], **params) -> [b, s + new]``."""
 
@@ -85,8 +92,13 @@ class DynamicBatcher:
             groups: Dict[Any, List[_Request]] = {}
             for r in window:
                 mixed = self.ragged and r.params.get("paged_cache") and not r.params.get("no_repeat_ngram_size")
-                groups.setdefault((None if mixed else len(r.input_ids), tuple(sorted(r.params.items()))), []).append(r)
-            for (_, _), reqs in groups.items():
+                try:
+                    key = None if mixed else len(r.input_ids), _frozen(r.params)
+                    hash(key)
+                except TypeError:  # a setting that cannot be compared: the request runs alone
+                    key = id(r)
+                groups.setdefault(key, []).append(r)
+            for reqs in groups.values():
                 await self._run(reqs)
 
     async def _run(self, reqs: List[_Request]):
