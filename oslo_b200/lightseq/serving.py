@@ -139,8 +139,13 @@ def create_app(model, tokenizer=None, device=None, max_batch: int = 8, max_wait_
 
     def settings(given: Dict[str, Any]) -> Dict[str, Any]:
         params = {k: v for k, v in given.items() if k in allowed}
-        if isinstance(params.get("logit_bias"), dict):  # hashable, so that requests with the same biases share a batch
-            params["logit_bias"] = tuple(sorted((int(k), float(v)) for k, v in params["logit_bias"].items()))
+        if params.get("logit_bias") is not None:  # one form, so that requests with the same biases share a batch
+            bias = params["logit_bias"]
+            try:
+                pairs = dict(bias.items() if isinstance(bias, dict) else bias)
+                params["logit_bias"] = tuple(sorted((int(k), float(v)) for k, v in pairs.items()))
+            except (TypeError, ValueError) as e:
+                raise HTTPException(status_code=422, detail=f"logit_bias is {{token: value}} or [[token, value], ...]: {e}")
         return params
 
     def run(ids, **params):

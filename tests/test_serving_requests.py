@@ -41,3 +41,48 @@ def test_settings_that_are_lists_do_not_stop_the_batcher():
     assert out[3] == ([7, 8, 9, 9, 9], 1)
     assert out[1][0][:2] == [3, 4] and len(out[1][0]) == 5
     assert isinstance(out[4], Exception) and sorted(calls) == [(1, 2)] * 3 + [(2, 2)]
+
+
+def test_biases_over_http():
+    testclient = pytest.importorskip("fastapi.testclient")
+    from oslo_b200.lightseq.serving import create_app
+
+    try:
+        client = testclient.TestClient(create_app(_gpt2(), max_wait_ms=1.0))
+    except RuntimeError as e:  # the test client needs a package that the server does not
+        pytest.skip(str(e))
+    with client:
+        _ask(lambda body: (lambda r: (r.status_code, r.json()))(client.post("/generate", json=body)))
+
+
+def test_biases_of_requests():
+    """The same through the application's own handlers."""
+    fastapi = pytest.importorskip("fastapi")
+    from oslo_b200.lightseq.serving import create_app
+
+    app = create_app(_gpt2(), max_wait_ms=1.0)
+    handler = next(r.endpoint for r in app.routes if getattr(r, "path", "") == "/generate")
+
+    async def one(body):
+        try:
+            return 200, await asyncio.wait_for(handler(body), 60)
+        except fastapi.HTTPException as e:
+            return e.status_code, e.detail
+        finally:
+            await app.state.batcher.stop()
+            app.state.batcher.queue = None
+
+    _ask(lambda body: asyncio.run(one(body)))
+
+
+def _ask(post):
+    ids = dict(input_ids=[[1, 2]], max_new_tokens=3)
+    for bias in ([[9, 1e4]], {"9": 1e4}, [["9", "1e4"]], [[9, -5.0], [9, 1e4]]):
+        status, body = post(dict(ids, logit_bias=bias))
+        assert status == 200 and body["output_ids"] == [[1, 2, 9, 9, 9]], (bias, body)
+    plain = post(ids)[1]["output_ids"]
+    assert post(dict(ids, logit_bias=None))[1]["output_ids"] == post(dict(ids, logit_bias=[]))[1]["output_ids"] == plain
+    for bias in (7, [1, 2], [[1, 2, 3]], {"a": 1}, {"1": "x"}, [[[1], 2]], "ab", True):
+        status, body = post(dict(ids, logit_bias=bias))
+        assert status == 422, (bias, status, body)
+    assert post(ids)[1]["output_ids"] == plain
