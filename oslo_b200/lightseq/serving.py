@@ -104,10 +104,10 @@ class DynamicBatcher:
     async def _run(self, reqs: List[_Request]):
         lengths = [len(r.input_ids) for r in reqs]
         width, params = max(lengths), dict(reqs[0].params)
-        ids = torch.tensor([r.input_ids + [0] * (width - n) for r, n in zip(reqs, lengths)], dtype=torch.long)
         if min(lengths) < width:
             params["prompt_lengths"] = lengths
         try:
+            ids = torch.tensor([r.input_ids + [0] * (width - n) for r, n in zip(reqs, lengths)], dtype=torch.long)
             out = await asyncio.get_running_loop().run_in_executor(None, lambda: self.generate_fn(ids, **params))
             rows = [row[: len(row) - width + n] for row, n in zip(out.tolist(), lengths)]
             now = time.perf_counter()
@@ -119,6 +119,10 @@ class DynamicBatcher:
                 if not r.future.done():
                     r.future.set_result((row, len(reqs)))
         except Exception as e:  # noqa: BLE001 - the error goes to every caller of the batch
+            if min(lengths) < width:  # unless lengths share it: an empty or too long prompt is not the others' fault
+                for n in sorted(set(lengths)):
+                    await self._run([r for r in reqs if len(r.input_ids) == n])
+                return
             for r in reqs:
                 if not r.future.done():
                     r.future.set_exception(e)

@@ -86,3 +86,15 @@ def _ask(post):
         status, body = post(dict(ids, logit_bias=bias))
         assert status == 422, (bias, status, body)
     assert post(ids)[1]["output_ids"] == plain
+
+
+def test_a_refused_prompt_does_not_take_others_along():
+    paged = dict(paged_cache=True)
+    alone = {n: generate(_gpt2(), torch.arange(1, n + 1)[None], max_new_tokens=3)[0].tolist() for n in (2, 3)}
+    # empty; longer than the model's positions; not numbers
+    for bad in ([], list(range(1, 40)), ["x", "y", "z", "w"]):
+        out, _ = _batch([([1, 2, 3], paged), (bad, paged), ([1, 2], paged), ([1, 2, 3], paged)], ragged=True)
+        assert isinstance(out[1], Exception), bad
+        assert [out[i][0] for i in (0, 2, 3)] == [alone[3], alone[2], alone[3]]
+    out, calls = _batch([([1, 2, 3], paged), ([1, 2], paged)], ragged=True)  # together as ever
+    assert [r for r, n in out] == [alone[3], alone[2]] and calls == [(2, 3)]
