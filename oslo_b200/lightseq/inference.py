@@ -81,10 +81,17 @@ def _filter(logits, top_k: int, top_p: float):
 class _LogitsRules:
     """The penalties, biases and grammar of one generation, applied to the next-token logits of a step."""
 
-    def __init__(self, repetition_penalty, presence_penalty, frequency_penalty, logit_bias, allowed_tokens):
+    def __init__(self, repetition_penalty, presence_penalty, frequency_penalty, logit_bias, allowed_tokens, beams=1):
+        self.beams, self.spread = beams, False
         self.penalties = dict(repetition_penalty=repetition_penalty, presence_penalty=presence_penalty,
                               frequency_penalty=frequency_penalty)
-        self.counts = repetition_penalty != 1.0 or presence_penalty != 0.0 or frequency_penalty != 0.0
+        for name, p in self.penalties.items():  # one number a row
+            if isinstance(p, (list, tuple)):
+                self.penalties[name] = torch.tensor(p, dtype=torch.float32)
+        self.counts = any(isinstance(p, torch.Tensor) or p != none for p, none in zip(self.penalties.values(), (1.0, 0.0, 0.0)))
+        repetition = self.penalties["repetition_penalty"]
+        if not (bool((repetition > 0).all()) if isinstance(repetition, torch.Tensor) else repetition > 0):
+            raise ValueError(f"repetition_penalty is positive: got {repetition_penalty}")
         self.bias, self.allowed_tokens = logit_bias, allowed_tokens
         self.active = self.counts or logit_bias is not None or allowed_tokens is not None
 
@@ -108,7 +115,15 @@ class _LogitsRules:
             allowed = self.allowed_tokens(ids, lengths)
             if allowed is not None and allowed.dtype == torch.bool:
                 allowed = pack_token_mask(allowed)
-        history = dict(tokens=ids, token_lengths=lengths, prompt_lengths=prompts, **self.penalties) if self.counts else {}
+        history = {}
+        if self.counts:
+            for name, p in self.penalties.items():
+                if isinstance(p, torch.Tensor) and not self.spread:
+                    if p.shape != (rows // self.beams,):
+                        raise ValueError(f"{name} is a number or one number for each of {rows // self.beams} rows: got {tuple(p.shape)}")
+                    self.penalties[name] = p.to(logits.device).repeat_interleave(self.beams)  # a row's beams share its number
+            self.spread = True
+            history = dict(tokens=ids, token_lengths=lengths, prompt_lengths=prompts, **self.penalties)
         return process_logits(logits, bias=self.bias, allowed=allowed, **history)
 
 
@@ -117,18 +132,19 @@ def generate(model, input_ids: torch.Tensor, max_new_tokens: int = 32, do_sample
              top_p: float = 1.0, temperature: float = 1.0, num_beams: int = 1, no_repeat_ngram_size: int = 0,
              eos_token_id: Optional[int] = None, length_penalty: float = 1.0, pad_multiple: int = 1,
              use_cache: bool = True, paged_cache: bool = False, page_size: int = 64,
-             prompt_lengths: Optional[Sequence[int]] = None, repetition_penalty: float = 1.0, presence_penalty: float = 0.0,
-             frequency_penalty: float = 0.0, logit_bias: Union[None, torch.Tensor, Mapping, Sequence] = None,
-             allowed_tokens: Optional[Callable] = None):
+             prompt_lengths: Optional[Sequence[int]] = None, repetition_penalty: Union[float, torch.Tensor, Sequence] = 1.0,
+             presence_penalty: Union[float, torch.Tensor, Sequence] = 0.0, frequency_penalty: Union[float, torch.Tensor, Sequence] = 0.0,
+             logit_bias: Union[None, torch.Tensor, Mapping, Sequence] = None, allowed_tokens: Optional[Callable] = None):
     """Returns ``[batch, prompt + new]`` token ids (best beam when ``num_beams > 1``).  ``use_cache=False`` re-runs the
     whole prefix every step (the reference behaviour for models whose attention does not go through ``oslo_b200.ops``).
 
     ``paged_cache``: keep keys and values in pages of ``page_size`` tokens and attend with the paged kernel (no beams).  With it,
     ``prompt_lengths`` gives the number of tokens of each right-padded prompt; row ``i`` of the result is then its prompt,
     what was generated, and padding (``eos_token_id`` or 0).
-    ``repetition_penalty`` (of prompt and generated tokens), ``presence_penalty``, ``frequency_penalty`` (of generated tokens),
-    ``logit_bias`` (a tensor ``[vocab]``, a mapping or pairs token -> value) and ``allowed_tokens`` change the logits before
-    temperature and sampling (of beams: their log-probabilities), see :func:`oslo_b200.ops.logits.process_logits`.
+    ``repetition_penalty`` (of prompt and generated tokens), ``presence_penalty``, ``frequency_penalty`` (of generated tokens;
+    each is a number or one number a row), ``logit_bias`` (a tensor ``[vocab]``, a mapping or pairs token -> value) and
+    ``allowed_tokens`` change the logits before temperature and sampling (of beams: their log-probabilities), see
+    :func:`oslo_b200.ops.logits.process_logits`.
     ``allowed_tokens(ids, lengths)`` is called every step with the tokens so far (``lengths``: int32 ``[rows]`` of those that
     count, ``None``: all) and returns ``[rows, vocab]`` booleans, packed words, or ``None`` for no restriction."""
     if paged_cache and not use_cache:
@@ -137,9 +153,7 @@ def generate(model, input_ids: torch.Tensor, max_new_tokens: int = 32, do_sample
         raise ValueError("the paged cache does not follow beams: use the dense cache for num_beams > 1")
     if prompt_lengths is not None and not paged_cache:
         raise ValueError("prompts of different lengths need paged_cache=True")
-    if repetition_penalty <= 0:
-        raise ValueError(f"repetition_penalty is positive: got {repetition_penalty}")
-    rules = _LogitsRules(repetition_penalty, presence_penalty, frequency_penalty, logit_bias, allowed_tokens)
+    rules = _LogitsRules(repetition_penalty, presence_penalty, frequency_penalty, logit_bias, allowed_tokens, num_beams)
     model.eval()
     pc = getattr(model, "parallel_context", None)
     if num_beams > 1 and use_cache and pc is not None and getattr(pc, "tensor_parallel_size", 1) > 1:
