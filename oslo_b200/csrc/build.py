@@ -1,6 +1,6 @@
 """In-tree build of the native libraries.
 
-Two shared objects are produced next to this file's package:
+Three shared objects are produced next to this file's package:
 
 * ``oslo_b200/_lib/liboslo_b200_cuda.so``  every ``csrc/*.cu`` compiled by nvcc for
   ``sm_100a`` only (``-gencode arch=compute_100a,code=sm_100a``); plain
@@ -8,7 +8,7 @@ Two shared objects are produced next to this file's package:
   Python through ``ctypes`` (no libtorch dependency, so a rebuild takes seconds).
 * ``oslo_b200/_lib/liboslo_b200_cpu.so``   ``csrc/cpu/*.cpp`` compiled by g++ with
   AVX-512/AVX2 + OpenMP (CPU Adam / Adagrad, memory planner, partitioner core).
-* ``oslo_b200/_lib/_oslo_b200_step.so``  ``csrc/torch/*.cpp`` against the installed PyTorch: a Python module that calls
+* ``oslo_b200/_lib/_oslo_b200_step_*.so``  ``csrc/torch/*.cpp`` against the installed PyTorch: a Python module that calls
   the decoding step's entry points of the CUDA library without Python's per-argument cost (optional: the same calls go
   through ``ctypes`` without it).
 
@@ -110,36 +110,60 @@ def build_cpu() -> Path:
     return out
 
 
+def _step_flags():
+    import torch
+
+    return ["-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+
+
+def step_path() -> Path:
+    """Where the module of ``csrc/torch`` is for this PyTorch, this interpreter and these sources: one that was built for others has
+    another name, so it is never loaded."""
+    import torch
+
+    h = hashlib.sha1()
+    for src in (CSRC / "torch" / "step_calls.cpp", CSRC / "step_args.h"):
+        h.update(src.read_bytes())
+    h.update(" ".join([*_step_flags(), torch.__version__, sys.version]).encode())
+    return LIB_DIR / f"_oslo_b200_step_{h.hexdigest()[:12]}.so"
+
+
 def build_step() -> Path:
     """The module of ``csrc/torch``, compiled against this interpreter's PyTorch."""
     import sysconfig
 
-    import torch
     from torch.utils.cpp_extension import include_paths, library_paths
 
-    OBJ_DIR.mkdir(parents=True, exist_ok=True)
-    src, out, stamp_file = CSRC / "torch" / "step_calls.cpp", LIB_DIR / "_oslo_b200_step.so", OBJ_DIR / "step_calls.stamp"
-    flags = ["-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
-    stamp = _stamp(src, flags + [torch.__version__, sys.version])
-    if out.exists() and stamp_file.exists() and stamp_file.read_text() == stamp:
+    out = step_path()
+    if out.exists():
         return out
-    cmd = ["g++", *flags]
-    for path in [*include_paths(device_type="cuda"), sysconfig.get_paths()["include"]]:
+    LIB_DIR.mkdir(parents=True, exist_ok=True)
+    try:
+        headers = include_paths(device_type="cuda")
+    except TypeError:  # the argument's older name
+        headers = include_paths(cuda=True)
+    part = out.with_name(f"{out.name}.{os.getpid()}")  # processes that build at once do not see each other's half
+    cmd = ["g++", *_step_flags()]
+    for path in [*headers, sysconfig.get_paths()["include"]]:
         cmd += ["-isystem", path]
-    cmd += [str(src), "-o", str(out)]
+    cmd += [str(CSRC / "torch" / "step_calls.cpp"), "-o", str(part)]
     for path in library_paths():
         cmd += [f"-L{path}", f"-Wl,-rpath,{path}"]
     cmd += ["-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
+        part.unlink(missing_ok=True)
         raise RuntimeError(f"g++ failed:\n{res.stdout}\n{res.stderr}")
-    stamp_file.write_text(stamp)
+    os.replace(part, out)
     return out
 
 
 def build_all(verbose: bool = False):
     built = build_cuda(verbose), build_cpu()
-    build_step()
+    try:
+        build_step()
+    except (RuntimeError, OSError) as e:  # the same calls go through ctypes without it
+        sys.stderr.write(f"[oslo_b200] the decoding step's module was not built: {e}\n")
     return built
 
 

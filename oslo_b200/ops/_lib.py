@@ -77,11 +77,11 @@ def _load_cuda_lib() -> ctypes.CDLL:
 def step_calls():
     """The module that launches a decoding step's kernels without Python's per-argument cost, bound to the kernel library, or
     ``None`` where it is not built for this PyTorch (the same kernels are then called through ``ctypes``)."""
-    path = _LIB_DIR / "_oslo_b200_step.so"
-    try:
-        if not path.exists() and os.environ.get("OSLO_B200_AUTOBUILD", "1") == "1":
-            from oslo_b200.csrc.build import build_step
+    from oslo_b200.csrc.build import build_step, step_path
 
+    try:
+        path = step_path()
+        if not path.exists() and os.environ.get("OSLO_B200_AUTOBUILD", "1") == "1":
             build_step()
         loader = importlib.machinery.ExtensionFileLoader("_oslo_b200_step", str(path))
         module = importlib.util.module_from_spec(importlib.util.spec_from_loader("_oslo_b200_step", loader))
