@@ -151,6 +151,101 @@ def test_many_light_tokens_behind_a_heavy_one(dtype, hq, n, batch, gap, masked):
     assert (off <= tol).all(), (off / tol).max().item()
 
 
+# ------------------------------------------------------------------------------------------------ attention: blocks of 64 rows
+SPLIT = [  # more than 32 rows of a key head, and many key heads
+    (5, 40, 2, 64, 16, [40, 5, 0, 17, 3, 90, 64, 65] * 5, 0),
+    (5, 40, 2, 128, 16, [40, 5, 0, 17, 3, 90, 64, 65] * 5, 9000),
+    (1, 70, 2, 256, 32, [40, 0, 1, 17, 63, 90, 64, 65] * 4, 9000),
+    (7, 12, 1, 96, 16, [70, 8, 0, 33] * 20, 0),
+]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("kind", ["none", "left", "lowest", "empty", "all-lowest", "bias"])
+@pytest.mark.parametrize("form", SPLIT)
+def test_blocks_of_64_rows_under_a_mask(dtype, kind, form):
+    q, kp, vp, table, lens = _form("cuda", dtype, form)
+    s, _, _, d, page, n, _ = form
+    b, low = len(n), torch.finfo(torch.float32).min
+    m = torch.zeros(b, 1, 1, max(n) + 3)
+    if kind == "left":
+        for r in range(b):
+            m[r, ..., : n[r] * (r % 4) // 4] = -math.inf
+    elif kind == "lowest":
+        m[::2, ..., 5:30] = low
+    elif kind == "empty":
+        m[1::3] = -math.inf
+        m[::3, ..., ::2] = -math.inf
+    elif kind == "all-lowest":
+        m[::2] = low
+    elif kind == "bias":
+        m = torch.randn(1, 1, 1, max(n) + 3)
+    m = None if kind == "none" else m.cuda()
+    got = OF.paged_attention(q, kp, vp, table, lens, mask=m)
+    _sync_status("cuda")
+    want, tol = _attend_exact(q, kp, vp, table, n, d ** -0.5, m)
+    assert ((got.double() - want).abs() <= tol).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("fill", [math.nan, math.inf])
+@pytest.mark.parametrize("form", SPLIT)
+def test_blocks_of_64_rows_do_not_look_behind_the_last_token(dtype, fill, form):
+    q, kp, vp, table, lens = _form("cuda", dtype, form)
+    s, _, _, d, page, n, _ = form
+    used = torch.zeros(kp.shape[0], page, dtype=torch.bool, device="cuda")
+    for r in range(len(n)):
+        t = torch.arange(n[r], device="cuda")
+        used[table[r].long()[t // page], t % page] = True
+    for pool in (kp, vp):
+        pool.masked_fill_(~used[:, None, :, None], fill)
+    got = OF.paged_attention(q, kp, vp, table, lens)
+    want, tol = _attend_exact(q, kp, vp, table, n, d ** -0.5, None)
+    assert ((got.double() - want).abs() <= tol).all()
+    # masked tokens may hold anything either
+    m = torch.zeros(len(n), 1, 1, max(n), device="cuda")
+    hidden = [0, 2, 30, max(n) - 1]
+    m[..., hidden] = -math.inf
+    want = OF.paged_attention(q, kp, vp, table, lens, mask=m)
+    for r in range(len(n)):
+        for t in hidden:
+            if t < n[r]:
+                kp[int(table[r, t // page]), :, t % page] = fill
+                vp[int(table[r, t // page]), :, t % page] = fill
+    assert torch.equal(OF.paged_attention(q, kp, vp, table, lens, mask=m), want)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("form", SPLIT)
+def test_blocks_of_64_rows_skip_and_report_bad_pages_and_lengths(dtype, form):
+    from oslo_b200.ops import _lib
+
+    q, kp, vp, table, lens = _form("cuda", dtype, form)
+    want = OF.paged_attention(q, kp, vp, table, lens)
+    _sync_status("cuda")
+    bad = table.clone()
+    bad[0, 1], bad[5, 0] = -1, kp.shape[0]
+    got = OF.paged_attention(q, kp, vp, bad, lens)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="paged cache"):
+        _lib.check_status()
+    same = [r for r in range(len(form[5])) if r not in (0, 5)]
+    assert torch.equal(got[same], want[same]) and torch.isfinite(got).all()
+    far = lens.clone()
+    far[0], far[7] = 2147483647, table.shape[1] * form[4] + 1
+    got = OF.paged_attention(q, kp, vp, table, far)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="paged cache"):
+        _lib.check_status()
+    same = [r for r in range(len(form[5])) if r not in (0, 7)]  # the blocks' shares follow the lengths: other sums of the same tokens
+    want, tol = _attend_exact(q[same], kp, vp, table[same], [form[5][r] for r in same], form[3] ** -0.5, None)
+    assert ((got[same].double() - want).abs() <= tol).all() and torch.isfinite(got).all()
+    _lib.check_status()
+
+
 # ------------------------------------------------------------------------------------------------ arguments without elements
 @pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("dtype", TYPES)
