@@ -246,6 +246,40 @@ def test_blocks_of_64_rows_skip_and_report_bad_pages_and_lengths(dtype, form):
     _lib.check_status()
 
 
+@gpu
+@pytest.mark.parametrize("s,hq,hkv,d,page,lens", [
+    (1, 4, 4, 128, 16, [1, 15, 16, 17, 0]), (1, 18, 2, 128, 64, [65, 200]), (1, 20, 1, 256, 32, [90]), (4, 6, 2, 64, 16, [4, 90, 3, 1, 0]),
+    (1, 3, 3, 136, 16, [50]), (1, 8, 8, 128, 64, [5000, 1, 0, 777, 63, 64, 65]), (1, 1, 1, 64, 16, [20001]), (6, 96, 6, 128, 32, [900, 33, 5, 6, 0]),
+])
+@pytest.mark.parametrize("masked", [False, True])
+def test_attention_in_32_bits_loses_no_bits(s, hq, hkv, d, page, lens, masked):
+    """32-bit inputs are multiplied and summed in 32 bits: d products, 2 d u of their magnitudes; scaling and mask 4 u of a score;
+    the exponential 2**-21; n weights and values, 2 (n + 16) u."""
+    torch.manual_seed(d + sum(lens))
+    kp, vp, table = _pool(lens, page, hkv, d, torch.float32, "cuda")
+    q = torch.randn(len(lens), s, hq, d, device="cuda")
+    m = torch.randn(len(lens), 1, 1, max(lens), device="cuda") if masked else None
+    got = OF.paged_attention(q, kp, vp, table, torch.tensor(lens, device="cuda", **I32), mask=m).view(len(lens), s, hkv, -1, d)
+    for r, n in enumerate(lens):
+        k, v = _seq(kp, table, r, n).double(), _seq(vp, table, r, n).double()
+        for i in range(s):
+            end = n - s + 1 + i
+            if end <= 0:
+                assert (got[r, i] == 0).all()
+                continue
+            for h in range(hkv):
+                qq, kk, vv = q[r, i].view(hkv, -1, d)[h].double(), k[:end, h], v[:end, h]
+                x = qq @ kk.T / math.sqrt(d)
+                e = 2 * d * U * (qq.abs() @ kk.abs().T / math.sqrt(d)) + 4 * U * x.abs()
+                if masked:
+                    x = x + m[r, 0, 0, :end].double()
+                    e = e + 4 * U * m[r, 0, 0, :end].abs()
+                p = torch.softmax(x, -1)
+                want = p @ vv
+                pre = (torch.expm1(2 * e.amax(-1, keepdim=True)) + 2.0 ** -21 + 2 * (end + 16) * U) * (p @ vv.abs())
+                assert ((got[r, i, h].double() - want).abs() <= pre + U * (want.abs() + pre)).all(), (r, i, h)
+
+
 # ------------------------------------------------------------------------------------------------ arguments without elements
 @pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("dtype", TYPES)
@@ -426,3 +460,68 @@ def test_logits_of_nothing(dev):
     tokens = torch.tensor([[3, 5], [0, -1]], device=dev)
     assert OF.process_logits(torch.empty(2, 0, device=dev), tokens, repetition_penalty=1.5).shape == (2, 0)
     assert OF.process_logits(torch.empty(0, 9, device=dev), tokens[:0], repetition_penalty=1.5).shape == (0, 9)
+
+
+# ------------------------------------------------------------------------------------------------ refusals, wherever the tensors are
+@pytest.mark.parametrize("dev", DEVICES)
+def test_refusals_of_the_cache_on_every_device(dev):
+    kp, vp, table = _pool([20, 20], 16, 2, 64, torch.float32, dev)
+    q, k, v = (torch.randn(2, 1, n, 64, device=dev) for n in (4, 2, 2))
+    lens = torch.tensor([3, 4], device=dev, **I32)
+    cos, sin = OF.rope_tables(64, 64, device=dev)
+    good = dict(k=k, v=v, k_pages=kp, v_pages=vp, block_table=table, start=lens, q=q, rope=(cos, sin, 64, True))
+    before = kp.clone(), vp.clone()
+    elsewhere = [dict(v=v.cpu()), dict(q=q.cpu()), dict(start=lens.cpu()), dict(count=lens.cpu()), dict(block_table=table.cpu()),
+                 dict(v_pages=vp.cpu()), dict(k_pages=kp.cpu()), dict(rope=(cos.cpu(), sin, 64, True)), dict(rope=(cos, sin.cpu(), 64, True))]
+    for change in (dict(k=k[:, :, :1]), dict(k=k.half()), dict(k=k.half(), v=v.half()), dict(v=v.double(), k=k.double()), dict(k=k[0]),
+                   dict(k_pages=kp[:, :, :8], v_pages=vp[:, :, :8]), dict(k_pages=kp[:-1]), dict(k_pages=kp.transpose(0, 1)),
+                   dict(k_pages=kp.transpose(2, 3).contiguous().transpose(2, 3)), dict(block_table=table.long()),
+                   dict(block_table=table[:1]), dict(block_table=table[0]), dict(start=lens.long()), dict(start=lens[:1]),
+                   dict(count=lens.long()), dict(count=lens[:1]), dict(q=q[:1]), dict(q=q.half()), dict(q=q[..., :32]),
+                   dict(rope=(cos.double(), sin.double(), 64, True)), dict(rope=(cos, sin, 66, True)), dict(rope=(cos, sin, 32, True)),
+                   dict(rope=(cos, sin, 3, True)), dict(rope=(cos, sin[:5], 64, True)), dict(rope=(cos, sin, -2, True)),
+                   dict(start=torch.stack([lens, lens], 1)[:, 0]),
+                   dict(block_table=torch.stack([table, table], 2)[..., 0]),
+                   *(elsewhere if dev == "cuda" else ())):
+        with pytest.raises(ValueError):
+            OF.paged_kv_append(**{**good, **change})
+    _sync_status(dev)
+    assert torch.equal(kp, before[0]) and torch.equal(vp, before[1])
+    OF.paged_kv_append(**good)
+    good = dict(q=q, k_pages=kp, v_pages=vp, block_table=table, lengths=lens)
+    OF.paged_attention(**good)
+    m = torch.zeros(2, 1, 1, 20, device=dev)
+    for change in (dict(q=q[0]), dict(q=q[:, :, :3]), dict(q=q.half()), dict(q=q[..., :32]), dict(lengths=lens.long()),
+                   dict(lengths=lens[:1]), dict(scale=math.nan), dict(scale=math.inf), dict(mask=m.expand(2, 4, 1, 20)),
+                   dict(mask=m.expand(2, 1, 2, 20)), dict(mask=m[0, 0]), dict(mask=m.bool()), dict(q=q[:, :, :0]), dict(block_table=table.float()),
+                   dict(lengths=torch.stack([lens, lens], 1)[:, 0]),
+                   *((dict(mask=m.cpu()), dict(lengths=lens.cpu()), dict(k_pages=kp.cpu()), dict(v_pages=vp.cpu())) if dev == "cuda" else ())):
+        with pytest.raises(ValueError):
+            OF.paged_attention(**{**good, **change})
+    big = torch.zeros(1, 1, 16, 264, device=dev)
+    with pytest.raises(ValueError, match="head_dim"):
+        OF.paged_attention(torch.zeros(1, 1, 1, 264, device=dev), big, big, table[:1], lens[:1])
+    _sync_status(dev)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_refusals_of_the_logits_on_every_device(dev):
+    x, tok = torch.randn(2, 50, device=dev), torch.zeros(2, 4, dtype=torch.int64, device=dev)
+    i32 = torch.tensor([1, 2], device=dev, **I32)
+    good = dict(logits=x, tokens=tok, repetition_penalty=1.1)
+    OF.process_logits(**good)
+    elsewhere = [dict(presence_penalty=torch.ones(2)), dict(bias=torch.zeros(50)), dict(allowed=torch.zeros(2, 2, **I32)),
+                 dict(out=torch.zeros(2, 50)), dict(tokens=tok.cpu()), dict(token_lengths=i32.cpu()), dict(prompt_lengths=i32.cpu())]
+    for change in (dict(logits=x[0]), dict(logits=x.double()), dict(tokens=tok[:1]), dict(tokens=tok.float()), dict(tokens=None),
+                   dict(token_lengths=i32.long()), dict(token_lengths=i32[:1]), dict(prompt_lengths=i32.float()),
+                   dict(repetition_penalty=0.0), dict(repetition_penalty=-1.0), dict(repetition_penalty=math.nan),
+                   dict(repetition_penalty=torch.ones(3, device=dev)), dict(frequency_penalty=torch.ones(2, 1, device=dev)),
+                   dict(presence_penalty=torch.ones(2, device=dev, dtype=torch.int64)),
+                   dict(bias=torch.zeros(49, device=dev)), dict(bias=torch.zeros(1, 50, device=dev)),
+                   dict(bias=torch.zeros(50, dtype=torch.int64, device=dev)),
+                   dict(allowed=torch.ones(2, 50, device=dev).bool()), dict(allowed=torch.zeros(2, 3, device=dev, **I32)),
+                   dict(allowed=torch.zeros(3, 2, device=dev, **I32)),
+                   dict(out=torch.zeros(2, 51, device=dev)), dict(out=torch.zeros(2, 50, device=dev).half()),
+                   dict(out=torch.zeros(50, 2, device=dev).t()), dict(tokens=None, token_lengths=i32), *(elsewhere if dev == "cuda" else ())):
+        with pytest.raises(ValueError):
+            OF.process_logits(**{**good, **change})
