@@ -7,8 +7,8 @@
 // Every logit is read once and written once.  A block owns a slice of one row's vocabulary and counts the history's tokens
 // of that slice in shared memory (integer atomics: their order does not matter), while its first logits are already on their
 // way; then it streams the slice, 16 bytes a thread.  Counters have 16 bits for histories of less than 32768 tokens: a group of
-// eight 16-bit logits then meets one 16-byte load of counters, most of them zero.  Plain streaming runs at the copy bandwidth
-// (192 x 250112 bf16: 35 us); with a history of 4095 tokens, a bias and a mask the same logits take 58 us, bound by
+// eight 16-bit logits then meets one 16-byte load of counters, most of them zero.  Plain streaming runs at 85 % of the copy
+// bandwidth (192 x 250112 bf16: 35 us); with a history of 4095 tokens, a bias and a mask the same logits take 58 us, bound by
 // issue and latency: the history is read by each of a row's 16 slices, the bias comes from L2 (as many bytes as the logits twice
 // over), and every element's mask is two instructions.  Adding a cluster's tokens to each other's counters through distributed
 // shared memory, so that a row reads its history once, was slower (105 us): frequent tokens serialise the remote atomics.
@@ -32,7 +32,7 @@ struct LogitsParams {
   const int* allowed;
   long long x_stride, y_stride, tok_stride, bias_stride, allowed_stride;
   float rep_s, pres_s, freq_s;
-  int rows, vocab, history, tok64, slice, slices;  // slices a row, a multiple of the cluster's size
+  int rows, vocab, history, tok64, slice, slices;  // tokens of a slice, slices of a row
 };
 
 constexpr int kLogitsThreads = 256;

@@ -5,7 +5,7 @@
 //
 // Every key and value is used by `group` query heads (times the new tokens) only, so HBM bounds it: 4 * head_dim bytes a token and
 // key head against 4 * group * head_dim operations.  Measured: 64 sequences of up to 6000 tokens, 32 key heads of 128, 5.48 GB in
-// 903 us (94% of the copy bandwidth); one sequence of 131071 tokens, 8 key heads, 98 us (85%: SMs are served unevenly, the
+// 907 us (94% of the copy bandwidth); one sequence of 131071 tokens, 8 key heads, 100 us (83%: SMs are served unevenly, the
 // last block ends 7 us after the mean, and the joining launch follows).
 //
 // Work is cut into units of 64 tokens (32 for fp32) of one (sequence, key head, block of query rows), a "segment" being all
@@ -26,8 +26,12 @@
 // (Rows of the ring are 16 bytes longer than a head, which keeps the value loads free of bank conflicts.)  tcgen05 would
 // multiply 128 rows where there are 1 to 16: the tensor cores are not what bounds this.
 // The weights enter the second product as the sum of two 16-bit numbers (high part and remainder): 16 bits of a weight in bf16, 22
-// in fp16.  fp16 ends at 2^-24, so its weights and their sum carry a factor of 2^15, which the last division takes out: a token
-// that weighs 2^-25 of the heaviest keeps 14 bits, and no weight loses more than 2^-22 of itself or 2^-40 of the heaviest.
+// in fp16.  In bf16 that is hidden by the result's own rounding: of 64 x 6000 tokens' results 24 in 10000 are the neighbour of the
+// nearest bf16 number, 7 in 10000 with 32-bit weights; a third part would cost half the product again.  fp16 ends at 2^-24, so its
+// weights and their sum carry a factor of 2^15, which the last division takes out: a token that weighs 2^-25 of the heaviest keeps
+// 14 bits, and no weight loses more than 2^-22 of itself or 2^-40 of the heaviest.
+// An infinite value times such a pair would be NaN, and so would a value that is not finite times the weight zero of a row that does
+// not see it: blocks whose sums are not finite walk over their tokens once more, with care (see CAREFUL).
 #pragma once
 #include "common.cuh"
 
@@ -1184,10 +1188,6 @@ struct PagedAttnLaunch {
     return cudaLaunchKernelEx(&cfg, paged_attention_join_kernel<T, DP, WIDE, MASK, SPLIT>, p) == cudaSuccess ? 0 : -2;
   }
 };
-
-// Whether a block takes 16 query rows instead of 8.  32-bit rows of 256 dims do not fit the registers twice: 24 rows took 1297 us
-// in two blocks' worth of 16 and 671 us in three of 8.
-inline bool paged_attention_wide(int dtype, int d, int rows) { return rows > 8 && !(dtype == 0 && d > 128); }
 
 // How a call's query rows are dealt to blocks: up to 8 a block, up to 16, or 16 to each of the four warps.  64 rows read a key once
 // instead of four times but cut the work into fewer pieces, so they pay where `groups` (sequences x key heads) are many: 49 x 12
