@@ -37,10 +37,24 @@ class _Request:
 
 
 def _frozen(x):
-    """Settings as a key: lists, tuples and dicts by their contents."""
+    """A setting as a key: lists, tuples and dicts by their contents."""
     if isinstance(x, dict):
         return tuple(sorted((str(k), _frozen(v)) for k, v in x.items()))
     return tuple(map(_frozen, x)) if isinstance(x, (list, tuple)) else x
+
+
+def _group_key(r: "_Request", ragged: bool):
+    """What requests of one batch have in common.  Biases are one setting for all rows of a batch; any other list or tensor would
+    have a number for each of them, so a request with one runs alone, as does one whose settings cannot be compared."""
+    mixed = ragged and r.params.get("paged_cache") and not r.params.get("no_repeat_ngram_size")
+    if any(isinstance(v, (list, tuple, dict, torch.Tensor)) for k, v in r.params.items() if k != "logit_bias"):
+        return id(r)
+    try:
+        key = None if mixed else len(r.input_ids), _frozen(r.params)
+        hash(key)
+        return key
+    except TypeError:
+        return id(r)
 
 
 class DynamicBatcher:
@@ -91,13 +105,7 @@ class DynamicBatcher:
                     break
             groups: Dict[Any, List[_Request]] = {}
             for r in window:
-                mixed = self.ragged and r.params.get("paged_cache") and not r.params.get("no_repeat_ngram_size")
-                try:
-                    key = None if mixed else len(r.input_ids), _frozen(r.params)
-                    hash(key)
-                except TypeError:  # a setting that cannot be compared: the request runs alone
-                    key = id(r)
-                groups.setdefault(key, []).append(r)
+                groups.setdefault(_group_key(r, self.ragged), []).append(r)
             for reqs in groups.values():
                 await self._run(reqs)
 
@@ -143,6 +151,9 @@ def create_app(model, tokenizer=None, device=None, max_batch: int = 8, max_wait_
 
     def settings(given: Dict[str, Any]) -> Dict[str, Any]:
         params = {k: v for k, v in given.items() if k in allowed}
+        for name in ("repetition_penalty", "presence_penalty", "frequency_penalty"):
+            if not isinstance(params.get(name, 0.0), (int, float)):
+                raise HTTPException(status_code=422, detail=f"{name} is a number: got {params[name]!r}")
         if params.get("logit_bias") is not None:  # one form, so that requests with the same biases share a batch
             bias = params["logit_bias"]
             try:

@@ -8,8 +8,9 @@ Keys and values live in pools ``[pages, kv_heads, page_size, head_dim]``; ``bloc
 ``PagedDecodeCache``  the paged counterpart of :class:`oslo_b200.ops.attention.DecodeCache`: pages are taken from a free list as
                       sequences grow, and the sequences of a batch may have different lengths
 
-The functions are for inference: inputs that require a gradient or carry a forward derivative are refused.  On the GPU a page, position or length outside
-its pool or table is skipped by the kernel and reported by ``oslo_b200.ops._lib.check_status()``; on the CPU it raises.
+The functions are for inference: inputs that require a gradient or carry a forward derivative are refused.  On the GPU a page,
+position or length outside its pool or table is skipped by the kernel and reported by ``oslo_b200.ops._lib.check_status()``; on the
+CPU it raises.
 """
 from __future__ import annotations
 

@@ -57,6 +57,10 @@ def test_biases_over_http():
 
 def test_biases_of_requests():
     """The same through the application's own handlers."""
+    _through_the_handlers(_ask)
+
+
+def _through_the_handlers(ask):
     fastapi = pytest.importorskip("fastapi")
     from oslo_b200.lightseq.serving import create_app
 
@@ -72,7 +76,7 @@ def test_biases_of_requests():
             await app.state.batcher.stop()
             app.state.batcher.queue = None
 
-    _ask(lambda body: asyncio.run(one(body)))
+    ask(lambda body: asyncio.run(one(body)))
 
 
 def _ask(post):
@@ -98,3 +102,22 @@ def test_a_refused_prompt_does_not_take_others_along():
         assert [out[i][0] for i in (0, 2, 3)] == [alone[3], alone[2], alone[3]]
     out, calls = _batch([([1, 2, 3], paged), ([1, 2], paged)], ragged=True)  # together as ever
     assert [r for r, n in out] == [alone[3], alone[2]] and calls == [(2, 3)]
+
+
+def test_numbers_for_rows_do_not_meet_in_a_batch():
+    """A list of penalties belongs to the rows of its own request, whatever shares the window."""
+    pen = lambda x: dict(presence_penalty=x)
+    requests = [([1, 2], pen([1e4])), ([1, 2], pen([1e4])), ([1, 2], pen((1e4,))), ([1, 2], pen((1e4,))), ([1, 2], pen([1e4, 0.0]))]
+    out, calls = _batch(requests)
+    want = generate(_gpt2(), torch.tensor([[1, 2]]), max_new_tokens=3, presence_penalty=1e4)[0].tolist()
+    assert all(r == (want, 1) for r in out[:4]) and isinstance(out[4], ValueError) and calls == [(1, 2)] * 5
+
+
+def test_penalties_over_http_are_numbers():
+    def ask(post):
+        ids = dict(input_ids=[[1, 2], [3, 4]], max_new_tokens=2)
+        assert post(dict(ids, presence_penalty=1, repetition_penalty=1.5))[0] == 200
+        for bad in ([1.0, 2.0], "1", None):
+            assert post(dict(ids, presence_penalty=bad))[0] == 422, bad
+
+    _through_the_handlers(ask)
