@@ -23,7 +23,7 @@ struct PagedAppendParams {
   const int* table;
   const int* start;
   const int* count;  // null: all s tokens are real
-  const float* cosb;  // [positions, rot / 2]; rot = 0: no rotation
+  const float* cosb;  // [positions, rot / 2]; null: no rotation
   const float* sinb;
   int* status;
   long long q_sb, q_ss, q_sh, k_sb, k_ss, k_sh, v_sb, v_ss, v_sh;  // element strides of batch, token, head
@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(kAppendThreads, MODE == kRotateElements ? 12 :
   const T* k = static_cast<const T*>(p.k) + b * p.k_sb + i * p.k_ss;
   const T* v = static_cast<const T*>(p.v) + b * p.v_sb + i * p.v_ss;
   T* q_out = static_cast<T*>(p.q_out) + static_cast<long long>(token) * p.hq * p.d;
-  const int rot = p.rot, rows = p.hq + p.hkv;
+  const int rot = p.cosb != nullptr ? p.rot : 0, rows = p.hq + p.hkv;
   const auto source = [&](int r) { return r < p.hq ? q + r * p.q_sh : k + (r - p.hq) * p.k_sh; };
 
   const int columns = H::columns(p.d, rot), r0 = threadIdx.x / columns, c = threadIdx.x - r0 * columns;
@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(kAppendThreads, MODE == kRotateElements ? 12 :
 template <typename T>
 int paged_append_launch(const PagedAppendParams& p, cudaStream_t st) {
   constexpr int E = PagedVec<T>::E;
-  const int rot = p.rot;
+  const int rot = p.cosb ? p.rot : 0;
   int mode = kRotateInside;
   if (rot && p.neox) {
     const bool whole = rot % (2 * E) == 0 && ((reinterpret_cast<uintptr_t>(p.cosb) | reinterpret_cast<uintptr_t>(p.sinb)) & 15) == 0;
@@ -249,7 +249,9 @@ extern "C" int oslo_paged_kv_append(const OsloPagedAppendArgs* a) {
   p.q_out = reinterpret_cast<void*>(a->q_out), p.k_pages = reinterpret_cast<void*>(a->k_pages);
   p.v_pages = reinterpret_cast<void*>(a->v_pages), p.table = reinterpret_cast<const int*>(a->table);
   p.start = reinterpret_cast<const int*>(a->start), p.count = reinterpret_cast<const int*>(a->count);
-  p.cosb = reinterpret_cast<const float*>(a->cosb), p.sinb = reinterpret_cast<const float*>(a->sinb);
+  // tables without positions have no address: another one stands for them, nothing is read there
+  p.cosb = reinterpret_cast<const float*>(a->rot == 0 ? 0 : a->positions > 0 ? a->cosb : a->status);
+  p.sinb = reinterpret_cast<const float*>(a->rot == 0 ? 0 : a->positions > 0 ? a->sinb : a->status);
   p.status = reinterpret_cast<int*>(a->status);
   p.q_sb = a->q_b, p.q_ss = a->q_s, p.q_sh = a->q_h, p.k_sb = a->k_b, p.k_ss = a->k_s, p.k_sh = a->k_h;
   p.v_sb = a->v_b, p.v_ss = a->v_s, p.v_sh = a->v_h;
